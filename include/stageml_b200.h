@@ -67,7 +67,8 @@ enum {
 const char* stageml_last_error(void);
 /* ABI version of this library (bumped on any signature or struct change). */
 int stageml_abi_version(void);
-/* sizeof() of the public structs, so bindings can check their mirrors. 0 = plan, 1 = moe args, 2 = lora linear args. */
+/* sizeof() of the public structs, so bindings can check their mirrors. 0 = plan, 1 = moe args, 2 = lora linear args,
+ * 3 = ep layout, 4 = ep args, 5 = moe blocks args, 6 = norm args. */
 size_t stageml_struct_size(int which);
 
 /* Per-stage device timing (benchmark support; no counterpart in the reference,
@@ -360,6 +361,122 @@ int stageml_lora_gemv_f32_noalloc(const float* x, const float* W, const float* A
  * with round-to-nearest-even and saturation to +-448. Input F32/BF16/F16. */
 int stageml_quantize_e4m3_rows(const void* w, int dtype, int64_t rows, int64_t cols, uint8_t* q_out,
                                float* scale_out, stageml_stream_t stream);
+
+/* ------------------------------------------------- block-scaled FP8 operands
+ * No counterpart in the reference, which has no FP8 path. e4m3 codes with one fp32
+ * scale per block: 1 x 128 values of a row (activations) or a 128 x 128 tile of a
+ * matrix (weights). The last block of a row or column may be short.
+ *   scale = max|x| / 448 over the block (1 where that is 0), q = e4m3(x / scale),
+ * correctly rounded division, round-to-nearest-even, saturated to +-448. A NaN or
+ * infinity in a block makes its scale a NaN or infinity.
+ * x [batch, rows, cols] F32/BF16/F16; q the same shape; scale [batch, rows, ceil(cols/128)]
+ * (tiles == 0) or [batch, ceil(rows/128), ceil(cols/128)] (tiles == 1). */
+int stageml_quantize_e4m3_blocks(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int tiles,
+                                 uint8_t* q_out, float* scale_out, stageml_stream_t stream);
+
+/* out[m, n] = sum_kb x_scale[m, kb] * w_scale[n / 128, kb] * sum_{k in block kb} x[m, k] * w[n, k]
+ * x [M, K] e4m3, x_scale [M, ceil(K/128)]; w [N, K] e4m3, w_scale [ceil(N/128), ceil(K/128)];
+ * out [M, N] F32/BF16/F16, fp32 sums rounded once. K a multiple of 16 (16-byte rows), any M, N.
+ * The workspace holds the partial sums of calls with few rows, whose K is split over CTAs. */
+size_t stageml_block_matmul_workspace_bytes(int M, int N, int K);
+int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int M, int N,
+                         int K, int out_dtype, void* out, int32_t* status, void* workspace, size_t workspace_bytes,
+                         stageml_stream_t stream);
+
+/* The routed SwiGLU feed-forward layer on block-scaled weights (the computation of
+ * stageml_moe_forward without LoRA, with both products on e4m3 operands):
+ *   out[t] = sum_j w[t,j] * W2_e . Q( silu(W1_e . Q(x_t)) * (W3_e . Q(x_t)) ),  e = ids[t, j],
+ * plus the n_shared always-on experts (index E + i, weight 1). Q(v) is v as its e4m3 codes
+ * and 1 x 128 scales hold it; the products sum in fp32, and a routed row leaves the down
+ * projection in the activation dtype, weighted, before the fp32 sum over a token's slots.
+ * gate_up [E_tot, 2I, H] e4m3 (rows [0, I) = W1, [I, 2I) = W3), gate_up_scale
+ * [E_tot, ceil(2I/128), ceil(H/128)]; down [E_tot, H, I], down_scale [E_tot, ceil(H/128),
+ * ceil(I/128)], E_tot = E + n_shared. H and I are multiples of 16. An id outside [0, E) drops
+ * its slot (STAGEML_DEV_BAD_INDEX). */
+typedef struct stageml_moe_blocks_args {
+  int T, H, I, E, k, n_shared;
+  int act_dtype;            /* BF16 or F16: x and out */
+  const void* x;            /* [T, H] */
+  const void* topk_ids;     /* [T, k] I32/I64 */
+  int ids_dtype;
+  const void* topk_weights; /* [T, k] F32/BF16/F16, used as given */
+  int weights_dtype;
+  const uint8_t* gate_up;
+  const float* gate_up_scale;
+  const uint8_t* down;
+  const float* down_scale;
+  void* out;                /* [T, H] */
+  int32_t* status;          /* device status word, may be NULL */
+} stageml_moe_blocks_args;
+
+size_t stageml_moe_blocks_workspace_bytes(const stageml_moe_blocks_args* args);
+int stageml_moe_forward_blocks(const stageml_moe_blocks_args* args, void* workspace, size_t workspace_bytes,
+                               stageml_stream_t stream);
+
+/* ------------------------------------------- norms around a block, gate, residual
+ * No counterpart in the reference (its layers stop at the MoE output).
+ *   u  = post_weight * y * rsqrt(mean(y^2) + eps)   (u = y without post_weight)
+ *   r' = residual_scale * r + gate * u              (residual_scale * r without block_out)
+ *   z  = pre_weight * r' * rsqrt(mean(r'^2) + eps)  (no z without pre_weight)
+ * y = block_out, r = residual. fp32 arithmetic, one rounding per output; z comes from the
+ * unrounded r'. With `codes` set, z leaves as e4m3 codes [T, H] and code_scale
+ * [T, ceil(H/128)] (stageml_quantize_e4m3_blocks of the fp32 z) instead of `normed`.
+ * The backward call takes the forward's inputs again (nothing else is saved) with the
+ * gradients of r' and z (either may be NULL = zero) and writes the gradients of every
+ * input that is present; the weights' and the gate's in their own dtype. H <= 16384. */
+enum { STAGEML_GATE_NONE = 0, STAGEML_GATE_CHANNEL = 1, STAGEML_GATE_TOKEN = 2, STAGEML_GATE_FULL = 3 };
+typedef struct stageml_norm_args {
+  int64_t T;
+  int H;
+  int resid_dtype;          /* F32, BF16 or F16: residual, new_residual and their gradients */
+  int block_dtype;          /* block_out, normed and their gradients; equals resid_dtype unless that is F32 */
+  const void* residual;     /* [T, H] */
+  const void* block_out;    /* [T, H] or NULL */
+  const void* post_weight;  /* [H] or NULL */
+  int post_dtype;           /* F32, BF16 or F16, as gate_dtype and pre_dtype */
+  const void* gate;         /* [H] (CHANNEL), [T] (TOKEN) or [T, H] (FULL) */
+  int gate_mode;
+  int gate_dtype;
+  const void* pre_weight;   /* [H] or NULL */
+  int pre_dtype;
+  float residual_scale;
+  float eps;
+  void* new_residual;       /* forward: [T, H] */
+  void* normed;             /* forward: [T, H], with pre_weight and without codes */
+  uint8_t* codes;
+  float* code_scale;
+  const void* grad_residual; /* backward: gradient of new_residual or NULL */
+  const void* grad_normed;   /* backward: gradient of normed or NULL */
+  void* d_residual;
+  void* d_block_out;
+  void* d_post;
+  void* d_gate;
+  void* d_pre;
+} stageml_norm_args;
+
+size_t stageml_norm_residual_workspace_bytes(const stageml_norm_args* args, int backward);
+int stageml_norm_residual(const stageml_norm_args* args, void* workspace, size_t workspace_bytes,
+                          stageml_stream_t stream);
+int stageml_norm_residual_backward(const stageml_norm_args* args, void* workspace, size_t workspace_bytes,
+                                   stageml_stream_t stream);
+
+/* ------------------------------------------------------ router balance loss
+ * No counterpart in the reference (its routers are not trained).
+ *   p[t, :] = softmax(logits[t, :]), n = number of tokens with valid[t] (all without `valid`)
+ *   counts[e] = slots (t, j) of those tokens with ids[t, j] = e;  f[e] = counts[e] / (n k)
+ *   loss = coefficient * E * sum_e f[e] * (1/n) sum_t p[t, e]
+ * logits [T, E] F32/BF16/F16, ids [T, k] I32/I64 (negative: no expert; >= E: skipped with
+ * STAGEML_DEV_BAD_INDEX), valid [T] bytes or NULL. Writes loss [1] fp32, counts [E] and
+ * tokens [1] = n, int32. The backward call writes the gradient of logits for a given
+ * gradient of the loss (device fp32 [1]); counts carry none. E <= 256, k <= 8. A token whose
+ * logits are all -infinity adds nothing and gets gradient 0. */
+size_t stageml_balance_workspace_bytes(int64_t T, int E);
+int stageml_balance_loss(const void* logits, int logits_dtype, const void* ids, int ids_dtype, const uint8_t* valid,
+                         int64_t T, int E, int k, float coefficient, float* loss, int32_t* counts, int32_t* tokens,
+                         int32_t* status, void* workspace, size_t workspace_bytes, stageml_stream_t stream);
+int stageml_balance_loss_backward(const float* grad_loss, const void* logits, int logits_dtype, const int32_t* counts,
+                                  const int32_t* tokens, const uint8_t* valid, int64_t T, int E, int k,
+                                  float coefficient, void* grad_logits, stageml_stream_t stream);
 
 /* ------------------------------------------------------- expert parallel over peer memory
  * No counterpart in the reference, which has no distributed code: this is the

@@ -36,6 +36,11 @@ CU_SOURCES = [
     "fold.cu",
     "gemv.cu",
     "fp8.cu",
+    "quantize_blocks.cu",
+    "block_gemm.cu",
+    "block_norm.cu",
+    "balance.cu",
+    "block_capi.cu",
     "stage_timer.cu",
     "capi.cu",
 ]

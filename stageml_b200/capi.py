@@ -129,6 +129,43 @@ class EpArgs(ctypes.Structure):
     ]
 
 
+class MoeBlocksArgs(ctypes.Structure):
+    _fields_ = [(n, c_int) for n in ("T", "H", "I", "E", "k", "n_shared", "act_dtype")] + [
+        ("x", c_void_p),
+        ("topk_ids", c_void_p),
+        ("ids_dtype", c_int),
+        ("topk_weights", c_void_p),
+        ("weights_dtype", c_int),
+        ("gate_up", c_void_p),
+        ("gate_up_scale", c_void_p),
+        ("down", c_void_p),
+        ("down_scale", c_void_p),
+        ("out", c_void_p),
+        ("status", c_void_p),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [
+        ("T", c_int64),
+        ("H", c_int),
+        ("resid_dtype", c_int),
+        ("block_dtype", c_int),
+        ("residual", c_void_p),
+        ("block_out", c_void_p),
+        ("post_weight", c_void_p),
+        ("post_dtype", c_int),
+        ("gate", c_void_p),
+        ("gate_mode", c_int),
+        ("gate_dtype", c_int),
+        ("pre_weight", c_void_p),
+        ("pre_dtype", c_int),
+        ("residual_scale", c_float),
+        ("eps", c_float),
+    ] + [(n, c_void_p) for n in ("new_residual", "normed", "codes", "code_scale", "grad_residual", "grad_normed",
+                                  "d_residual", "d_block_out", "d_post", "d_gate", "d_pre")]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "stageml_last_error": (ctypes.c_char_p, []),
@@ -161,6 +198,21 @@ SIGNATURES = {
     "stageml_lora_gemv_f32_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_int,
                                               c_int, c_void_p, c_void_p]),
     "stageml_quantize_e4m3_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "stageml_quantize_e4m3_blocks": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                             c_void_p]),
+    "stageml_block_matmul_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "stageml_block_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                                     c_void_p, c_void_p, c_size_t, c_void_p]),
+    "stageml_moe_blocks_workspace_bytes": (c_size_t, [POINTER(MoeBlocksArgs)]),
+    "stageml_moe_forward_blocks": (c_int, [POINTER(MoeBlocksArgs), c_void_p, c_size_t, c_void_p]),
+    "stageml_norm_residual_workspace_bytes": (c_size_t, [POINTER(NormArgs), c_int]),
+    "stageml_norm_residual": (c_int, [POINTER(NormArgs), c_void_p, c_size_t, c_void_p]),
+    "stageml_norm_residual_backward": (c_int, [POINTER(NormArgs), c_void_p, c_size_t, c_void_p]),
+    "stageml_balance_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "stageml_balance_loss": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_float,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "stageml_balance_loss_backward": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                              c_int, c_float, c_void_p, c_void_p]),
     "stageml_stage_timer_enable": (c_int, [c_int]),
     "stageml_stage_timer_select": (c_int, [ctypes.c_uint]),
     "stageml_stage_timer_read": (c_int, [c_float_p, c_int32_p, c_int]),
@@ -178,7 +230,9 @@ SIGNATURES = {
 STAGE_NAMES = ("route", "permute", "gather_shrink", "gemm_gate_up", "shrink_h", "gemm_down", "combine", "gemm",
                "fold", "gemv")
 
-STRUCTS = {0: MoePlan, 1: MoeArgs, 2: LoraLinearArgs, 3: EpLayout, 4: EpArgs}
+STRUCTS = {0: MoePlan, 1: MoeArgs, 2: LoraLinearArgs, 3: EpLayout, 4: EpArgs, 5: MoeBlocksArgs, 6: NormArgs}
+
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 
 
 def declare(lib: ctypes.CDLL) -> None:
@@ -206,5 +260,5 @@ def stream_handle(stream=None) -> int:
     return s.cuda_stream
 
 
-__all__ = ["MoePlan", "MoeArgs", "LoraLinearArgs", "EpLayout", "EpArgs", "SIGNATURES", "STRUCTS", "declare", "check", "ptr",
+__all__ = ["MoePlan", "MoeArgs", "LoraLinearArgs", "EpLayout", "EpArgs", "MoeBlocksArgs", "NormArgs", "SIGNATURES", "STRUCTS", "declare", "check", "ptr",
            "stream_handle", "F32", "BF16", "F16", "E4M3", "I32", "I64", "OK"]

@@ -419,6 +419,300 @@ Tensor combine_rows(const Tensor& y, const Tensor& pair_row, int64_t T, int64_t 
   return out;
 }
 
+// ------------------------------------------------ block-scaled FP8, block norm, balance loss
+void check_e4m3(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn, "stageml: ", what, " must be float8_e4m3fn, got ", t.scalar_type());
+}
+void check_float_dtype(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, "stageml: ",
+              what, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+}
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+
+std::tuple<Tensor, Tensor> quantize_e4m3_blocks(const Tensor& x, bool tiles) {
+  check_cuda(x, "x", x);
+  check_float_dtype(x, "quantize_e4m3_blocks: x");
+  TORCH_CHECK(x.dim() >= (tiles ? 2 : 1), "quantize_e4m3_blocks: x needs at least ", tiles ? 2 : 1, " dims");
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t cols = x.size(-1), rows = x.dim() >= 2 ? x.size(-2) : 1;
+  int64_t batch = 1;
+  for (int64_t d = 0; d + 2 < x.dim(); ++d) batch *= x.size(d);
+  auto sizes = x.sizes().vec();
+  sizes.back() = blocks128(cols);
+  if (tiles) sizes[sizes.size() - 2] = blocks128(rows);
+  auto q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  auto s = at::empty(sizes, x.options().dtype(at::kFloat));
+  check_rc(stageml_quantize_e4m3_blocks(x.data_ptr(), dtype_code(x), batch, rows, cols, tiles ? 1 : 0,
+                                        static_cast<uint8_t*>(q.data_ptr()), s.data_ptr<float>(), cur_stream()),
+           "quantize_e4m3_blocks");
+  return {q, s};
+}
+
+Tensor block_matmul(const Tensor& x, const Tensor& x_scale, const Tensor& w, const Tensor& w_scale,
+                    at::ScalarType out_dtype) {
+  check_cuda(x, "x", x);
+  check_cuda(x_scale, "x_scale", x);
+  check_cuda(w, "w", x);
+  check_cuda(w_scale, "w_scale", x);
+  check_e4m3(x, "block_matmul: x");
+  check_e4m3(w, "block_matmul: w");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && w.size(1) == x.size(1), "block_matmul: x [M, K] and w [N, K], got ",
+              x.sizes(), " and ", w.sizes());
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  TORCH_CHECK(M <= INT32_MAX && N <= INT32_MAX && K <= INT32_MAX, "block_matmul: sizes past 2^31");
+  TORCH_CHECK(x_scale.scalar_type() == at::kFloat && x_scale.dim() == 2 && x_scale.size(0) == M &&
+                  x_scale.size(1) == blocks128(K),
+              "block_matmul: x_scale must be fp32 [M, ceil(K/128)], got ", x_scale.sizes());
+  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.dim() == 2 && w_scale.size(0) == blocks128(N) &&
+                  w_scale.size(1) == blocks128(K),
+              "block_matmul: w_scale must be fp32 [ceil(N/128), ceil(K/128)], got ", w_scale.sizes());
+  c10::cuda::CUDAGuard guard(x.device());
+  auto out = at::empty({M, N}, x.options().dtype(out_dtype));
+  check_float_dtype(out, "block_matmul: out_dtype");
+  const size_t bytes = stageml_block_matmul_workspace_bytes((int)M, (int)N, (int)K);
+  Tensor ws = bytes ? workspace(bytes, x) : Tensor();
+  check_rc(stageml_block_matmul(static_cast<const uint8_t*>(x.data_ptr()), x_scale.data_ptr<float>(),
+                                static_cast<const uint8_t*>(w.data_ptr()), w_scale.data_ptr<float>(), (int)M, (int)N,
+                                (int)K, dtype_code(out), out.data_ptr(), status_word(x), bytes ? ws.data_ptr() : nullptr,
+                                bytes, cur_stream()),
+           "block_matmul");
+  return out;
+}
+
+Tensor moe_forward_blocks(const Tensor& x, const Tensor& gate_up, const Tensor& gate_up_scale, const Tensor& down,
+                          const Tensor& down_scale, const c10::optional<Tensor>& topk_ids,
+                          const c10::optional<Tensor>& topk_weights, int64_t n_shared) {
+  TORCH_CHECK(x.dim() == 2 && gate_up.dim() == 3 && down.dim() == 3, "moe_forward_blocks: x [T, H], gate_up [E, 2I, H], ",
+              "down [E, H, I]");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+              "moe_forward_blocks: x must be bfloat16 or float16");
+  check_e4m3(gate_up, "moe_forward_blocks: gate_up");
+  check_e4m3(down, "moe_forward_blocks: down");
+  const int64_t T = x.size(0), H = x.size(1), E_tot = gate_up.size(0), I = gate_up.size(1) / 2;
+  TORCH_CHECK(gate_up.size(1) % 2 == 0 && gate_up.size(2) == H && down.size(0) == E_tot && down.size(1) == H &&
+                  down.size(2) == I,
+              "moe_forward_blocks: weight shapes do not match x");
+  TORCH_CHECK(n_shared >= 0 && n_shared <= E_tot, "moe_forward_blocks: n_shared out of range");
+  TORCH_CHECK(gate_up_scale.scalar_type() == at::kFloat &&
+                  gate_up_scale.sizes() == at::IntArrayRef({E_tot, blocks128(2 * I), blocks128(H)}),
+              "moe_forward_blocks: gate_up_scale must be fp32 [E, ceil(2I/128), ceil(H/128)], got ",
+              gate_up_scale.sizes());
+  TORCH_CHECK(down_scale.scalar_type() == at::kFloat &&
+                  down_scale.sizes() == at::IntArrayRef({E_tot, blocks128(H), blocks128(I)}),
+              "moe_forward_blocks: down_scale must be fp32 [E, ceil(H/128), ceil(I/128)], got ", down_scale.sizes());
+  for (auto* t : {&x, &gate_up, &gate_up_scale, &down, &down_scale}) check_cuda(*t, "input", x);
+  TORCH_CHECK(topk_ids.has_value() == topk_weights.has_value(), "moe_forward_blocks: topk_ids and topk_weights go together");
+  int64_t k = 0;
+  if (topk_ids.has_value()) {
+    check_cuda(*topk_ids, "topk_ids", x);
+    check_cuda(*topk_weights, "topk_weights", x);
+    check_float_dtype(*topk_weights, "moe_forward_blocks: topk_weights");
+    TORCH_CHECK(topk_ids->dim() == 2 && topk_ids->size(0) == T && topk_weights->sizes() == topk_ids->sizes(),
+                "moe_forward_blocks: topk_ids and topk_weights must be [T, k]");
+    k = topk_ids->size(1);
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  auto out = at::empty({T, H}, x.options());
+  stageml_moe_blocks_args a{};
+  a.T = (int)T;
+  a.H = (int)H;
+  a.I = (int)I;
+  a.E = (int)(E_tot - n_shared);
+  a.k = (int)k;
+  a.n_shared = (int)n_shared;
+  a.act_dtype = dtype_code(x);
+  a.x = x.data_ptr();
+  a.topk_ids = opt_ptr(topk_ids);
+  a.ids_dtype = topk_ids.has_value() ? dtype_code(*topk_ids) : STAGEML_I32;
+  a.topk_weights = opt_ptr(topk_weights);
+  a.weights_dtype = topk_weights.has_value() ? dtype_code(*topk_weights) : STAGEML_F32;
+  a.gate_up = static_cast<const uint8_t*>(gate_up.data_ptr());
+  a.gate_up_scale = gate_up_scale.data_ptr<float>();
+  a.down = static_cast<const uint8_t*>(down.data_ptr());
+  a.down_scale = down_scale.data_ptr<float>();
+  a.out = out.data_ptr();
+  a.status = status_word(x);
+  const size_t ws = stageml_moe_blocks_workspace_bytes(&a);
+  TORCH_CHECK(ws > 0, "moe_forward_blocks: invalid arguments: ", stageml_last_error());
+  auto w = workspace(ws, x);
+  check_rc(stageml_moe_forward_blocks(&a, w.data_ptr(), (size_t)w.numel(), cur_stream()), "moe_forward_blocks");
+  return out;
+}
+
+// The arguments that the forward and the backward share; gate_mode 0 none, 1 [H], 2 [T], 3 [T, H].
+void norm_args(stageml_norm_args* a, const c10::optional<Tensor>& block_out, const Tensor& residual,
+               const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate, int64_t gate_mode,
+               const c10::optional<Tensor>& pre_weight, double residual_scale, double eps, at::ScalarType block_dtype) {
+  TORCH_CHECK(residual.dim() == 2, "norm_residual: residual must be [T, H]");
+  check_cuda(residual, "residual", residual);
+  check_float_dtype(residual, "norm_residual: residual");
+  const int64_t T = residual.size(0), H = residual.size(1);
+  if (block_out.has_value()) {
+    check_cuda(*block_out, "block_out", residual);
+    TORCH_CHECK(block_out->sizes() == residual.sizes(), "norm_residual: block_out must have residual's shape");
+    TORCH_CHECK(block_out->scalar_type() == block_dtype, "norm_residual: block_out must be ", block_dtype);
+  }
+  for (const auto* w : {&post_weight, &pre_weight})
+    if (w->has_value()) {
+      check_cuda(**w, "weight", residual);
+      check_float_dtype(**w, "norm_residual: weight");
+      TORCH_CHECK((*w)->dim() == 1 && (*w)->size(0) == H, "norm_residual: a norm weight must be [H]");
+    }
+  if (gate.has_value()) {
+    check_cuda(*gate, "gate", residual);
+    check_float_dtype(*gate, "norm_residual: gate");
+    const int64_t need = gate_mode == STAGEML_GATE_CHANNEL ? H : gate_mode == STAGEML_GATE_TOKEN ? T : T * H;
+    TORCH_CHECK(gate->numel() == need, "norm_residual: gate does not match its mode");
+  }
+  a->T = T;
+  TORCH_CHECK(H >= 1 && H <= INT32_MAX, "norm_residual: bad width ", H);
+  a->H = (int)H;
+  a->resid_dtype = dtype_code(residual);
+  a->block_dtype = block_dtype == at::kFloat ? STAGEML_F32 : block_dtype == at::kBFloat16 ? STAGEML_BF16
+                   : block_dtype == at::kHalf ? STAGEML_F16 : -1;
+  a->residual = residual.data_ptr();
+  a->block_out = opt_ptr(block_out);
+  a->post_weight = opt_ptr(post_weight);
+  a->post_dtype = post_weight.has_value() ? dtype_code(*post_weight) : STAGEML_F32;
+  a->gate = opt_ptr(gate);
+  a->gate_mode = gate.has_value() ? (int)gate_mode : STAGEML_GATE_NONE;
+  a->gate_dtype = gate.has_value() ? dtype_code(*gate) : STAGEML_F32;
+  a->pre_weight = opt_ptr(pre_weight);
+  a->pre_dtype = pre_weight.has_value() ? dtype_code(*pre_weight) : STAGEML_F32;
+  a->residual_scale = (float)residual_scale;
+  a->eps = (float)eps;
+}
+
+// -> [new_residual], [new_residual, normed] or [new_residual, codes, scale]
+std::vector<Tensor> norm_residual(const c10::optional<Tensor>& block_out, const Tensor& residual,
+                                  const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
+                                  int64_t gate_mode, const c10::optional<Tensor>& pre_weight, double residual_scale,
+                                  double eps, bool quantize, at::ScalarType normed_dtype) {
+  stageml_norm_args a{};
+  norm_args(&a, block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale, eps, normed_dtype);
+  TORCH_CHECK(!quantize || pre_weight.has_value(), "norm_residual: quantize needs pre_weight");
+  c10::cuda::CUDAGuard guard(residual.device());
+  std::vector<Tensor> out{at::empty_like(residual)};
+  a.new_residual = out[0].data_ptr();
+  if (quantize) {
+    out.push_back(at::empty(residual.sizes(), residual.options().dtype(at::kFloat8_e4m3fn)));
+    out.push_back(at::empty({a.T, blocks128(a.H)}, residual.options().dtype(at::kFloat)));
+    a.codes = static_cast<uint8_t*>(out[1].data_ptr());
+    a.code_scale = out[2].data_ptr<float>();
+  } else if (pre_weight.has_value()) {
+    out.push_back(at::empty(residual.sizes(), residual.options().dtype(normed_dtype)));
+    a.normed = out[1].data_ptr();
+  }
+  const size_t bytes = stageml_norm_residual_workspace_bytes(&a, 0);
+  Tensor ws = bytes ? workspace(bytes, residual) : Tensor();
+  check_rc(stageml_norm_residual(&a, bytes ? ws.data_ptr() : nullptr, bytes, cur_stream()), "norm_residual");
+  return out;
+}
+
+// -> gradients of [residual, block_out?, post_weight?, gate?, pre_weight?] (those present, in this order)
+std::vector<Tensor> norm_residual_backward(const c10::optional<Tensor>& grad_residual,
+                                           const c10::optional<Tensor>& grad_normed,
+                                           const c10::optional<Tensor>& block_out, const Tensor& residual,
+                                           const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
+                                           int64_t gate_mode, const c10::optional<Tensor>& pre_weight,
+                                           double residual_scale, double eps) {
+  TORCH_CHECK(grad_residual.has_value() || grad_normed.has_value(), "norm_residual_backward: no gradient given");
+  const at::ScalarType bd = block_out.has_value()     ? block_out->scalar_type()
+                            : grad_normed.has_value() ? grad_normed->scalar_type()
+                                                      : residual.scalar_type();
+  stageml_norm_args a{};
+  norm_args(&a, block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale, eps, bd);
+  if (grad_residual.has_value()) {
+    check_cuda(*grad_residual, "grad_residual", residual);
+    TORCH_CHECK(grad_residual->sizes() == residual.sizes() && grad_residual->scalar_type() == residual.scalar_type(),
+                "norm_residual_backward: grad_residual must match residual");
+  }
+  if (grad_normed.has_value()) {
+    check_cuda(*grad_normed, "grad_normed", residual);
+    TORCH_CHECK(grad_normed->sizes() == residual.sizes() && grad_normed->scalar_type() == bd,
+                "norm_residual_backward: grad_normed must have residual's shape and the block dtype");
+    TORCH_CHECK(pre_weight.has_value(), "norm_residual_backward: grad_normed without pre_weight");
+  }
+  c10::cuda::CUDAGuard guard(residual.device());
+  a.grad_residual = opt_ptr(grad_residual);
+  a.grad_normed = opt_ptr(grad_normed);
+  std::vector<Tensor> out{at::empty_like(residual)};
+  a.d_residual = out[0].data_ptr();
+  if (block_out.has_value()) {
+    out.push_back(at::empty_like(*block_out));
+    a.d_block_out = out.back().data_ptr();
+  }
+  if (post_weight.has_value()) {
+    out.push_back(at::empty_like(*post_weight));
+    a.d_post = out.back().data_ptr();
+  }
+  if (gate.has_value()) {
+    out.push_back(at::empty_like(*gate));
+    a.d_gate = out.back().data_ptr();
+  }
+  if (pre_weight.has_value()) {
+    out.push_back(at::empty_like(*pre_weight));
+    a.d_pre = out.back().data_ptr();
+  }
+  const size_t bytes = stageml_norm_residual_workspace_bytes(&a, 1);
+  Tensor ws = bytes ? workspace(bytes, residual) : Tensor();
+  check_rc(stageml_norm_residual_backward(&a, bytes ? ws.data_ptr() : nullptr, bytes, cur_stream()),
+           "norm_residual_backward");
+  return out;
+}
+
+const uint8_t* valid_ptr(const c10::optional<Tensor>& valid, const Tensor& logits) {
+  if (!valid.has_value()) return nullptr;
+  check_cuda(*valid, "valid", logits);
+  TORCH_CHECK((valid->scalar_type() == at::kBool || valid->scalar_type() == at::kByte) &&
+                  valid->numel() == logits.size(0),
+              "balance_loss: valid must be bool or uint8 [T]");
+  return static_cast<const uint8_t*>(valid->data_ptr());
+}
+
+std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& topk_ids, double coefficient,
+                                                const c10::optional<Tensor>& valid) {
+  check_cuda(logits, "logits", logits);
+  check_cuda(topk_ids, "topk_ids", logits);
+  check_float_dtype(logits, "balance_loss: logits");
+  TORCH_CHECK(logits.dim() == 2 && topk_ids.dim() == 2 && topk_ids.size(0) == logits.size(0),
+              "balance_loss: logits [T, E] and topk_ids [T, k], got ", logits.sizes(), " and ", topk_ids.sizes());
+  const int64_t T = logits.size(0), E = logits.size(1), k = topk_ids.size(1);
+  TORCH_CHECK(E >= 1 && E <= 256 && k >= 1 && k <= 8, "balance_loss: E=", E, " must be in 1..256 and k=", k, " in 1..8");
+  const uint8_t* v = valid_ptr(valid, logits);
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto loss = at::empty({}, logits.options().dtype(at::kFloat));
+  auto counts = at::empty({E}, logits.options().dtype(at::kInt));
+  auto tokens = at::empty({}, logits.options().dtype(at::kInt));
+  auto w = workspace(stageml_balance_workspace_bytes(T, (int)E), logits);
+  check_rc(stageml_balance_loss(logits.data_ptr(), dtype_code(logits), topk_ids.data_ptr(), dtype_code(topk_ids), v, T,
+                                (int)E, (int)k, (float)coefficient, loss.data_ptr<float>(), counts.data_ptr<int32_t>(),
+                                tokens.data_ptr<int32_t>(), status_word(logits), w.data_ptr(), (size_t)w.numel(),
+                                cur_stream()),
+           "balance_loss");
+  return {loss, counts, tokens};
+}
+
+Tensor balance_loss_backward(const Tensor& grad_loss, const Tensor& logits, const Tensor& counts, const Tensor& tokens,
+                             int64_t k, double coefficient, const c10::optional<Tensor>& valid) {
+  check_cuda(logits, "logits", logits);
+  check_float_dtype(logits, "balance_loss_backward: logits");
+  TORCH_CHECK(logits.dim() == 2, "balance_loss_backward: logits must be [T, E]");
+  for (auto* t : {&grad_loss, &counts, &tokens}) check_cuda(*t, "input", logits);
+  TORCH_CHECK(grad_loss.scalar_type() == at::kFloat && grad_loss.numel() == 1, "balance_loss_backward: grad_loss fp32 [1]");
+  TORCH_CHECK(counts.scalar_type() == at::kInt && counts.numel() == logits.size(1) &&
+                  tokens.scalar_type() == at::kInt && tokens.numel() == 1,
+              "balance_loss_backward: counts int32 [E] and tokens int32 [1] of the forward");
+  const uint8_t* v = valid_ptr(valid, logits);
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto grad = at::empty_like(logits);
+  check_rc(stageml_balance_loss_backward(grad_loss.data_ptr<float>(), logits.data_ptr(), dtype_code(logits),
+                                         counts.data_ptr<int32_t>(), tokens.data_ptr<int32_t>(), v, logits.size(0),
+                                         (int)logits.size(1), (int)k, (float)coefficient, grad.data_ptr(), cur_stream()),
+           "balance_loss_backward");
+  return grad;
+}
+
 // Returns the device status word (synchronising on it) and clears it.
 int64_t take_status(const Tensor& like) {
   c10::cuda::CUDAGuard guard(like.device());
@@ -456,6 +750,22 @@ TORCH_LIBRARY(stageml, m) {
   m.def("quantize_e4m3_rows(Tensor w) -> (Tensor, Tensor)");
   m.def("combine_rows(Tensor y, Tensor pair_row, int T, int kk) -> Tensor");
   m.def("take_status(Tensor like) -> int");
+  m.def("quantize_e4m3_blocks(Tensor x, bool tiles) -> (Tensor, Tensor)");
+  m.def("block_matmul(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale, ScalarType out_dtype) -> Tensor");
+  m.def(
+      "moe_forward_blocks(Tensor x, Tensor gate_up, Tensor gate_up_scale, Tensor down, Tensor down_scale, "
+      "Tensor? topk_ids, Tensor? topk_weights, int n_shared) -> Tensor");
+  m.def(
+      "norm_residual(Tensor? block_out, Tensor residual, Tensor? post_weight, Tensor? gate, int gate_mode, "
+      "Tensor? pre_weight, float residual_scale, float eps, bool quantize, ScalarType normed_dtype) -> Tensor[]");
+  m.def(
+      "norm_residual_backward(Tensor? grad_residual, Tensor? grad_normed, Tensor? block_out, Tensor residual, "
+      "Tensor? post_weight, Tensor? gate, int gate_mode, Tensor? pre_weight, float residual_scale, float eps) "
+      "-> Tensor[]");
+  m.def("balance_loss(Tensor logits, Tensor topk_ids, float coefficient, Tensor? valid) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "balance_loss_backward(Tensor grad_loss, Tensor logits, Tensor counts, Tensor tokens, int k, "
+      "float coefficient, Tensor? valid) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(stageml, CUDA, m) {
@@ -471,4 +781,11 @@ TORCH_LIBRARY_IMPL(stageml, CUDA, m) {
   m.impl("quantize_e4m3_rows", &quantize_e4m3_rows);
   m.impl("combine_rows", &combine_rows);
   m.impl("take_status", &take_status);
+  m.impl("quantize_e4m3_blocks", &quantize_e4m3_blocks);
+  m.impl("block_matmul", &block_matmul);
+  m.impl("moe_forward_blocks", &moe_forward_blocks);
+  m.impl("norm_residual", &norm_residual);
+  m.impl("norm_residual_backward", &norm_residual_backward);
+  m.impl("balance_loss", &balance_loss);
+  m.impl("balance_loss_backward", &balance_loss_backward);
 }

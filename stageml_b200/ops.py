@@ -65,6 +65,49 @@ def _register_fakes() -> None:
     def _(x, W, A, B, scale):
         return x.new_empty((x.shape[0], W.shape[1]))
 
+    def blocks(n):
+        return (n + 127) // 128
+
+    @lib.register_fake("stageml::quantize_e4m3_blocks")
+    def _(x, tiles):
+        shape = list(x.shape)
+        shape[-1] = blocks(shape[-1])
+        if tiles:
+            shape[-2] = blocks(shape[-2])
+        return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(shape, dtype=torch.float32)
+
+    @lib.register_fake("stageml::block_matmul")
+    def _(x, x_scale, w, w_scale, out_dtype):
+        return x.new_empty((x.shape[0], w.shape[0]), dtype=out_dtype)
+
+    @lib.register_fake("stageml::moe_forward_blocks")
+    def _(x, gate_up, gate_up_scale, down, down_scale, topk_ids, topk_weights, n_shared):
+        return x.new_empty(x.shape)
+
+    @lib.register_fake("stageml::norm_residual")
+    def _(block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale, eps, quantize, normed_dtype):
+        out = [torch.empty_like(residual)]
+        if quantize:
+            out.append(residual.new_empty(residual.shape, dtype=torch.float8_e4m3fn))
+            out.append(residual.new_empty((residual.shape[0], blocks(residual.shape[1])), dtype=torch.float32))
+        elif pre_weight is not None:
+            out.append(residual.new_empty(residual.shape, dtype=normed_dtype))
+        return out
+
+    @lib.register_fake("stageml::norm_residual_backward")
+    def _(grad_residual, grad_normed, block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale,
+          eps):
+        return [torch.empty_like(t) for t in (residual, block_out, post_weight, gate, pre_weight) if t is not None]
+
+    @lib.register_fake("stageml::balance_loss")
+    def _(logits, topk_ids, coefficient, valid):
+        return (logits.new_empty((), dtype=torch.float32), logits.new_empty((logits.shape[1],), dtype=torch.int32),
+                logits.new_empty((), dtype=torch.int32))
+
+    @lib.register_fake("stageml::balance_loss_backward")
+    def _(grad_loss, logits, counts, tokens, k, coefficient, valid):
+        return torch.empty_like(logits)
+
 
 try:
     _register_fakes()
@@ -167,6 +210,165 @@ def quantize_e4m3_rows(w):
     return _ops.quantize_e4m3_rows(w.contiguous())
 
 
+def quantize_e4m3_blocks(x, tiles: bool = False):
+    """e4m3 codes with one fp32 scale per 128 values -> (q float8_e4m3fn, scale fp32).
+
+    x [..., K] float32/bfloat16/float16. tiles False (activations): scale [..., ceil(K/128)], one per 128
+    values of a row. tiles True (weights [..., N, K]): scale [..., ceil(N/128), ceil(K/128)], one per
+    128 x 128 tile. scale = max|x| / 448 (1 for a block of zeros), q = e4m3(x / scale), nearest even.
+    """
+    ensure_cuda_device(x)
+    return _ops.quantize_e4m3_blocks(x.contiguous(), bool(tiles))
+
+
+def block_matmul(x, x_scale, w, w_scale, out_dtype=torch.bfloat16):
+    """x w^T on block-scaled e4m3 operands, fp32 sums rounded once to out_dtype.
+
+    x [M, K] with x_scale [M, ceil(K/128)], w [N, K] with w_scale [ceil(N/128), ceil(K/128)], as
+    ``quantize_e4m3_blocks`` (tiles False / True) makes them; K a multiple of 16. -> [M, N].
+    """
+    ensure_cuda_device(x)
+    return _ops.block_matmul(x.contiguous(), x_scale.contiguous(), w.contiguous(), w_scale.contiguous(), out_dtype)
+
+
+def moe_forward_blocks(x, gate_up, gate_up_scale, down, down_scale, *, topk_ids=None, topk_weights=None,
+                       n_shared: int = 0):
+    """One routed SwiGLU FFN layer on block-scaled e4m3 weights, both products on e4m3 operands.
+
+    x [T, H] bfloat16/float16; gate_up [E + n_shared, 2I, H] and down [E + n_shared, H, I] e4m3 with the
+    scales of ``quantize_e4m3_blocks(w, tiles=True)``; topk_ids [T, k] and topk_weights [T, k] as
+    ``route_topk`` gives them (None: only the shared experts). H and I are multiples of 16. x and
+    silu(gate) * up are quantized per 128 values of a row on the way. No LoRA: tenants with adapters
+    take ``moe_forward``.
+    """
+    ensure_cuda_device(x)
+    return _ops.moe_forward_blocks(x.contiguous(), gate_up, gate_up_scale, down, down_scale, topk_ids, topk_weights,
+                                   int(n_shared))
+
+
+def _rows(t):
+    return None if t is None else t.reshape(-1, t.shape[-1]).contiguous()
+
+
+def _gate_mode(gate, residual) -> int:
+    """0 none, 1 per channel [H] or [1, .., H], 2 per token [..., 1], 3 full."""
+    if gate is None:
+        return 0
+    H = residual.shape[-1]
+    if gate.shape == residual.shape:
+        return 3
+    if gate.numel() == H and gate.shape[-1:] == residual.shape[-1:]:
+        return 1
+    if gate.shape == residual.shape[:-1] + (1,):
+        return 2
+    raise ValueError(f"norm_residual: gate {tuple(gate.shape)} must be [H], [..., 1] or [..., H] for a residual "
+                     f"{tuple(residual.shape)}")
+
+
+def norm_residual_backward(grad_residual, grad_normed, block_out, residual, *, post_weight=None, gate=None,
+                           residual_scale: float = 1.0, pre_weight=None, eps: float = 1e-6):
+    """Gradients of ``norm_residual`` from those of its outputs (either may be None = zero) and its inputs.
+
+    -> (d_residual, d_block_out, d_post_weight, d_gate, d_pre_weight), None for inputs that are None. Each
+    has its input's shape and dtype; sums over tokens are fp32 in a fixed order.
+    """
+    ensure_cuda_device(residual)
+    inputs = (residual, block_out, post_weight, gate, pre_weight)
+    out = iter(_ops.norm_residual_backward(_rows(grad_residual), _rows(grad_normed), _rows(block_out), _rows(residual),
+                                           post_weight, None if gate is None else gate.contiguous(),
+                                           _gate_mode(gate, residual), pre_weight, float(residual_scale), float(eps)))
+    return tuple(None if t is None else next(out).view(t.shape) for t in inputs)
+
+
+class _NormResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, normed_dtype):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(block_out, residual, post_weight, gate, pre_weight)
+        ctx.numbers = {"residual_scale": residual_scale, "eps": eps}
+        return _norm_residual(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, False,
+                              normed_dtype)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        block_out, residual, post_weight, gate, pre_weight = ctx.saved_tensors
+        grad_normed = grads[1] if len(grads) > 1 else None
+        d = norm_residual_backward(grads[0], grad_normed, block_out, residual, post_weight=post_weight, gate=gate,
+                                   pre_weight=pre_weight, **ctx.numbers)
+        return d[1], d[0], d[2], d[3], d[4], None, None, None
+
+
+def _norm_residual(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, quantize, normed_dtype):
+    out = _ops.norm_residual(_rows(block_out), _rows(residual), post_weight,
+                             None if gate is None else gate.contiguous(), _gate_mode(gate, residual), pre_weight,
+                             float(residual_scale), float(eps), bool(quantize), normed_dtype)
+    shape = residual.shape
+    return tuple(t.view(shape[:-1] + t.shape[-1:]) for t in out)
+
+
+def norm_residual(block_out, residual, *, post_weight=None, gate=None, residual_scale: float = 1.0, pre_weight=None,
+                  eps: float = 1e-6, quantize: bool = False, normed_dtype=None):
+    """The norm after a block, its gate, the residual sum and the next block's norm in one pass.
+
+    u = post_weight * rms_norm(block_out) (block_out itself without post_weight),
+    new_residual = residual_scale * residual + gate * u (without block_out: residual_scale * residual),
+    normed = pre_weight * rms_norm(new_residual).
+
+    residual [..., H] float32/bfloat16/float16; block_out of the same shape, in residual's dtype or, beside a
+    float32 residual, in any of the three; gate [H], [..., 1] or [..., H]; weights [H]. fp32 arithmetic, each
+    output rounded once. -> (new_residual, normed), (new_residual,) without pre_weight. quantize=True returns
+    (new_residual, codes, scale) instead: normed as ``quantize_e4m3_blocks`` would hold it, the operand of the
+    block-scaled products. normed_dtype (block_out's dtype by default, else residual's) names normed's type.
+    Differentiable, except with quantize. H <= 16384.
+    """
+    ensure_cuda_device(residual)
+    if normed_dtype is None or block_out is not None:
+        normed_dtype = (residual if block_out is None else block_out).dtype
+    tensors = (block_out, residual, post_weight, gate, pre_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        if quantize:
+            raise ValueError("norm_residual: the codes of quantize=True carry no gradient")
+        return _NormResidual.apply(*tensors, residual_scale, eps, normed_dtype)
+    return _norm_residual(*tensors, residual_scale, eps, quantize, normed_dtype)
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk_ids, coefficient, valid):
+        loss, counts, tokens = _ops.balance_loss(logits, topk_ids, coefficient, valid)
+        ctx.save_for_backward(logits, counts, tokens, valid)
+        ctx.numbers = (topk_ids.shape[1], coefficient)
+        ctx.mark_non_differentiable(counts, tokens)
+        return loss, counts, tokens
+
+    @staticmethod
+    def backward(ctx, grad_loss, _counts, _tokens):
+        logits, counts, tokens, valid = ctx.saved_tensors
+        return balance_loss_backward(grad_loss, logits, counts, tokens, *ctx.numbers, valid=valid), None, None, None
+
+
+def balance_loss(logits, topk_ids, coefficient: float = 1.0, *, valid=None):
+    """The router's balance loss with the counts per expert -> (loss fp32 [], counts int32 [E], tokens int32 []).
+
+    loss = coefficient * E * sum_e f_e P_e: f_e the share of the chosen slots that went to expert e, P_e the mean
+    softmax probability of e, both over the tokens with valid[t] (all without valid); tokens is their number.
+    logits [T, E] as ``route_topk`` returns them (or bfloat16/float16), topk_ids [T, k] (negative: no expert).
+    Differentiable in logits; the counts carry no gradient.
+    """
+    ensure_cuda_device(logits)
+    logits, topk_ids = logits.contiguous(), topk_ids.contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _BalanceLoss.apply(logits, topk_ids, float(coefficient), valid)
+    return _ops.balance_loss(logits, topk_ids, float(coefficient), valid)
+
+
+def balance_loss_backward(grad_loss, logits, counts, tokens, k: int, coefficient: float = 1.0, *, valid=None):
+    """Gradient of ``balance_loss``'s logits for grad_loss (CUDA fp32 scalar), from the forward's counts and tokens."""
+    ensure_cuda_device(logits)
+    return _ops.balance_loss_backward(grad_loss.contiguous(), logits.contiguous(), counts, tokens, int(k),
+                                      float(coefficient), valid)
+
+
 def combine_rows(y, pair_row, T: int, kk: int):
     """out[t] = sum_j y[pair_row[t*kk + j]] (rows < 0 skipped), fp32 sum, one rounding."""
     ensure_cuda_device(y)
@@ -189,6 +391,13 @@ __all__ = [
     "moe_linear",
     "lora_gemv_f32",
     "quantize_e4m3_rows",
+    "quantize_e4m3_blocks",
+    "block_matmul",
+    "moe_forward_blocks",
+    "norm_residual",
+    "norm_residual_backward",
+    "balance_loss",
+    "balance_loss_backward",
     "combine_rows",
     "take_status",
     "PLAN_FIELDS",
