@@ -452,6 +452,7 @@ typedef struct stageml_norm_args {
   void* d_post;
   void* d_gate;
   void* d_pre;
+  int32_t* status;           /* device status word, may be NULL */
 } stageml_norm_args;
 
 size_t stageml_norm_residual_workspace_bytes(const stageml_norm_args* args, int backward);

@@ -163,7 +163,7 @@ class NormArgs(ctypes.Structure):
         ("residual_scale", c_float),
         ("eps", c_float),
     ] + [(n, c_void_p) for n in ("new_residual", "normed", "codes", "code_scale", "grad_residual", "grad_normed",
-                                  "d_residual", "d_block_out", "d_post", "d_gate", "d_pre")]
+                                  "d_residual", "d_block_out", "d_post", "d_gate", "d_pre", "status")]
 
 
 # name -> (restype, argtypes)

@@ -10,12 +10,15 @@
 // goes to the status word and is skipped. A token whose logits are all -infinity has no
 // softmax: its p and its gradient are 0. n = 0 gives loss 0.
 //
-// Forward: lanes of a warp own experts (groups of 2..32 lanes per token, up to 8 experts
-// per lane); each warp sums its tokens' p in registers, each CTA writes one partial sum per
-// expert, and a second kernel adds the partials in CTA order: no floating-point atomics,
-// the same bits on every run. Counts are integer atomics in shared memory. Backward: the
-// softmax again from the logits, one pass. Bound: HBM for long batches (logits read twice,
-// gradient written once), launches for short ones.
+// A token's experts lie on 1..8 lanes, 4 consecutive experts per 16-byte load and up to 32
+// per lane, so a warp works on 4 to 32 tokens at once and a softmax costs few shuffles.
+// Each lane sums its experts' p over its tokens in registers; a CTA adds them in a fixed
+// order in shared memory. Counts are integer atomics in shared memory. Batches of up to
+// kClusterValues logits run as one cluster whose first CTA adds the others' sums over
+// distributed shared memory and writes the loss: one launch. Longer ones write one partial
+// per CTA, added in CTA order by a second kernel. No floating-point atomics: the same bits
+// on every run. Backward: the softmax again from the logits, one pass. Bound: HBM for long
+// batches (logits read twice, gradient written once), launches for short ones.
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -23,72 +26,107 @@
 namespace sb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxE = 256;
+constexpr int kClusterCtas = 8;                // portable cluster size
+constexpr int64_t kClusterValues = 256 * 1024;  // logits of a one-launch batch
 
-// The token's softmax over `LANES` lanes, NJ experts per lane (expert lane + LANES j),
-// from its logits in x; 0 everywhere when no logit is above -infinity.
-template <int LANES, int NJ>
-__device__ __forceinline__ void softmax_lanes(float (&x)[NJ]) {
-  float m = x[0];
+// Lanes per token and 4-expert groups per lane: expert (lane + LANES * j) * 4 + i.
+template <int LANES, int NV>
+struct Layout {
+  static constexpr int lanes = LANES, groups = NV, per_warp = 32 / LANES, experts = LANES * NV * 4;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load4(const T* p, int e, int E, bool live, float (&f)[4]) {
+  if (!live || e >= E) {
+    f[0] = f[1] = f[2] = f[3] = -INFINITY;
+  } else if constexpr (VEC && sizeof(T) == 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p + e));
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  } else if constexpr (VEC) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p + e));
+    const T* h = reinterpret_cast<const T*>(&v);
 #pragma unroll
-  for (int j = 1; j < NJ; ++j) m = fmaxf(m, x[j]);
+    for (int i = 0; i < 4; ++i) f[i] = to_f32<T>(h[i]);
+  } else {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const bool none = m == -INFINITY;
+    for (int i = 0; i < 4; ++i) f[i] = e + i < E ? to_f32<T>(p[e + i]) : -INFINITY;
+  }
+}
+
+// The token's logits on its lanes, then its softmax; 0 everywhere when no logit is above
+// -infinity (or the token does not count).
+template <typename T, typename L, bool VEC>
+__device__ __forceinline__ void load_softmax(const T* __restrict__ logits, int64_t t, bool live, int E, int lane,
+                                             float (&x)[L::groups][4]) {
+  const T* row = logits + t * E;
+#pragma unroll
+  for (int j = 0; j < L::groups; ++j) load4<T, VEC>(row, (lane + L::lanes * j) * 4, E, live, x[j]);
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, x[j][i]);
+#pragma unroll
+  for (int o = L::lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float shift = m == -INFINITY ? 0.f : m;
   float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    x[j] = none && x[j] == -INFINITY ? 0.f : expf(x[j] - m);
-    s += x[j];
-  }
+  for (int j = 0; j < L::groups; ++j)
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const float inv = none && s == 0.f ? 0.f : 1.f / s;
+    for (int i = 0; i < 4; ++i) {
+      x[j][i] = __expf(x[j][i] - shift);
+      s += x[j][i];
+    }
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) x[j] *= inv;
+  for (int o = L::lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const float inv = s == 0.f ? 0.f : 1.f / s;
+#pragma unroll
+  for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[j][i] *= inv;
 }
 
-template <typename T, int LANES, int NJ>
-__device__ __forceinline__ void load_logits(const T* __restrict__ logits, int64_t t, bool live, int E, int lane,
-                                            float (&x)[NJ]) {
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int e = lane + LANES * j;
-    x[j] = live && e < E ? to_f32<T>(logits[t * E + e]) : -INFINITY;
-  }
-}
+struct BalanceIn {
+  const void* ids;
+  int ids_i64;
+  const uint8_t* valid;
+  int64_t T;
+  int E, k;
+  int32_t* status;
+};
 
-template <typename T, int LANES, int NJ>
-__global__ void __launch_bounds__(kThreads)
-    balance_sums_kernel(const T* __restrict__ logits, const void* __restrict__ ids, int ids_i64,
-                        const uint8_t* __restrict__ valid, int64_t T_, int E, int k, float* __restrict__ psum,
-                        int32_t* __restrict__ pcount, int32_t* status) {
-  constexpr int PER_WARP = 32 / LANES;
-  __shared__ float sums[kWarps][LANES * NJ];
-  __shared__ int32_t counts[LANES * NJ + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LANES - 1), sub = (threadIdx.x & 31) / LANES;
-  for (int i = threadIdx.x; i <= LANES * NJ; i += kThreads) counts[i] = 0;
+// This CTA's tokens (cta of ctas): sums[e] = sum of p, counts[e], counts[E] = tokens.
+template <typename T, typename L, bool VEC>
+__device__ __forceinline__ void cta_sums(const T* __restrict__ logits, const BalanceIn& in, int cta, int ctas,
+                                         float (*warp_sums)[kMaxE], float* sums, int32_t* counts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & (L::lanes - 1), sub = (threadIdx.x & 31) / L::lanes;
+  for (int i = threadIdx.x; i <= kMaxE; i += kThreads) counts[i] = 0;
   __syncthreads();
-  const int64_t first = (int64_t)blockIdx.x * kWarps * PER_WARP, step = (int64_t)gridDim.x * kWarps * PER_WARP;
-  float acc[NJ];
+  float acc[L::groups][4];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) acc[j] = 0.f;
+  for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
   int tokens = 0;
-  for (int64_t t0 = first + warp * PER_WARP; t0 < T_; t0 += step) {
+  const int64_t step = (int64_t)ctas * kWarps * L::per_warp;
+  for (int64_t t0 = ((int64_t)cta * kWarps + warp) * L::per_warp; t0 < in.T; t0 += step) {
     const int64_t t = t0 + sub;
-    const bool live = t < T_ && (!valid || valid[t]);
-    float x[NJ];
-    load_logits<T, LANES, NJ>(logits, t, live, E, lane, x);
-    softmax_lanes<LANES, NJ>(x);
+    const bool live = t < in.T && (!in.valid || in.valid[t]);
+    float x[L::groups][4];
+    load_softmax<T, L, VEC>(logits, t, live, in.E, lane, x);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[j] += x[j];
+    for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] += x[j][i];
     if (live) {
-      for (int j = lane; j < k; j += LANES) {
-        const int64_t i = t * k + j;
-        const int64_t e = ids_i64 ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
-        if (e >= E) {
-          if (status) atomicCAS(status, 0, (int)kDevBadIndex);
+      for (int j = lane; j < in.k; j += L::lanes) {
+        const int64_t i = t * in.k + j;
+        const int64_t e = in.ids_i64 ? static_cast<const int64_t*>(in.ids)[i] : static_cast<const int32_t*>(in.ids)[i];
+        if (e >= in.E) {
+          if (in.status) atomicCAS(in.status, 0, (int)kDevBadIndex);
         } else if (e >= 0) {
           atomicAdd(&counts[e], 1);
         }
@@ -97,41 +135,115 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 #pragma unroll
-  for (int o = LANES; o < 32; o <<= 1)
+  for (int o = L::lanes; o < 32; o <<= 1)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-  if (tokens) atomicAdd(&counts[LANES * NJ], tokens);
+    for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+  if ((threadIdx.x & 31) == 0 && tokens) atomicAdd(&counts[in.E], tokens);
   if (sub == 0)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) sums[warp][lane + LANES * j] = acc[j];
+    for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) warp_sums[warp][(lane + L::lanes * j) * 4 + i] = acc[j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kThreads) {
+  for (int e = threadIdx.x; e < in.E; e += kThreads) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += sums[w][e];
-    psum[(int64_t)blockIdx.x * E + e] = s;
-    pcount[(int64_t)blockIdx.x * (E + 1) + e] = counts[e];
+    for (int w = 0; w < kWarps; ++w) s += warp_sums[w][e];
+    sums[e] = s;
   }
-  if (threadIdx.x == 0) pcount[(int64_t)blockIdx.x * (E + 1) + E] = counts[LANES * NJ];
+  __syncthreads();
 }
 
-// One CTA: totals over the CTAs of the first kernel in a fixed order, then the loss.
+// From the totals in shared memory (counts[E] = tokens): loss, counts, tokens. One CTA.
+__device__ __forceinline__ void write_loss(const float* sums, const int32_t* counts, int E, int k, float coefficient,
+                                           float* loss, int32_t* counts_out, int32_t* tokens_out) {
+  for (int e = threadIdx.x; e < E; e += blockDim.x) counts_out[e] = counts[e];
+  if (threadIdx.x < 32) {
+    const float n = fmaxf((float)counts[E], 1.f);
+    float t = 0.f;
+    for (int e = threadIdx.x; e < E; e += 32) t += (float)counts[e] / (n * (float)k) * (sums[e] / n);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (threadIdx.x == 0) {
+      *loss = coefficient * (float)E * t;
+      *tokens_out = counts[E];
+    }
+  }
+}
+
+// One cluster: every CTA its sums, the first CTA their totals in CTA order and the loss.
+template <typename T, typename L, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+    balance_cluster_kernel(const T* __restrict__ logits, const BalanceIn in, float coefficient, float* loss,
+                           int32_t* counts_out, int32_t* tokens_out) {
+  __shared__ float warp_sums[kWarps][kMaxE];
+  __shared__ float sums[kMaxE];
+  __shared__ int32_t counts[kMaxE + 1];
+  cta_sums<T, L, VEC>(logits, in, blockIdx.x, gridDim.x, warp_sums, sums, counts);
+  if (gridDim.x > 1) {
+    cluster_sync_all();
+    if (blockIdx.x == 0) {
+      for (int e = threadIdx.x; e <= in.E; e += kThreads) {
+        float s = e < in.E ? sums[e] : 0.f;
+        int c = counts[e];
+        for (int r = 1; r < (int)gridDim.x; ++r) {
+          uint32_t v;
+          if (e < in.E) {
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(&sums[e]), r)) : "memory");
+            s += __uint_as_float(v);
+          }
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(&counts[e]), r)) : "memory");
+          c += (int)v;
+        }
+        if (e < in.E) sums[e] = s;
+        counts[e] = c;
+      }
+    }
+    cluster_sync_all();  // the others stay until their sums have been read
+  }
+  if (blockIdx.x == 0) write_loss(sums, counts, in.E, in.k, coefficient, loss, counts_out, tokens_out);
+}
+
+template <typename T, typename L, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+    balance_partial_kernel(const T* __restrict__ logits, const BalanceIn in, float* __restrict__ psum,
+                           int32_t* __restrict__ pcount) {
+  __shared__ float warp_sums[kWarps][kMaxE];
+  __shared__ float sums[kMaxE];
+  __shared__ int32_t counts[kMaxE + 1];
+  cta_sums<T, L, VEC>(logits, in, blockIdx.x, gridDim.x, warp_sums, sums, counts);
+  for (int e = threadIdx.x; e <= in.E; e += kThreads) {
+    if (e < in.E) psum[(int64_t)blockIdx.x * in.E + e] = sums[e];
+    pcount[(int64_t)blockIdx.x * (in.E + 1) + e] = counts[e];
+  }
+}
+
+// One CTA: totals over the partials in a fixed order (strands of every n-th CTA, then the
+// strands), then the loss.
 __global__ void __launch_bounds__(1024) balance_loss_kernel(const float* __restrict__ psum,
                                                             const int32_t* __restrict__ pcount, int ctas, int E, int k,
-                                                            float coefficient, float* loss, int32_t* counts,
-                                                            int32_t* tokens) {
+                                                            float coefficient, float* loss, int32_t* counts_out,
+                                                            int32_t* tokens_out) {
   __shared__ float fsum[1024];
   __shared__ int32_t isum[1024];
-  __shared__ int32_t n_tokens;
-  const int strands = 1024 / (E + 1);  // E <= 256
+  __shared__ float sums[kMaxE];
+  __shared__ int32_t counts[kMaxE + 1];
+  pdl_wait();
+  const int strands = 1024 / (E + 1);
   const int e = threadIdx.x % (E + 1), strand = threadIdx.x / (E + 1);
   float s = 0.f;
   int c = 0;
-  if (strand < strands)
+  if (strand < strands) {
+#pragma unroll 8
     for (int i = strand; i < ctas; i += strands) {
-      if (e < E) s += psum[(int64_t)i * E + e];
+      s += e < E ? psum[(int64_t)i * E + e] : 0.f;
       c += pcount[(int64_t)i * (E + 1) + e];
     }
+  }
   fsum[threadIdx.x] = s;
   isum[threadIdx.x] = c;
   __syncthreads();
@@ -140,107 +252,156 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const float* __restr
       s += fsum[w * (E + 1) + e];
       c += isum[w * (E + 1) + e];
     }
-    if (e == E) {
-      n_tokens = c;
-      *tokens = c;
-    } else {
-      counts[e] = c;
-    }
+    if (e < E) sums[e] = s;
+    counts[e] = c;
   }
   __syncthreads();
-  const float n = fmaxf((float)n_tokens, 1.f);
-  fsum[threadIdx.x] = strand == 0 && e < E ? (float)c / (n * (float)k) * (s / n) : 0.f;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    float t = 0.f;
-    for (int i = threadIdx.x; i < E; i += 32) t += fsum[i];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (threadIdx.x == 0) *loss = coefficient * (float)E * t;
-  }
+  write_loss(sums, counts, E, k, coefficient, loss, counts_out, tokens_out);
 }
 
-template <typename T, int LANES, int NJ>
+template <typename T, typename L, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     balance_backward_kernel(const float* __restrict__ grad_loss, const T* __restrict__ logits,
                             const int32_t* __restrict__ counts, const int32_t* __restrict__ tokens,
                             const uint8_t* __restrict__ valid, int64_t T_, int E, int k, float coefficient,
                             T* __restrict__ grad) {
-  constexpr int PER_WARP = 32 / LANES;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LANES - 1), sub = (threadIdx.x & 31) / LANES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & (L::lanes - 1), sub = (threadIdx.x & 31) / L::lanes;
   const float n = fmaxf((float)*tokens, 1.f);
   const float scale = *grad_loss * coefficient * (float)E / n;
-  float f[NJ];
+  float f[L::groups][4];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int e = lane + LANES * j;
-    f[j] = e < E ? (float)counts[e] / (n * (float)k) : 0.f;
-  }
-  const int64_t first = (int64_t)blockIdx.x * kWarps * PER_WARP, step = (int64_t)gridDim.x * kWarps * PER_WARP;
-  for (int64_t t0 = first + warp * PER_WARP; t0 < T_; t0 += step) {
+  for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = (lane + L::lanes * j) * 4 + i;
+      f[j][i] = e < E ? (float)counts[e] / (n * (float)k) : 0.f;
+    }
+  const int64_t step = (int64_t)gridDim.x * kWarps * L::per_warp;
+  for (int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp) * L::per_warp; t0 < T_; t0 += step) {
     const int64_t t = t0 + sub;
     const bool live = t < T_ && (!valid || valid[t]);
-    float x[NJ];
-    load_logits<T, LANES, NJ>(logits, t, live, E, lane, x);
-    softmax_lanes<LANES, NJ>(x);
+    float x[L::groups][4];
+    load_softmax<T, L, VEC>(logits, t, live, E, lane, x);
     float dot = 0.f;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) dot = fmaf(x[j], f[j], dot);
+    for (int j = 0; j < L::groups; ++j)
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (t < T_) {
+      for (int i = 0; i < 4; ++i) dot = fmaf(x[j][i], f[j][i], dot);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int e = lane + LANES * j;
-        if (e < E) grad[t * E + e] = from_f32<T>(live ? scale * x[j] * (f[j] - dot) : 0.f);
+    for (int o = L::lanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (t >= T_) continue;
+    T* out = grad + t * E;
+#pragma unroll
+    for (int j = 0; j < L::groups; ++j) {
+      const int e = (lane + L::lanes * j) * 4;
+      if (e >= E) continue;
+      float g[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = scale * x[j][i] * (f[j][i] - dot);
+      if constexpr (VEC && sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(out + e) = make_float4(g[0], g[1], g[2], g[3]);
+      } else if constexpr (VEC) {
+        T h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = from_f32<T>(g[i]);
+        *reinterpret_cast<uint2*>(out + e) = *reinterpret_cast<const uint2*>(h);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (e + i < E) out[e + i] = from_f32<T>(g[i]);
       }
     }
   }
 }
 
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 2;
 
-int ctas_for(int64_t T, int E) {
-  int lanes = 2;
-  while (lanes < 32 && lanes < E) lanes <<= 1;
-  const int64_t per_cta = (int64_t)kWarps * (32 / lanes);
-  return (int)std::min<int64_t>((T + per_cta - 1) / per_cta, (int64_t)sm_count() * kCtasPerSm);
-}
-
-// Calls f(lanes, experts per lane) as compile-time constants for E experts (E <= 256).
+// Calls f with the layout for E experts as a type.
 template <typename F>
 int with_layout(int E, F&& f) {
-  using std::integral_constant;
-#define SB_LAYOUT(L, J) return f(integral_constant<int, L>{}, integral_constant<int, J>{})
-  if (E <= 2) SB_LAYOUT(2, 1);
-  if (E <= 4) SB_LAYOUT(4, 1);
-  if (E <= 8) SB_LAYOUT(8, 1);
-  if (E <= 16) SB_LAYOUT(16, 1);
-  if (E <= 32) SB_LAYOUT(32, 1);
-  if (E <= 64) SB_LAYOUT(32, 2);
-  if (E <= 128) SB_LAYOUT(32, 4);
-  SB_LAYOUT(32, 8);
-#undef SB_LAYOUT
+  if (E <= 4) return f(Layout<1, 1>{});
+  if (E <= 8) return f(Layout<2, 1>{});
+  if (E <= 16) return f(Layout<4, 1>{});
+  if (E <= 32) return f(Layout<8, 1>{});
+  if (E <= 64) return f(Layout<8, 2>{});
+  if (E <= 128) return f(Layout<8, 4>{});
+  return f(Layout<8, 8>{});
+}
+
+int ctas_for(int64_t T, int E, int64_t most) {
+  int per_warp = 0;
+  with_layout(E, [&](auto l) { return per_warp = decltype(l)::per_warp; });
+  const int64_t per_cta = (int64_t)kWarps * per_warp;
+  return (int)std::min<int64_t>((T + per_cta - 1) / per_cta, most);
+}
+int long_ctas(int64_t T, int E) { return ctas_for(T, E, (int64_t)sm_count() * kCtasPerSm); }
+
+// 4 logits per load: E % 4 == 0 and the rows aligned to it.
+template <typename T>
+bool vectors(const void* logits, const void* grad, int E) {
+  const uintptr_t mask = 4 * sizeof(T) - 1;
+  return E % 4 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(grad)) & mask) == 0;
+}
+
+struct ForwardOut {
+  float* loss;
+  int32_t* counts;
+  int32_t* tokens;
+};
+
+template <typename T, typename L, bool VEC>
+int forward_layout(const T* logits, const BalanceIn& in, float coefficient, const ForwardOut& o, void* scratch,
+                   cudaStream_t stream) {
+  if (in.T * in.E <= kClusterValues) {
+    // a power of two of CTAs with a token group per warp, at least one
+    int ctas = 1;
+    while (ctas < kClusterCtas && ctas < ctas_for(in.T, in.E, kClusterCtas)) ctas <<= 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, balance_cluster_kernel<T, L, VEC>, logits, in, coefficient, o.loss, o.counts,
+                                     o.tokens));
+    count_launch();
+    return STAGEML_OK;
+  }
+  const int grid = long_ctas(in.T, in.E);
+  float* psum = static_cast<float*>(scratch);
+  int32_t* pcount = reinterpret_cast<int32_t*>(psum + (size_t)grid * in.E);
+  SB_CUDA_CHECK(launch_kernel(balance_partial_kernel<T, L, VEC>, dim3((unsigned)grid), dim3(kThreads), 0, stream, false,
+                              logits, in, psum, pcount));
+  count_launch();
+  SB_CUDA_CHECK(launch_kernel(balance_loss_kernel, dim3(1), dim3(1024), 0, stream, true, (const float*)psum,
+                              (const int32_t*)pcount, grid, in.E, in.k, coefficient, o.loss, o.counts, o.tokens));
+  count_launch();
+  return STAGEML_OK;
 }
 
 template <typename T>
-int forward(const void* logits, const void* ids, int ids_i64, const uint8_t* valid, int64_t T_, int E, int k,
-            float* psum, int32_t* pcount, int grid, int32_t* status, cudaStream_t stream) {
-  return with_layout(E, [&](auto lanes, auto nj) {
-    SB_CUDA_CHECK(launch_kernel(balance_sums_kernel<T, decltype(lanes)::value, decltype(nj)::value>,
-                                dim3((unsigned)grid), dim3(kThreads), 0, stream, false, static_cast<const T*>(logits),
-                                ids, ids_i64, valid, T_, E, k, psum, pcount, status));
-    count_launch();
-    return (int)STAGEML_OK;
+int forward(const void* logits, const BalanceIn& in, float coefficient, const ForwardOut& o, void* scratch,
+            cudaStream_t stream) {
+  const T* x = static_cast<const T*>(logits);
+  return with_layout(in.E, [&](auto l) {
+    using L = decltype(l);
+    return vectors<T>(x, nullptr, in.E) ? forward_layout<T, L, true>(x, in, coefficient, o, scratch, stream)
+                                        : forward_layout<T, L, false>(x, in, coefficient, o, scratch, stream);
   });
 }
 
 template <typename T>
 int backward(const float* grad_loss, const void* logits, const int32_t* counts, const int32_t* tokens,
-             const uint8_t* valid, int64_t T_, int E, int k, float coefficient, void* grad, int grid,
-             cudaStream_t stream) {
-  return with_layout(E, [&](auto lanes, auto nj) {
-    SB_CUDA_CHECK(launch_kernel(balance_backward_kernel<T, decltype(lanes)::value, decltype(nj)::value>,
+             const uint8_t* valid, int64_t T_, int E, int k, float coefficient, void* grad, cudaStream_t stream) {
+  const int grid = ctas_for(T_, E, (int64_t)sm_count() * 4);
+  const bool vec = vectors<T>(logits, grad, E);
+  return with_layout(E, [&](auto l) {
+    using L = decltype(l);
+    SB_CUDA_CHECK(launch_kernel(vec ? balance_backward_kernel<T, L, true> : balance_backward_kernel<T, L, false>,
                                 dim3((unsigned)grid), dim3(kThreads), 0, stream, false, grad_loss,
                                 static_cast<const T*>(logits), counts, tokens, valid, T_, E, k, coefficient,
                                 static_cast<T*>(grad)));
@@ -251,38 +412,29 @@ int backward(const float* grad_loss, const void* logits, const int32_t* counts, 
 
 }  // namespace
 
-size_t balance_scratch_bytes(int64_t T, int E) { return (size_t)std::max(ctas_for(T, E), 1) * (2 * E + 1) * 4; }
+size_t balance_scratch_bytes(int64_t T, int E) {
+  return T * E <= kClusterValues ? 0 : (size_t)long_ctas(T, E) * (2 * E + 1) * 4;
+}
 
 int launch_balance_loss(const void* logits, int dtype, const void* ids, int ids_i64, const uint8_t* valid, int64_t T,
                         int E, int k, float coefficient, float* loss, int32_t* counts, int32_t* tokens,
                         int32_t* status, void* scratch, cudaStream_t stream) {
-  const int grid = ctas_for(T, E);
-  float* psum = static_cast<float*>(scratch);
-  int32_t* pcount = reinterpret_cast<int32_t*>(psum + (size_t)grid * E);
-  if (grid > 0) {
-    if (dtype == STAGEML_F32)
-      SB_TRY(forward<float>(logits, ids, ids_i64, valid, T, E, k, psum, pcount, grid, status, stream));
-    else if (dtype == STAGEML_BF16)
-      SB_TRY(forward<bf16>(logits, ids, ids_i64, valid, T, E, k, psum, pcount, grid, status, stream));
-    else
-      SB_TRY(forward<f16>(logits, ids, ids_i64, valid, T, E, k, psum, pcount, grid, status, stream));
-  }
-  SB_CUDA_CHECK(launch_kernel(balance_loss_kernel, dim3(1), dim3(1024), 0, stream, false, (const float*)psum,
-                              (const int32_t*)pcount, grid, E, k, coefficient, loss, counts, tokens));
-  count_launch();
-  return STAGEML_OK;
+  const BalanceIn in = {ids, ids_i64, valid, T, E, k, status};
+  const ForwardOut o = {loss, counts, tokens};
+  if (dtype == STAGEML_F32) return forward<float>(logits, in, coefficient, o, scratch, stream);
+  if (dtype == STAGEML_BF16) return forward<bf16>(logits, in, coefficient, o, scratch, stream);
+  return forward<f16>(logits, in, coefficient, o, scratch, stream);
 }
 
 int launch_balance_loss_backward(const float* grad_loss, const void* logits, int dtype, const int32_t* counts,
                                  const int32_t* tokens, const uint8_t* valid, int64_t T, int E, int k,
-                                 float coefficient, void* grad_logits, cudaStream_t stream) {
-  const int grid = ctas_for(T, E);
-  if (grid == 0) return STAGEML_OK;
+                                 float coefficient, void* grad, cudaStream_t stream) {
+  if (T == 0) return STAGEML_OK;
   if (dtype == STAGEML_F32)
-    return backward<float>(grad_loss, logits, counts, tokens, valid, T, E, k, coefficient, grad_logits, grid, stream);
+    return backward<float>(grad_loss, logits, counts, tokens, valid, T, E, k, coefficient, grad, stream);
   if (dtype == STAGEML_BF16)
-    return backward<bf16>(grad_loss, logits, counts, tokens, valid, T, E, k, coefficient, grad_logits, grid, stream);
-  return backward<f16>(grad_loss, logits, counts, tokens, valid, T, E, k, coefficient, grad_logits, grid, stream);
+    return backward<bf16>(grad_loss, logits, counts, tokens, valid, T, E, k, coefficient, grad, stream);
+  return backward<f16>(grad_loss, logits, counts, tokens, valid, T, E, k, coefficient, grad, stream);
 }
 
 }  // namespace sb

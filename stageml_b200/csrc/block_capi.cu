@@ -49,6 +49,8 @@ int moe_blocks_validate(const stageml_moe_blocks_args* a, bool check_ptrs) {
   SB_CHECK_ARG(a->H % 16 == 0 && a->I % 16 == 0, "moe_blocks: H=%d and I=%d must be multiples of 16", a->H, a->I);
   SB_CHECK_ARG((int64_t)(a->E + a->n_shared) * 2 * a->I <= 0x7fffffff && (int64_t)(a->E + a->n_shared) * a->H <= 0x7fffffff,
                "moe_blocks: too many weight rows");
+  SB_CHECK_ARG(a->E + a->n_shared <= block_gemm_max_groups(), "moe_blocks: %d experts exceed %d", a->E + a->n_shared,
+               block_gemm_max_groups());
   SB_CHECK_ARG(is16(a->act_dtype), "moe_blocks: act_dtype must be BF16 or F16");
   if (a->k > 0) {
     SB_CHECK_ARG(a->ids_dtype == STAGEML_I32 || a->ids_dtype == STAGEML_I64, "moe_blocks: ids must be int32 or int64");
@@ -93,10 +95,7 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   g.K = a->H;
   g.N = a->I;
   g.swiglu = true;
-  g.tile_group = b.plan.tile_group;
   g.group_offsets = b.plan.group_offsets;
-  g.num_tiles_dev = b.plan.num_tiles;
-  g.tiles_cap = (int)(b.plan.rows_cap / 128);
   g.q_out = b.hq;
   g.q_scale = b.hs;
   g.status = status;
@@ -267,7 +266,7 @@ int stageml_balance_loss(const void* logits, int logits_dtype, const void* ids, 
   SB_CHECK_ARG(ids_dtype == STAGEML_I32 || ids_dtype == STAGEML_I64, "balance_loss: ids must be int32 or int64");
   SB_CHECK_ARG((T == 0 || ids) && loss && counts && tokens, "balance_loss: null pointer");
   const size_t need = balance_scratch_bytes(T, E);
-  if (!workspace || workspace_bytes < need)
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(STAGEML_ERR_WORKSPACE, "balance_loss: workspace of %zu bytes < required %zu", workspace_bytes, need);
   return launch_balance_loss(logits, logits_dtype, ids, ids_dtype == STAGEML_I64, valid, T, E, k, coefficient, loss,
                              counts, tokens, status, workspace, static_cast<cudaStream_t>(stream));

@@ -36,11 +36,9 @@ struct BlockGemmLaunch {
   int K = 0;
   int N = 0;                       // output columns
   bool swiglu = false;
-  // grouped rows (a MoE plan's padded rows); tile_group null: plain rows, all of group 0
-  const int32_t* tile_group = nullptr;
+  // grouped rows (a MoE plan's padded rows): [groups + 1] row offsets, multiples of 128, at most
+  // block_gemm_max_groups() groups; null: plain rows, all of group 0
   const int32_t* group_offsets = nullptr;
-  const int32_t* num_tiles_dev = nullptr;
-  int tiles_cap = 0;
   const float* row_scale = nullptr;
   void* out = nullptr;             // [rows, N] out_dtype (plain)
   int out_dtype = STAGEML_BF16;    // F32, BF16 or F16
@@ -49,6 +47,7 @@ struct BlockGemmLaunch {
   int32_t* status = nullptr;
   bool pdl = false;
 };
+int block_gemm_max_groups();
 int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream);
 
 // block_norm.cu (a.T > 0 rows or none; arguments checked by the C ABI)

@@ -4,37 +4,64 @@
 //   out[r, n] = sum_kb sa[r, kb] * sb[n / 128, kb] * (sum_{k in block kb} a[r, k] * b[n, k])
 //
 // The inner sum of one K block runs on the tensor cores (tcgen05.mma kind::f8f6f4,
-// four K = 32 steps into a fresh fp32 accumulator in TMEM); eight warps then read it,
-// multiply by the block's scale and add it to the tile's sums in their registers.
-// Two TMEM accumulators alternate, so the next block's MMAs run during that read.
+// K = 32 per instruction) into a fresh fp32 accumulator in TMEM; math warps then read it,
+// multiply by the block's scale and add it to the tile's sums in their registers. What
+// bounds such a kernel is the round trip of an accumulator (MMAs, signal, TMEM read,
+// signal), so the 512 TMEM columns are four accumulators of 128 columns in rotation: with
+// two of 256 columns the same tile ran at 1250 to 1700 clocks per K block instead of 512.
 //
-// Tile: 128 rows x 256 columns per CTA, persistent CTAs. Warp 0: TMA producer, warp 1:
-// TMEM allocation and MMA issue, warps 2..9: scaling and epilogue (warp w owns TMEM
-// lanes 32 * (w % 4) and half of the columns, 128 fp32 sums per thread).
+// Pair kernel: a two-CTA cluster computes 256 rows x 256 columns with cta_group::2 MMAs of
+// M = 256, N = 128 (two halves per K block); each CTA stages its own 128 rows of A and
+// half of the B rows (32 KB per K block instead of 48), six stages. Per CTA: warp 0 TMA
+// producer, warps 1 and 3 (even CTA) MMA issue, one half each, warp 2 the K blocks' scales
+// (asynchronous copies to shared memory), warps 4..11 scaling and epilogue: a warp owns 32
+// TMEM lanes of one half, 128 fp32 sums per thread, and reads the next 16 columns while it
+// adds the last 16. Eight warps of 128 sums, not sixteen of 64: a scheduler's budget is 512
+// issue slots per K block, 256 of them the additions, and every warp pays its own waits.
+// The control warps give registers to the math warps. Persistent clusters.
 //
-// SwiGLU: the tile's columns are 128 gate rows and the matching 128 up rows of B; the
-// epilogue forms h = silu(gate) * up in fp32 and writes it as e4m3 codes with one scale
-// per (row, 128 columns), the next product's operand, so h never exists in 16 bits.
+// SwiGLU: half h of a tile is 64 gate rows and the matching 64 up rows of B, so a thread
+// holds the gate and up values of the same columns; the epilogue forms
+// h = silu(gate) * up in fp32 and writes it as e4m3 codes with one scale per (row, 128
+// columns), the next product's operand, so h never exists in 16 bits.
+//
+// Every wait is bounded. No load is multicast.
 #include "block_fp8.h"
 #include "common.cuh"
-#include "grouped_gemm.cuh"
 #include "host_util.h"
 
 namespace sb {
 namespace {
 
-constexpr int BM = 128;
-constexpr int BN = 256;
+constexpr int BM = 128;                  // rows per CTA
+constexpr int BN = 256;                  // columns of a pair tile
 constexpr int BK = 128;                  // e4m3 values = one 128-byte swizzle row = one scale block
+constexpr int NACC = 128;                // columns of one accumulator
 constexpr int A_BYTES = BM * BK;         // 16 KB
-constexpr int B_BYTES = BN * BK;         // 32 KB
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int STAGES = 4;
-constexpr int THREADS = 320;
-constexpr int MATH_WARPS = 8;
-constexpr int TMEM_COLS = 512;           // two 256-column accumulators
-constexpr int kBandTiles = 16;           // plain rows: row tiles that share a pass over the columns
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ + 4 * BM * 4 /*row maxima*/;
+constexpr int B_HALF_BYTES = 64 * BK;    // this CTA's 64 rows of one half: 8 KB
+constexpr int STAGE_BYTES = A_BYTES + 2 * B_HALF_BYTES;
+constexpr int STAGES = 6;
+constexpr int BUFS = 4;                  // TMEM accumulators
+constexpr int TMEM_COLS = BUFS * NACC;
+constexpr int MATH_WARP0 = 4;
+constexpr int HALF_WARPS = 4;            // math warps per half
+constexpr int THREADS = 32 * (MATH_WARP0 + 2 * HALF_WARPS);
+// 384 threads are launched with 168 registers each; 128 x 80 + 256 x 208 is less than the total.
+constexpr int CONTROL_REGS = 80, MATH_REGS = 208;
+static_assert(128 * CONTROL_REGS + 256 * MATH_REGS <= THREADS * 168, "register split");
+// Scales come in groups of four K blocks, so that the math warps wait for them once in four:
+// [128 rows of A][4], then [3 weight scales][4].
+constexpr int GROUP = 4;
+constexpr int SLOTS = 3;
+constexpr int SLOT_FLOATS = (BM + 4) * GROUP;
+constexpr int MAX_GROUPS = 1024;
+constexpr int kBandUnits = 8;            // plain rows: row units that share a pass over the columns
+constexpr int BAR_BYTES = 512;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + BAR_BYTES + 2 * 2 * BM * 4 /*row maxima*/ +
+                           SLOTS * SLOT_FLOATS * 4 + (MAX_GROUPS + 1) * 4;
+static_assert(BUFS == 4, "two halves, two K blocks in flight");
+static_assert(SMEM_BYTES <= 232448, "shared memory per block");
+static_assert((2 * STAGES + 2 * BUFS + 2 + 2 * SLOTS) * 8 + 16 <= BAR_BYTES, "barrier area");
 
 struct Params {
   int K, N, kb;                 // kb = ceil(K / 128)
@@ -42,10 +69,9 @@ struct Params {
   int n_tiles;
   const float* a_scale;
   const float* b_scale;
-  const int32_t* tile_group;
-  const int32_t* group_offsets;
-  const int32_t* num_tiles_dev;
-  int tiles_cap;
+  int vec_scales;               // four scales of a row are one aligned 16-byte load
+  const int32_t* group_offsets; // grouped rows: [groups + 1] padded row offsets; null: plain rows
+  int groups;
   int64_t rows;
   const float* row_scale;
   void* out;
@@ -54,12 +80,18 @@ struct Params {
   int32_t* status;
 };
 
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+__device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -69,28 +101,129 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Asynchronous copy of BYTES (4 or 16) global -> shared, zeros when not valid.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const float* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(valid ? BYTES : 0)
+               : "memory");
+}
+// This thread's arrival on `bar` (counted at its initialisation) once its copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// The wait of a whole warp, which then stays or leaves together. Every lane polls (one
+// instruction for the warp); nothing but the poll and a vote lies on the path of a wait that is
+// already over. Bounded by the SM's clock.
+constexpr uint32_t kWaitClocks = 2000000000u;  // about 1 s
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t abort_flag, int* err, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    uint32_t gone;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(gone) : "r"(abort_flag) : "memory");
+    const bool late = (uint32_t)clock() - t0 > kWaitClocks;
+    if (__any_sync(0xffffffffu, gone || late)) {
+      if (late) {
+        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(1) : "memory");
+        if (err) atomicCAS(err, 0, code);
+      }
+      __syncwarp();
+      return false;
+    }
+  }
+  return true;
+}
+
+// The same for a role of one thread; `also` is a second barrier waited for at the same time, so
+// that the polls' latencies overlap.
+__device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, uint32_t also, uint32_t also_parity,
+                                          uint32_t abort_flag, int* err, int code) {
+  bool a = mbar_try_wait(bar, parity), b = mbar_try_wait(also, also_parity);
+  if (a && b) return true;
+  const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+  while (true) {
+    if (!a) a = mbar_try_wait(bar, parity);
+    if (!b) b = mbar_try_wait(also, also_parity);
+    if (a && b) return true;
+    uint32_t gone;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(gone) : "r"(abort_flag) : "memory");
+    if (gone) return false;
+    if ((uint32_t)clock() - t0 > kWaitClocks) {
+      asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(1) : "memory");
+      if (err) atomicCAS(err, 0, code);
+      return false;
+    }
+  }
+}
+
+// Arrive on a barrier of either CTA where no memory is handed over (tensor-memory reads are
+// ordered by the tcgen05 fences around it): no cluster-scope release, whose flush every K block of every warp would pay for.
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// A work unit: up to `step` consecutive row tiles of one weight group, one column tile.
 struct Unit {
-  int m, n, group;
+  int m, n, group;  // m = first row tile
+  int tiles;        // row tiles of the unit
 };
 
-// Unit u -> (row tile, column tile). All column tiles of a weight group's row tiles (or of
-// a band of plain row tiles) come before the next group, row tiles fastest, so that the
-// CTAs at work at one time share weight tiles and the group's rows stay in L2.
-__device__ __forceinline__ Unit unit_of(const Params& p, int u, int tiles) {
-  Unit w;
-  int first, cnt;
-  if (p.tile_group) {
-    w.group = p.tile_group[u / p.n_tiles];
-    first = p.group_offsets[w.group] / BM;
-    cnt = p.group_offsets[w.group + 1] / BM - first;
-  } else {
-    w.group = 0;
-    first = u / (p.n_tiles * kBandTiles) * kBandTiles;
-    cnt = min(kBandTiles, tiles - first);
+// first[g] = row units of the groups before g (grouped rows), in shared memory; returns the
+// number of row units. One warp.
+__device__ __forceinline__ void group_units(const Params& p, int step, int32_t* first) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += 32) {
+    const int g = g0 + lane;
+    int c = 0;
+    if (g < p.groups) c = ((p.group_offsets[g + 1] - p.group_offsets[g]) / BM + step - 1) / step;
+    int s = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    if (g < p.groups) first[g] = base + s - c;
+    base += __shfl_sync(0xffffffffu, s, 31);
   }
-  const int local = u - first * p.n_tiles;
-  w.n = local / cnt;
-  w.m = first + local - w.n * cnt;
+  if (lane == 0) first[p.groups] = base;
+}
+
+// Unit u -> row tiles and column tile. All column tiles of a weight group's row units (or of
+// a band of plain row units) come before the next group, row units fastest, so that the
+// CTAs at work at one time share weight tiles and the group's rows stay in L2.
+__device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const int32_t* first) {
+  Unit w;
+  if (p.group_offsets) {
+    const int r = u / p.n_tiles;
+    int lo = 0, hi = p.groups - 1;  // the last group with first[g] <= r (empty groups are passed over)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= r)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    const int begin = p.group_offsets[lo] / BM, tiles = p.group_offsets[lo + 1] / BM - begin;
+    const int cnt = first[lo + 1] - first[lo], local = u - first[lo] * p.n_tiles;
+    w.group = lo;
+    w.n = local / cnt;
+    const int m = (local - w.n * cnt) * step;
+    w.m = begin + m;
+    w.tiles = min(step, tiles - m);
+  } else {
+    const int tiles = (int)((p.rows + BM - 1) / BM), all = (tiles + step - 1) / step;
+    const int band = u / (p.n_tiles * kBandUnits) * kBandUnits;
+    const int cnt = min(kBandUnits, all - band), local = u - band * p.n_tiles;
+    w.group = 0;
+    w.n = local / cnt;
+    const int m = (band + local - w.n * cnt) * step;
+    w.m = m;
+    w.tiles = min(step, tiles - m);
+  }
   return w;
 }
 
@@ -126,208 +259,169 @@ __device__ __forceinline__ void store_row16<float>(float* dst, const float* v, i
 // OutT: output element (plain); SWIGLU writes codes and ignores it.
 template <typename OutT, bool SWIGLU>
 __global__ void __launch_bounds__(THREADS, 1)
-    block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                      const Params p) {
+    block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                           const Params p) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* row_max = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + 256);  // [2][2][128]
-  auto full_bar = [&](int s) { return smem_u32(&bars[s]); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * BUFS + 2 + 2 * SLOTS);
+  const uint32_t abort_flag = smem_u32(tmem_slot + 1);
+  uint32_t* row_max = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + BAR_BYTES);  // [2][2][128]
+  float* scales = reinterpret_cast<float*>(row_max + 2 * 2 * BM);                                 // [SLOTS][SLOT_FLOATS]
+  int32_t* first = reinterpret_cast<int32_t*>(scales + SLOTS * SLOT_FLOATS);                      // [groups + 1]
+  auto full_bar = [&](int s) { return smem_u32(&bars[s]); };                // both CTAs' copies (even CTA)
   auto empty_bar = [&](int s) { return smem_u32(&bars[STAGES + s]); };
   auto tfull_bar = [&](int i) { return smem_u32(&bars[2 * STAGES + i]); };
-  auto tempty_bar = [&](int i) { return smem_u32(&bars[2 * STAGES + 2 + i]); };
-  const uint32_t drain_bar = smem_u32(&bars[2 * STAGES + 4]);
-  const uint32_t max_bar = smem_u32(&bars[2 * STAGES + 5]);  // the row maxima of a SwiGLU tile are written
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto tempty_bar = [&](int i) { return smem_u32(&bars[2 * STAGES + BUFS + i]); };  // both CTAs' math (even CTA)
+  const uint32_t drain_bar = smem_u32(&bars[2 * STAGES + 2 * BUFS]);
+  const uint32_t max_bar = smem_u32(&bars[2 * STAGES + 2 * BUFS + 1]);  // the row maxima of a SwiGLU tile are written
+  auto sfull_bar = [&](uint32_t i) { return smem_u32(&bars[2 * STAGES + 2 * BUFS + 2 + i]); };
+  auto sempty_bar = [&](uint32_t i) { return smem_u32(&bars[2 * STAGES + 2 * BUFS + 2 + SLOTS + i]); };
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(empty_bar(s), 2);  // each half's MMAs
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < BUFS; ++i) {
       mbar_init(tfull_bar(i), 1);
-      mbar_init(tempty_bar(i), MATH_WARPS);
+      mbar_init(tempty_bar(i), 2 * HALF_WARPS);
     }
-    mbar_init(drain_bar, 1);
-    mbar_init(max_bar, MATH_WARPS);
-    *abort_flag = 0;
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(sfull_bar(i), 32);  // the copies of every lane of the scale warp
+      mbar_init(sempty_bar(i), 2 * HALF_WARPS);
+    }
+    mbar_init(drain_bar, 2);
+    mbar_init(max_bar, 2 * HALF_WARPS);
+    tmem_slot[1] = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
-    tmem_relinquish();
+    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish_pair();
   }
+  if (warp == 2 && p.group_offsets) group_units(p, 2, first);
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   volatile int never_abort = 0;
 
-  int tiles = p.tiles_cap;
-  if (p.num_tiles_dev) tiles = min(tiles, *p.num_tiles_dev);
-  const int units = tiles * p.n_tiles;
+  const int row_units = p.group_offsets ? first[p.groups] : (int)((p.rows + 2 * BM - 1) / (2 * BM));
+  const int units = row_units * p.n_tiles;
 
-  if (threadIdx.x == 0) {
-    // ------------------------------------------------------------ producer
-    tma_prefetch_desc(&tm_a);
-    tma_prefetch_desc(&tm_b);
-    const uint64_t pol_a = l2_policy_evict_last(), pol_b = l2_policy_evict_normal();
-    const uint32_t base = smem_u32(smem);
-    int last_phase[STAGES];
-    for (int s = 0; s < STAGES; ++s) last_phase[s] = -1;
-    uint32_t it = 0;
-    bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      const Unit w = unit_of(p, u, tiles);
-      const int n0 = w.n * (SWIGLU ? 128 : BN);
-      const int b0 = w.group * p.b_group_rows + n0;
-      const int b1 = SWIGLU ? b0 + p.N : b0 + 128;
-      for (int kb = 0; kb < p.kb; ++kb, ++it) {
-        const int s = it % STAGES;
-        const uint32_t ph = (it / STAGES) & 1;
-        if (!mbar_wait(empty_bar(s), ph ^ 1, abort_flag, p.status, kDefaultWaitNs, kDevTimeoutProducer)) {
-          ok = false;
-          break;
-        }
-        const uint32_t sa = base + s * STAGE_BYTES;
-        mbar_arrive_expect_tx(full_bar(s), STAGE_BYTES);
-        tma_load_2d(sa, &tm_a, full_bar(s), kb * BK, w.m * BM, pol_a);
-        tma_load_2d(sa + A_BYTES, &tm_b, full_bar(s), kb * BK, b0, pol_b);
-        tma_load_2d(sa + A_BYTES + B_BYTES / 2, &tm_b, full_bar(s), kb * BK, b1, pol_b);
-        last_phase[s] = (int)ph;
-      }
-    }
-    if (!ok) {  // let the copies in flight land before the CTA leaves
-      for (int s = 0; s < STAGES; ++s)
-        if (last_phase[s] >= 0)
-          mbar_wait(full_bar(s), (uint32_t)last_phase[s], &never_abort, p.status, 200000000ull, kDevTimeoutDrain);
-    }
-  } else if (threadIdx.x == 32) {
-    // ------------------------------------------------------------ MMA issuer
-    constexpr uint32_t idesc = idesc_e4m3(BM, BN);
-    const uint32_t base = smem_u32(smem);
-    uint32_t it = 0;
-    bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      for (int kb = 0; kb < p.kb; ++kb, ++it) {
-        const int s = it % STAGES, acc = it & 1;
-        if (!mbar_wait(tempty_bar(acc), ((it >> 1) & 1) ^ 1, abort_flag, p.status, kDefaultWaitNs, kDevTimeoutMma) ||
-            !mbar_wait(full_bar(s), (it / STAGES) & 1, abort_flag, p.status, kDefaultWaitNs, kDevTimeoutMma)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint64_t ad = smem_desc_sw128(base + s * STAGE_BYTES);
-        const uint64_t bd = smem_desc_sw128(base + s * STAGE_BYTES + A_BYTES);
-#pragma unroll
-        for (int k = 0; k < BK / 32; ++k) mma_f8(tmem_base + acc * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0 ? 1u : 0u);
-        tc_commit(empty_bar(s));
-        tc_commit(tfull_bar(acc));
-      }
-    }
-    // every MMA has stopped reading shared memory before the CTA leaves
-    tc_commit(drain_bar);
-    mbar_wait(drain_bar, 0, &never_abort, p.status, 1000000000ull, kDevTimeoutDrain);
-  } else if (warp >= 2) {
+  if (warp >= MATH_WARP0) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MATH_REGS));
     // ------------------------------------------------------------ scaling and epilogue
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, half = (warp - MATH_WARP0) / HALF_WARPS;
     const int row_in_tile = quarter * 32 + lane;
-    const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    // TMEM column of this thread's 16-column chunk c. Plain: columns [128 half, 128 half + 128).
-    // SwiGLU: chunks 0-3 gate columns [64 half, +64), chunks 4-7 the same up columns.
-    auto col_of = [&](int c) { return SWIGLU ? (c & 4) * 32 + 64 * half + 16 * (c & 3) : 128 * half + 16 * c; };
+    // this thread's lane of its half's accumulator: all 128 columns (SwiGLU: 64 gate, the same 64 up)
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * NACC;
+    const uint32_t lead_tempty = mapa_shared(tempty_bar(0), 0);
     const bool vec = p.N % (16 / (int)sizeof(OutT)) == 0;
-    uint32_t it = 0, tile = 0;
+    uint32_t it = 0, grp = 0, tile = 0;
+    const float* slot = scales;
     bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++tile) {
-      const Unit w = unit_of(p, u, tiles);
-      const int64_t row = (int64_t)w.m * BM + row_in_tile;
-      const bool row_ok = row < p.rows;
-      const float* sa = p.a_scale + (row_ok ? row : 0) * p.kb;
-      // weight scales: one per tile half (plain), gate and up (SwiGLU). The up rows start at
-      // N inside the group, so a tile's up columns can straddle two 128-row scale blocks:
-      // columns below `cut` take the first, the others the second (N % 16 == 0).
-      const float *sb0, *sb1, *sb2;
-      int cut = 128;
-      {
-        const float* g = p.b_scale + (int64_t)w.group * p.b_blocks * p.kb;
-        if (SWIGLU) {
-          const int up = p.N + w.n * 128;
-          cut = 128 - (up & 127);
-          sb0 = g + (int64_t)w.n * p.kb;
-          sb1 = g + (int64_t)min(up >> 7, p.b_blocks - 1) * p.kb;
-          sb2 = g + (int64_t)min((up >> 7) + 1, p.b_blocks - 1) * p.kb;
-        } else {
-          sb0 = sb1 = sb2 = g + (int64_t)min(2 * w.n + half, p.b_blocks - 1) * p.kb;
-        }
-      }
+    for (int u = cluster; ok && u < units; u += clusters, ++tile) {
+      const Unit w = unit_of(p, u, 2, first);
+      const int64_t row = (int64_t)(w.m + rank) * BM + row_in_tile;
+      const bool row_ok = rank < w.tiles && row < p.rows;
+      // The up rows start at N inside the group, so a tile's up columns can straddle two 128-row
+      // scale blocks: the columns below `cut` take the first, the others the second. N % 16 == 0,
+      // so 16 columns share a scale.
+      const int cut = SWIGLU ? 128 - ((p.N + w.n * 128) & 127) - 64 * half : 0;
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
       for (int kb = 0; kb < p.kb; ++kb, ++it) {
-        const float xa = row_ok ? __ldg(sa + kb) : 0.f;
-        const float s0 = xa * __ldg(sb0 + kb);
-        float s1 = s0, s2 = s0;
-        if (SWIGLU) {
-          s1 = xa * __ldg(sb1 + kb);
-          s2 = xa * __ldg(sb2 + kb);
+        const uint32_t buf = (it & 1) * 2 + half;
+        if (kb % GROUP == 0) {
+          ok = warp_wait(sfull_bar(grp % SLOTS), (grp / SLOTS) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
+          if (!ok) break;
+          slot = scales + grp % SLOTS * SLOT_FLOATS;
         }
-        const int buf = it & 1;
-        // the whole warp stays or leaves: tcgen05.ld is warp-collective
-        ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(buf), (it >> 1) & 1, abort_flag, p.status, kDefaultWaitNs,
-                                               kDevTimeoutEpilogue));
+        const float xa = slot[row_in_tile * GROUP + kb % GROUP];
+        const float* wb = slot + BM * GROUP + kb % GROUP;
+        const float b0 = wb[SWIGLU ? 0 : half * GROUP], b1 = SWIGLU ? wb[GROUP] : 0.f, b2 = SWIGLU ? wb[2 * GROUP] : 0.f;
+        ok = warp_wait(tfull_bar(buf), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
         if (!ok) break;
         tc_fence_after();
+        const uint32_t src = t_lane + (it & 1) * 2 * NACC;
+        // 32 and 16 columns in turn: one run is read while the other is added
+        uint32_t t[32], v[16];
+        tmem_ld_x32(src, t);
+        const float s0 = xa * b0, s1 = SWIGLU ? xa * b1 : s0, s2 = SWIGLU ? xa * b2 : s0;
+        auto scale_of = [&](int col) { return SWIGLU && col >= 64 ? (col - 64 < cut ? s1 : s2) : s0; };
+        auto add16 = [&](int col, const uint32_t* r) {
+          const float sc = scale_of(col);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t t[16];
-          tmem_ld_x16(t_lane + buf * BN + col_of(c), t);
-          tmem_wait_ld();
-          const float s = SWIGLU && c >= 4 ? (64 * half + 16 * (c - 4) < cut ? s1 : s2) : s0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(s, __uint_as_float(t[i]), acc[16 * c + i]);
-        }
+          for (int i = 0; i < 16; ++i) acc[col + i] = fmaf(sc, __uint_as_float(r[i]), acc[col + i]);
+        };
+        tmem_wait_ld();
+        tmem_ld_x16(src + 32, v);
+        add16(0, t), add16(16, t + 16);
+        tmem_wait_ld();
+        tmem_ld_x32(src + 48, t);
+        add16(32, v);
+        tmem_wait_ld();
+        tmem_ld_x16(src + 80, v);
+        add16(48, t), add16(64, t + 16);
+        tmem_wait_ld();
+        tmem_ld_x32(src + 96, t);
+        add16(80, v);
+        tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(buf));
+        if (lane == 0) arrive_remote(lead_tempty + 8u * buf);
+        add16(96, t), add16(112, t + 16);
+        if (kb % GROUP == GROUP - 1 || kb == p.kb - 1) {  // the group's scales have been read
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty_bar(grp % SLOTS));
+          ++grp;
+        }
       }
       if (!ok) break;
       if (SWIGLU) {
         const int n0 = w.n * 128 + 64 * half;
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          acc[i] = n0 + i < p.N ? silu_f32(acc[i]) * acc[64 + i] : 0.f;
+        for (int i = 0; i < 64; ++i) {  // h takes the gate values' place
+          acc[i] = n0 + i < p.N ? __fdividef(acc[i], 1.f + __expf(-acc[i])) * acc[64 + i] : 0.f;
           m = max(m, __float_as_uint(acc[i]) & 0x7fffffffu);
         }
         // the row's maximum over both halves; two buffers, so that one barrier per tile is enough
         // (a warp writes a buffer again only after every warp has read it and come to the next tile)
-        uint32_t* mine = row_max + (tile & 1) * 2 * BM;
-        mine[half * BM + row_in_tile] = m;
+        uint32_t* mine = row_max + (tile & 1) * 2 * BM + row_in_tile;
+        mine[half * BM] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(max_bar);
-        ok = __all_sync(0xffffffffu, mbar_wait(max_bar, tile & 1, abort_flag, p.status, kDefaultWaitNs,
-                                               kDevTimeoutEpilogue));
+        ok = warp_wait(max_bar, tile & 1, abort_flag, p.status, kDevTimeoutEpilogue);
         if (!ok) break;
-        m = max(m, mine[(half ^ 1) * BM + row_in_tile]);
+        m = max(m, mine[(half ^ 1) * BM]);
         float s = __uint_as_float(m) / 448.0f;
         s = s == 0.f ? 1.f : s;
+        // h never leaves in another form, so its codes may come from the reciprocal: the quotient
+        // is off by an ulp of fp32 at most, 2^-20 of an e4m3 step
+        const float inv = 1.f / s;
         if (row_ok) {
           uint8_t* q = p.q_out + row * p.N + n0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (n0 + 16 * c < p.N) {  // N % 16 == 0: a chunk is inside or outside
+            if (n0 + 16 * c < p.N) {  // N % 16 == 0: 16 columns are inside or outside
               uint32_t v[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float* f = acc + 16 * c + 4 * i;
-                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0] / s, f[1] / s), __NV_SATFINITE, __NV_E4M3);
-                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2] / s, f[3] / s), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t lo =
+                    __nv_cvt_float2_to_fp8x2(make_float2(f[0] * inv, f[1] * inv), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi =
+                    __nv_cvt_float2_to_fp8x2(make_float2(f[2] * inv, f[3] * inv), __NV_SATFINITE, __NV_E4M3);
                 v[i] = lo | hi << 16;
               }
               *reinterpret_cast<uint4*>(q + 16 * c) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -348,26 +442,158 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONTROL_REGS));
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (one thread)
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_a);
+      tma_prefetch_desc(&tm_b);
+      const uint64_t pol_a = l2_policy_evict_last(), pol_b = l2_policy_evict_normal();
+      const uint32_t base = smem_u32(smem);
+      const uint32_t lead_full = mapa_shared(full_bar(0), 0);
+      uint32_t s = 0, phase = 0, filled = 0;  // filled: bit i = stage i has been filled
+      bool ok = true;
+      for (int u = cluster; ok && u < units; u += clusters) {
+        const Unit w = unit_of(p, u, 2, first);
+        const int n0 = w.n * (SWIGLU ? 128 : BN);
+        // B rows of half 0; half 1 is `next` rows on
+        const int b0 = w.group * p.b_group_rows + n0 + rank * (SWIGLU ? p.N : 64);
+        const int next = SWIGLU ? 64 : 128;
+        const int a0 = (w.m + rank) * BM;
+        const bool live = rank < w.tiles;  // an idle half multiplies what its stage holds; nobody stores it
+        const uint32_t bytes = (w.tiles * A_BYTES) + 4 * B_HALF_BYTES;  // of both CTAs
+        for (int kb = 0; kb < p.kb; ++kb) {
+          ok = lane_wait(empty_bar(s), phase ^ 1, empty_bar(s), phase ^ 1, abort_flag, p.status, kDevTimeoutProducer);
+          if (!ok) break;
+          const uint32_t dst = base + s * STAGE_BYTES, bar = lead_full + 8u * s;
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), bytes);
+          if (live) tma_load_2d_pair(dst, &tm_a, bar, kb * BK, a0, pol_a);
+          tma_load_2d_pair(dst + A_BYTES, &tm_b, bar, kb * BK, b0, pol_b);
+          tma_load_2d_pair(dst + A_BYTES + B_HALF_BYTES, &tm_b, bar, kb * BK, b0 + next, pol_b);
+          filled |= 1u << s;
+          if (++s == STAGES) s = 0, phase ^= 1;
+        }
+      }
+      if (!ok) {
+        // Let the copies in flight land before the CTA pair leaves. The odd CTA's complete on the
+        // even CTA's barrier; it waits a fixed, ample time.
+        if (rank == 0) {
+          for (uint32_t i = 0; i < STAGES; ++i)  // stages before s were filled in this phase, the others in the last
+            if (filled >> i & 1)
+              mbar_wait(full_bar(i), i < s ? phase : phase ^ 1, &never_abort, p.status, 200000000ull, kDevTimeoutDrain);
+        } else {
+          const unsigned long long t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 200000ull) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1 || warp == 3) {
+    // ------------------------------------------------------------ MMA issue, one half (one thread)
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_e4m3(2 * BM, NACC);
+      const uint32_t half = warp >> 1;
+      const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
+      const uint32_t b_off = (A_BYTES + half * B_HALF_BYTES) >> 4;
+      uint32_t s = 0, phase = 0, it = 0;
+      bool ok = true;
+      for (int u = cluster; ok && u < units; u += clusters) {
+        for (int kb = 0; kb < p.kb; ++kb, ++it) {
+          const uint32_t buf = (it & 1) * 2 + half;
+          ok = lane_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, full_bar(s), phase, abort_flag, p.status, kDevTimeoutMma);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = desc0 + (uint64_t)(s * (STAGE_BYTES >> 4)), bd = ad + b_off;
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma_f8_pair(tmem_base + buf * NACC, ad + 2 * k, bd + 2 * k, idesc, k > 0 ? 1u : 0u);
+          tc_commit_pair_both(tfull_bar(buf), 0x3);
+          tc_commit_pair_both(empty_bar(s), 0x3);
+          if (++s == STAGES) s = 0, phase ^= 1;
+        }
+      }
+      // every MMA of this thread has stopped reading shared memory before the CTAs leave
+      tc_commit_pair(drain_bar);
+      mbar_wait(drain_bar, 0, &never_abort, p.status, 1000000000ull, kDevTimeoutDrain);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ scales
+    // Every lane copies the scales of four rows (32 i + lane), lanes 0..2 also one weight scale
+    // each: plain, the tile's two halves; SwiGLU, gate, then the one or two 128-row blocks that
+    // the up rows touch. 16-byte copies where a row's scales allow them.
+    const uint32_t slots = smem_u32(scales);
+    uint32_t grp = 0;
+    bool ok = true;
+    for (int u = cluster; ok && u < units; u += clusters) {
+      const Unit w = unit_of(p, u, 2, first);
+      const int64_t row0 = (int64_t)(w.m + rank) * BM + lane;
+      const int valid = rank < w.tiles ? (int)min((int64_t)BM, p.rows - row0) : 0;  // row 32 i + lane: 32 i < valid
+      const float* sa = p.a_scale + (valid > 0 ? row0 : 0) * p.kb;
+      int block = 2 * w.n + (lane & 1);
+      if (SWIGLU) block = lane == 0 ? w.n : ((p.N + w.n * 128) >> 7) + (lane == 2);
+      const float* sb = p.b_scale + ((int64_t)w.group * p.b_blocks + min(block, p.b_blocks - 1)) * p.kb;
+      for (int kb = 0; kb < p.kb; kb += GROUP, ++grp) {
+        const uint32_t sl = grp % SLOTS;
+        ok = warp_wait(sempty_bar(sl), ((grp / SLOTS) & 1) ^ 1, abort_flag, p.status, kDevTimeoutProducer);
+        if (!ok) break;
+        const uint32_t dst = slots + sl * (SLOT_FLOATS * 4) + 16 * lane;
+        if (p.vec_scales) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            copy_async<16>(dst + 512 * i, 32 * i < valid ? sa + (int64_t)(32 * i) * p.kb + kb : p.a_scale,
+                           32 * i < valid);
+          if (lane < 3) copy_async<16>(dst + 16 * BM, sb + kb, true);
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < GROUP && kb + j < p.kb; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              copy_async<4>(dst + 512 * i + 4 * j, 32 * i < valid ? sa + (int64_t)(32 * i) * p.kb + kb + j : p.a_scale,
+                            32 * i < valid);
+            if (lane < 3) copy_async<4>(dst + 16 * BM + 4 * j, sb + kb + j, true);
+          }
+        }
+        copies_arrive(sfull_bar(sl));
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
   }
   __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
   }
 }
 
 template <typename OutT, bool SWIGLU>
-int run(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int grid, bool pdl, cudaStream_t stream) {
-  auto kernel = block_gemm_kernel<OutT, SWIGLU>;
+int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int clusters, bool pdl, cudaStream_t stream) {
+  auto kernel = block_gemm_pair_kernel<OutT, SWIGLU>;
   SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
-  SB_CUDA_CHECK(launch_kernel(kernel, dim3((unsigned)grid), dim3(THREADS), SMEM_BYTES, stream, pdl, ta, tb, p));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * clusters);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, p));
   count_launch();
   return STAGEML_OK;
 }
 
 }  // namespace
+
+int block_gemm_max_groups() { return MAX_GROUPS; }
 
 int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   if (g.a_rows == 0 || g.N == 0) return STAGEML_OK;
@@ -380,11 +606,10 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   p.n_tiles = g.swiglu ? (int)scale_blocks(g.N) : (g.N + BN - 1) / BN;
   p.a_scale = g.a_scale;
   p.b_scale = g.b_scale;
-  p.tile_group = g.tile_group;
+  p.vec_scales = p.kb % GROUP == 0 && (reinterpret_cast<uintptr_t>(g.a_scale) | reinterpret_cast<uintptr_t>(g.b_scale)) % 16 == 0;
   p.group_offsets = g.group_offsets;
-  p.num_tiles_dev = g.num_tiles_dev;
+  p.groups = g.groups;
   p.rows = g.a_rows;
-  p.tiles_cap = g.tile_group ? g.tiles_cap : (int)((g.a_rows + BM - 1) / BM);
   p.row_scale = g.row_scale;
   p.out = g.out;
   p.q_out = g.q_out;
@@ -394,14 +619,17 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   SB_TRY(make_tmap_2d(&ta, g.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.a_rows, (uint64_t)g.K, (uint64_t)g.K, BM,
                       BK, 128));
   SB_TRY(make_tmap_2d(&tb, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.groups * p.b_group_rows, (uint64_t)g.K,
-                      (uint64_t)g.K, 128, BK, 128));
-  const int64_t units = (int64_t)p.tiles_cap * p.n_tiles;
+                      (uint64_t)g.K, 64, BK, 128));
+  // row units: every group can end in a unit of one tile
+  const int64_t tiles = (g.a_rows + BM - 1) / BM;
+  const int64_t row_units = g.group_offsets ? std::min<int64_t>(tiles, tiles / 2 + g.groups) : (tiles + 1) / 2;
+  const int64_t units = row_units * p.n_tiles;
   SB_CHECK_ARG(units <= 0x7fffffff, "block_gemm: too many tiles");
-  const int grid = (int)(units < sm_count() ? units : sm_count());
-  if (g.swiglu) return run<bf16, true>(ta, tb, p, grid, g.pdl, stream);
-  if (g.out_dtype == STAGEML_F32) return run<float, false>(ta, tb, p, grid, g.pdl, stream);
-  if (g.out_dtype == STAGEML_BF16) return run<bf16, false>(ta, tb, p, grid, g.pdl, stream);
-  return run<f16, false>(ta, tb, p, grid, g.pdl, stream);
+  const int clusters = (int)std::min<int64_t>(units, sm_count() / 2);
+  if (g.swiglu) return run_pair<bf16, true>(ta, tb, p, clusters, g.pdl, stream);
+  if (g.out_dtype == STAGEML_F32) return run_pair<float, false>(ta, tb, p, clusters, g.pdl, stream);
+  if (g.out_dtype == STAGEML_BF16) return run_pair<bf16, false>(ta, tb, p, clusters, g.pdl, stream);
+  return run_pair<f16, false>(ta, tb, p, clusters, g.pdl, stream);
 }
 
 }  // namespace sb

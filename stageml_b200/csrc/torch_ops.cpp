@@ -539,68 +539,104 @@ Tensor moe_forward_blocks(const Tensor& x, const Tensor& gate_up, const Tensor& 
   return out;
 }
 
-// The arguments that the forward and the backward share; gate_mode 0 none, 1 [H], 2 [T], 3 [T, H].
-void norm_args(stageml_norm_args* a, const c10::optional<Tensor>& block_out, const Tensor& residual,
-               const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate, int64_t gate_mode,
-               const c10::optional<Tensor>& pre_weight, double residual_scale, double eps, at::ScalarType block_dtype) {
-  TORCH_CHECK(residual.dim() == 2, "norm_residual: residual must be [T, H]");
-  check_cuda(residual, "residual", residual);
+// How a gate is broadcast over a residual [..., H]: per channel [H] (or [1, .., H]), per
+// token [..., 1], or full.
+int gate_mode_of(const Tensor& gate, const Tensor& residual) {
+  const auto rs = residual.sizes(), gs = gate.sizes();
+  if (gs == rs) return STAGEML_GATE_FULL;
+  if (!gs.empty() && gs.back() == rs.back() && gate.numel() == rs.back()) return STAGEML_GATE_CHANNEL;
+  if (gs.size() == rs.size() && gs.back() == 1 && gs.slice(0, gs.size() - 1) == rs.slice(0, rs.size() - 1))
+    return STAGEML_GATE_TOKEN;
+  TORCH_CHECK(false, "norm_residual: gate ", gs, " must be [H], [..., 1] or [..., H] for a residual ", rs);
+  return -1;
+}
+
+// The inputs that the forward and the backward share, made contiguous, and their arguments.
+struct NormInputs {
+  c10::optional<Tensor> block_out, post, gate, pre;
+  Tensor residual;
+  stageml_norm_args a{};
+};
+
+c10::optional<Tensor> norm_input(const c10::optional<Tensor>& t, const Tensor& residual, const char* name) {
+  if (!t.has_value()) return c10::nullopt;
+  TORCH_CHECK(t->is_cuda() && t->device() == residual.device(), "norm_residual: ", name, " must be on ",
+              residual.device(), ", got ", t->device());
+  check_float_dtype(*t, name);
+  return t->contiguous();
+}
+
+void norm_inputs(NormInputs* n, const c10::optional<Tensor>& block_out, const Tensor& residual,
+                 const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
+                 const c10::optional<Tensor>& pre_weight, double residual_scale, double eps,
+                 at::ScalarType block_dtype) {
+  TORCH_CHECK(residual.is_cuda(), "norm_residual: residual must be a CUDA tensor");
+  TORCH_CHECK(residual.dim() >= 1, "norm_residual: residual must be [..., H]");
   check_float_dtype(residual, "norm_residual: residual");
-  const int64_t T = residual.size(0), H = residual.size(1);
+  const int64_t H = residual.size(-1);
+  TORCH_CHECK(H >= 1 && H <= INT32_MAX, "norm_residual: bad width ", H);
+  n->residual = residual.contiguous();
+  n->block_out = norm_input(block_out, residual, "block_out");
+  n->post = norm_input(post_weight, residual, "post_weight");
+  n->gate = norm_input(gate, residual, "gate");
+  n->pre = norm_input(pre_weight, residual, "pre_weight");
   if (block_out.has_value()) {
-    check_cuda(*block_out, "block_out", residual);
     TORCH_CHECK(block_out->sizes() == residual.sizes(), "norm_residual: block_out must have residual's shape");
     TORCH_CHECK(block_out->scalar_type() == block_dtype, "norm_residual: block_out must be ", block_dtype);
   }
-  for (const auto* w : {&post_weight, &pre_weight})
-    if (w->has_value()) {
-      check_cuda(**w, "weight", residual);
-      check_float_dtype(**w, "norm_residual: weight");
-      TORCH_CHECK((*w)->dim() == 1 && (*w)->size(0) == H, "norm_residual: a norm weight must be [H]");
-    }
-  if (gate.has_value()) {
-    check_cuda(*gate, "gate", residual);
-    check_float_dtype(*gate, "norm_residual: gate");
-    const int64_t need = gate_mode == STAGEML_GATE_CHANNEL ? H : gate_mode == STAGEML_GATE_TOKEN ? T : T * H;
-    TORCH_CHECK(gate->numel() == need, "norm_residual: gate does not match its mode");
-  }
-  a->T = T;
-  TORCH_CHECK(H >= 1 && H <= INT32_MAX, "norm_residual: bad width ", H);
-  a->H = (int)H;
-  a->resid_dtype = dtype_code(residual);
-  a->block_dtype = block_dtype == at::kFloat ? STAGEML_F32 : block_dtype == at::kBFloat16 ? STAGEML_BF16
-                   : block_dtype == at::kHalf ? STAGEML_F16 : -1;
-  a->residual = residual.data_ptr();
-  a->block_out = opt_ptr(block_out);
-  a->post_weight = opt_ptr(post_weight);
-  a->post_dtype = post_weight.has_value() ? dtype_code(*post_weight) : STAGEML_F32;
-  a->gate = opt_ptr(gate);
-  a->gate_mode = gate.has_value() ? (int)gate_mode : STAGEML_GATE_NONE;
-  a->gate_dtype = gate.has_value() ? dtype_code(*gate) : STAGEML_F32;
-  a->pre_weight = opt_ptr(pre_weight);
-  a->pre_dtype = pre_weight.has_value() ? dtype_code(*pre_weight) : STAGEML_F32;
-  a->residual_scale = (float)residual_scale;
-  a->eps = (float)eps;
+  for (const auto* w : {&n->post, &n->pre})
+    if (w->has_value())
+      TORCH_CHECK((*w)->dim() == 1 && (*w)->size(0) == H, "norm_residual: a norm weight must be [H], got ",
+                  (*w)->sizes());
+  stageml_norm_args& a = n->a;
+  a.T = residual.numel() / H;
+  a.H = (int)H;
+  a.resid_dtype = dtype_code(residual);
+  a.block_dtype = block_dtype == at::kFloat      ? STAGEML_F32
+                  : block_dtype == at::kBFloat16 ? STAGEML_BF16
+                  : block_dtype == at::kHalf     ? STAGEML_F16
+                                                 : -1;
+  a.residual = n->residual.data_ptr();
+  a.block_out = opt_ptr(n->block_out);
+  a.post_weight = opt_ptr(n->post);
+  a.post_dtype = n->post.has_value() ? dtype_code(*n->post) : STAGEML_F32;
+  a.gate = opt_ptr(n->gate);
+  a.gate_mode = n->gate.has_value() ? gate_mode_of(*gate, residual) : STAGEML_GATE_NONE;
+  a.gate_dtype = n->gate.has_value() ? dtype_code(*n->gate) : STAGEML_F32;
+  a.pre_weight = opt_ptr(n->pre);
+  a.pre_dtype = n->pre.has_value() ? dtype_code(*n->pre) : STAGEML_F32;
+  a.residual_scale = (float)residual_scale;
+  a.eps = (float)eps;
+  a.status = status_word(residual);
 }
 
 // -> [new_residual], [new_residual, normed] or [new_residual, codes, scale]
 std::vector<Tensor> norm_residual(const c10::optional<Tensor>& block_out, const Tensor& residual,
                                   const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
-                                  int64_t gate_mode, const c10::optional<Tensor>& pre_weight, double residual_scale,
-                                  double eps, bool quantize, at::ScalarType normed_dtype) {
-  stageml_norm_args a{};
-  norm_args(&a, block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale, eps, normed_dtype);
+                                  const c10::optional<Tensor>& pre_weight, double residual_scale, double eps,
+                                  bool quantize, c10::optional<at::ScalarType> normed_dtype) {
+  const at::ScalarType bd = block_out.has_value()      ? block_out->scalar_type()
+                            : normed_dtype.has_value() ? *normed_dtype
+                                                       : residual.scalar_type();
+  TORCH_CHECK(!normed_dtype.has_value() || *normed_dtype == bd, "norm_residual: normed_dtype must be block_out's dtype");
+  NormInputs n;
+  norm_inputs(&n, block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, bd);
+  stageml_norm_args& a = n.a;
   TORCH_CHECK(!quantize || pre_weight.has_value(), "norm_residual: quantize needs pre_weight");
   c10::cuda::CUDAGuard guard(residual.device());
-  std::vector<Tensor> out{at::empty_like(residual)};
+  std::vector<Tensor> out;
+  out.reserve(3);
+  out.push_back(at::empty(residual.sizes(), residual.options()));
   a.new_residual = out[0].data_ptr();
   if (quantize) {
+    auto sizes = residual.sizes().vec();
+    sizes.back() = blocks128(a.H);
     out.push_back(at::empty(residual.sizes(), residual.options().dtype(at::kFloat8_e4m3fn)));
-    out.push_back(at::empty({a.T, blocks128(a.H)}, residual.options().dtype(at::kFloat)));
+    out.push_back(at::empty(sizes, residual.options().dtype(at::kFloat)));
     a.codes = static_cast<uint8_t*>(out[1].data_ptr());
     a.code_scale = out[2].data_ptr<float>();
   } else if (pre_weight.has_value()) {
-    out.push_back(at::empty(residual.sizes(), residual.options().dtype(normed_dtype)));
+    out.push_back(at::empty(residual.sizes(), residual.options().dtype(bd)));
     a.normed = out[1].data_ptr();
   }
   const size_t bytes = stageml_norm_residual_workspace_bytes(&a, 0);
@@ -614,46 +650,35 @@ std::vector<Tensor> norm_residual_backward(const c10::optional<Tensor>& grad_res
                                            const c10::optional<Tensor>& grad_normed,
                                            const c10::optional<Tensor>& block_out, const Tensor& residual,
                                            const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
-                                           int64_t gate_mode, const c10::optional<Tensor>& pre_weight,
-                                           double residual_scale, double eps) {
+                                           const c10::optional<Tensor>& pre_weight, double residual_scale, double eps) {
   TORCH_CHECK(grad_residual.has_value() || grad_normed.has_value(), "norm_residual_backward: no gradient given");
   const at::ScalarType bd = block_out.has_value()     ? block_out->scalar_type()
                             : grad_normed.has_value() ? grad_normed->scalar_type()
                                                       : residual.scalar_type();
-  stageml_norm_args a{};
-  norm_args(&a, block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale, eps, bd);
-  if (grad_residual.has_value()) {
-    check_cuda(*grad_residual, "grad_residual", residual);
-    TORCH_CHECK(grad_residual->sizes() == residual.sizes() && grad_residual->scalar_type() == residual.scalar_type(),
-                "norm_residual_backward: grad_residual must match residual");
-  }
-  if (grad_normed.has_value()) {
-    check_cuda(*grad_normed, "grad_normed", residual);
-    TORCH_CHECK(grad_normed->sizes() == residual.sizes() && grad_normed->scalar_type() == bd,
-                "norm_residual_backward: grad_normed must have residual's shape and the block dtype");
-    TORCH_CHECK(pre_weight.has_value(), "norm_residual_backward: grad_normed without pre_weight");
-  }
+  NormInputs n;
+  norm_inputs(&n, block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, bd);
+  stageml_norm_args& a = n.a;
+  const auto dr = norm_input(grad_residual, residual, "grad_residual");
+  const auto dz = norm_input(grad_normed, residual, "grad_normed");
+  TORCH_CHECK(!dr.has_value() || (dr->sizes() == residual.sizes() && dr->scalar_type() == residual.scalar_type()),
+              "norm_residual_backward: grad_residual must match residual");
+  TORCH_CHECK(!dz.has_value() || (dz->sizes() == residual.sizes() && dz->scalar_type() == bd),
+              "norm_residual_backward: grad_normed must have residual's shape and the block dtype");
+  TORCH_CHECK(!dz.has_value() || pre_weight.has_value(), "norm_residual_backward: grad_normed without pre_weight");
   c10::cuda::CUDAGuard guard(residual.device());
-  a.grad_residual = opt_ptr(grad_residual);
-  a.grad_normed = opt_ptr(grad_normed);
-  std::vector<Tensor> out{at::empty_like(residual)};
-  a.d_residual = out[0].data_ptr();
-  if (block_out.has_value()) {
-    out.push_back(at::empty_like(*block_out));
-    a.d_block_out = out.back().data_ptr();
-  }
-  if (post_weight.has_value()) {
-    out.push_back(at::empty_like(*post_weight));
-    a.d_post = out.back().data_ptr();
-  }
-  if (gate.has_value()) {
-    out.push_back(at::empty_like(*gate));
-    a.d_gate = out.back().data_ptr();
-  }
-  if (pre_weight.has_value()) {
-    out.push_back(at::empty_like(*pre_weight));
-    a.d_pre = out.back().data_ptr();
-  }
+  a.grad_residual = opt_ptr(dr);
+  a.grad_normed = opt_ptr(dz);
+  std::vector<Tensor> out;
+  out.reserve(5);
+  auto add = [&](const Tensor& like) {
+    out.push_back(at::empty(like.sizes(), like.options()));
+    return out.back().data_ptr();
+  };
+  a.d_residual = add(residual);
+  if (block_out.has_value()) a.d_block_out = add(*block_out);
+  if (post_weight.has_value()) a.d_post = add(*post_weight);
+  if (gate.has_value()) a.d_gate = add(*gate);
+  if (pre_weight.has_value()) a.d_pre = add(*pre_weight);
   const size_t bytes = stageml_norm_residual_workspace_bytes(&a, 1);
   Tensor ws = bytes ? workspace(bytes, residual) : Tensor();
   check_rc(stageml_norm_residual_backward(&a, bytes ? ws.data_ptr() : nullptr, bytes, cur_stream()),
@@ -684,10 +709,11 @@ std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, const Tens
   auto loss = at::empty({}, logits.options().dtype(at::kFloat));
   auto counts = at::empty({E}, logits.options().dtype(at::kInt));
   auto tokens = at::empty({}, logits.options().dtype(at::kInt));
-  auto w = workspace(stageml_balance_workspace_bytes(T, (int)E), logits);
+  const size_t bytes = stageml_balance_workspace_bytes(T, (int)E);
+  Tensor w = bytes ? workspace(bytes, logits) : Tensor();
   check_rc(stageml_balance_loss(logits.data_ptr(), dtype_code(logits), topk_ids.data_ptr(), dtype_code(topk_ids), v, T,
                                 (int)E, (int)k, (float)coefficient, loss.data_ptr<float>(), counts.data_ptr<int32_t>(),
-                                tokens.data_ptr<int32_t>(), status_word(logits), w.data_ptr(), (size_t)w.numel(),
+                                tokens.data_ptr<int32_t>(), status_word(logits), bytes ? w.data_ptr() : nullptr, bytes,
                                 cur_stream()),
            "balance_loss");
   return {loss, counts, tokens};
@@ -756,11 +782,11 @@ TORCH_LIBRARY(stageml, m) {
       "moe_forward_blocks(Tensor x, Tensor gate_up, Tensor gate_up_scale, Tensor down, Tensor down_scale, "
       "Tensor? topk_ids, Tensor? topk_weights, int n_shared) -> Tensor");
   m.def(
-      "norm_residual(Tensor? block_out, Tensor residual, Tensor? post_weight, Tensor? gate, int gate_mode, "
-      "Tensor? pre_weight, float residual_scale, float eps, bool quantize, ScalarType normed_dtype) -> Tensor[]");
+      "norm_residual(Tensor? block_out, Tensor residual, Tensor? post_weight, Tensor? gate, "
+      "Tensor? pre_weight, float residual_scale, float eps, bool quantize, ScalarType? normed_dtype) -> Tensor[]");
   m.def(
       "norm_residual_backward(Tensor? grad_residual, Tensor? grad_normed, Tensor? block_out, Tensor residual, "
-      "Tensor? post_weight, Tensor? gate, int gate_mode, Tensor? pre_weight, float residual_scale, float eps) "
+      "Tensor? post_weight, Tensor? gate, Tensor? pre_weight, float residual_scale, float eps) "
       "-> Tensor[]");
   m.def("balance_loss(Tensor logits, Tensor topk_ids, float coefficient, Tensor? valid) -> (Tensor, Tensor, Tensor)");
   m.def(
@@ -788,4 +814,13 @@ TORCH_LIBRARY_IMPL(stageml, CUDA, m) {
   m.impl("norm_residual_backward", &norm_residual_backward);
   m.impl("balance_loss", &balance_loss);
   m.impl("balance_loss_backward", &balance_loss_backward);
+}
+
+// The operators above without an autograd formula of their own in the dispatcher: ops.py
+// wraps the differentiable ones in autograd functions and refuses gradients for the others,
+// so the dispatcher's generic autograd kernel (several us per call) is passed by.
+TORCH_LIBRARY_IMPL(stageml, Autograd, m) {
+  for (const char* op : {"quantize_e4m3_blocks", "block_matmul", "moe_forward_blocks", "norm_residual",
+                         "norm_residual_backward", "balance_loss", "balance_loss_backward"})
+    m.impl(op, torch::CppFunction::makeFallthrough());
 }

@@ -16,6 +16,14 @@ from ._native import ensure_cuda_device, load_torch_ops
 
 load_torch_ops()
 _ops = torch.ops.stageml
+# overloads resolved once: the calls below are launch-bound for small batches
+_quantize_e4m3_blocks = _ops.quantize_e4m3_blocks.default
+_block_matmul = _ops.block_matmul.default
+_moe_forward_blocks = _ops.moe_forward_blocks.default
+_norm_residual = _ops.norm_residual.default
+_norm_residual_backward = _ops.norm_residual_backward.default
+_balance_loss = _ops.balance_loss.default
+_balance_loss_backward = _ops.balance_loss_backward.default
 
 
 def _register_fakes() -> None:
@@ -85,19 +93,20 @@ def _register_fakes() -> None:
         return x.new_empty(x.shape)
 
     @lib.register_fake("stageml::norm_residual")
-    def _(block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale, eps, quantize, normed_dtype):
-        out = [torch.empty_like(residual)]
+    def _(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, quantize, normed_dtype=None):
+        shape = tuple(residual.shape)
+        out = [residual.new_empty(shape)]
         if quantize:
-            out.append(residual.new_empty(residual.shape, dtype=torch.float8_e4m3fn))
-            out.append(residual.new_empty((residual.shape[0], blocks(residual.shape[1])), dtype=torch.float32))
+            out.append(residual.new_empty(shape, dtype=torch.float8_e4m3fn))
+            out.append(residual.new_empty(shape[:-1] + (blocks(shape[-1]),), dtype=torch.float32))
         elif pre_weight is not None:
-            out.append(residual.new_empty(residual.shape, dtype=normed_dtype))
+            dtype = block_out.dtype if block_out is not None else normed_dtype or residual.dtype
+            out.append(residual.new_empty(shape, dtype=dtype))
         return out
 
     @lib.register_fake("stageml::norm_residual_backward")
-    def _(grad_residual, grad_normed, block_out, residual, post_weight, gate, gate_mode, pre_weight, residual_scale,
-          eps):
-        return [torch.empty_like(t) for t in (residual, block_out, post_weight, gate, pre_weight) if t is not None]
+    def _(grad_residual, grad_normed, block_out, residual, post_weight, gate, pre_weight, residual_scale, eps):
+        return [t.new_empty(t.shape) for t in (residual, block_out, post_weight, gate, pre_weight) if t is not None]
 
     @lib.register_fake("stageml::balance_loss")
     def _(logits, topk_ids, coefficient, valid):
@@ -218,7 +227,8 @@ def quantize_e4m3_blocks(x, tiles: bool = False):
     128 x 128 tile. scale = max|x| / 448 (1 for a block of zeros), q = e4m3(x / scale), nearest even.
     """
     ensure_cuda_device(x)
-    return _ops.quantize_e4m3_blocks(x.contiguous(), bool(tiles))
+    _no_grad("quantize_e4m3_blocks", x)
+    return _quantize_e4m3_blocks(x.contiguous(), tiles)
 
 
 def block_matmul(x, x_scale, w, w_scale, out_dtype=torch.bfloat16):
@@ -228,7 +238,7 @@ def block_matmul(x, x_scale, w, w_scale, out_dtype=torch.bfloat16):
     ``quantize_e4m3_blocks`` (tiles False / True) makes them; K a multiple of 16. -> [M, N].
     """
     ensure_cuda_device(x)
-    return _ops.block_matmul(x.contiguous(), x_scale.contiguous(), w.contiguous(), w_scale.contiguous(), out_dtype)
+    return _block_matmul(x.contiguous(), x_scale.contiguous(), w.contiguous(), w_scale.contiguous(), out_dtype)
 
 
 def moe_forward_blocks(x, gate_up, gate_up_scale, down, down_scale, *, topk_ids=None, topk_weights=None,
@@ -242,27 +252,9 @@ def moe_forward_blocks(x, gate_up, gate_up_scale, down, down_scale, *, topk_ids=
     take ``moe_forward``.
     """
     ensure_cuda_device(x)
-    return _ops.moe_forward_blocks(x.contiguous(), gate_up, gate_up_scale, down, down_scale, topk_ids, topk_weights,
-                                   int(n_shared))
-
-
-def _rows(t):
-    return None if t is None else t.reshape(-1, t.shape[-1]).contiguous()
-
-
-def _gate_mode(gate, residual) -> int:
-    """0 none, 1 per channel [H] or [1, .., H], 2 per token [..., 1], 3 full."""
-    if gate is None:
-        return 0
-    H = residual.shape[-1]
-    if gate.shape == residual.shape:
-        return 3
-    if gate.numel() == H and gate.shape[-1:] == residual.shape[-1:]:
-        return 1
-    if gate.shape == residual.shape[:-1] + (1,):
-        return 2
-    raise ValueError(f"norm_residual: gate {tuple(gate.shape)} must be [H], [..., 1] or [..., H] for a residual "
-                     f"{tuple(residual.shape)}")
+    _no_grad("moe_forward_blocks", x, topk_weights)
+    return _moe_forward_blocks(x.contiguous(), gate_up, gate_up_scale, down, down_scale, topk_ids, topk_weights,
+                               n_shared)
 
 
 def norm_residual_backward(grad_residual, grad_normed, block_out, residual, *, post_weight=None, gate=None,
@@ -273,11 +265,22 @@ def norm_residual_backward(grad_residual, grad_normed, block_out, residual, *, p
     has its input's shape and dtype; sums over tokens are fp32 in a fixed order.
     """
     ensure_cuda_device(residual)
-    inputs = (residual, block_out, post_weight, gate, pre_weight)
-    out = iter(_ops.norm_residual_backward(_rows(grad_residual), _rows(grad_normed), _rows(block_out), _rows(residual),
-                                           post_weight, None if gate is None else gate.contiguous(),
-                                           _gate_mode(gate, residual), pre_weight, float(residual_scale), float(eps)))
-    return tuple(None if t is None else next(out).view(t.shape) for t in inputs)
+    out = iter(_norm_residual_backward(grad_residual, grad_normed, block_out, residual, post_weight, gate, pre_weight,
+                                       residual_scale, eps))
+    return (next(out), None if block_out is None else next(out), None if post_weight is None else next(out),
+            None if gate is None else next(out), None if pre_weight is None else next(out))
+
+
+def _any_grad(*tensors) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _no_grad(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and _any_grad(*tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 class _NormResidual(torch.autograd.Function):
@@ -286,8 +289,8 @@ class _NormResidual(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(block_out, residual, post_weight, gate, pre_weight)
         ctx.numbers = {"residual_scale": residual_scale, "eps": eps}
-        return _norm_residual(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, False,
-                              normed_dtype)
+        return tuple(_norm_residual(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, False,
+                                    normed_dtype))
 
     @staticmethod
     def backward(ctx, *grads):
@@ -296,14 +299,6 @@ class _NormResidual(torch.autograd.Function):
         d = norm_residual_backward(grads[0], grad_normed, block_out, residual, post_weight=post_weight, gate=gate,
                                    pre_weight=pre_weight, **ctx.numbers)
         return d[1], d[0], d[2], d[3], d[4], None, None, None
-
-
-def _norm_residual(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, quantize, normed_dtype):
-    out = _ops.norm_residual(_rows(block_out), _rows(residual), post_weight,
-                             None if gate is None else gate.contiguous(), _gate_mode(gate, residual), pre_weight,
-                             float(residual_scale), float(eps), bool(quantize), normed_dtype)
-    shape = residual.shape
-    return tuple(t.view(shape[:-1] + t.shape[-1:]) for t in out)
 
 
 def norm_residual(block_out, residual, *, post_weight=None, gate=None, residual_scale: float = 1.0, pre_weight=None,
@@ -322,20 +317,19 @@ def norm_residual(block_out, residual, *, post_weight=None, gate=None, residual_
     Differentiable, except with quantize. H <= 16384.
     """
     ensure_cuda_device(residual)
-    if normed_dtype is None or block_out is not None:
-        normed_dtype = (residual if block_out is None else block_out).dtype
-    tensors = (block_out, residual, post_weight, gate, pre_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and _any_grad(block_out, residual, post_weight, gate, pre_weight):
         if quantize:
             raise ValueError("norm_residual: the codes of quantize=True carry no gradient")
-        return _NormResidual.apply(*tensors, residual_scale, eps, normed_dtype)
-    return _norm_residual(*tensors, residual_scale, eps, quantize, normed_dtype)
+        return _NormResidual.apply(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps,
+                                   normed_dtype)
+    return tuple(_norm_residual(block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, quantize,
+                                normed_dtype))
 
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topk_ids, coefficient, valid):
-        loss, counts, tokens = _ops.balance_loss(logits, topk_ids, coefficient, valid)
+        loss, counts, tokens = _balance_loss(logits, topk_ids, coefficient, valid)
         ctx.save_for_backward(logits, counts, tokens, valid)
         ctx.numbers = (topk_ids.shape[1], coefficient)
         ctx.mark_non_differentiable(counts, tokens)
@@ -358,15 +352,14 @@ def balance_loss(logits, topk_ids, coefficient: float = 1.0, *, valid=None):
     ensure_cuda_device(logits)
     logits, topk_ids = logits.contiguous(), topk_ids.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _BalanceLoss.apply(logits, topk_ids, float(coefficient), valid)
-    return _ops.balance_loss(logits, topk_ids, float(coefficient), valid)
+        return _BalanceLoss.apply(logits, topk_ids, coefficient, valid)
+    return _balance_loss(logits, topk_ids, coefficient, valid)
 
 
 def balance_loss_backward(grad_loss, logits, counts, tokens, k: int, coefficient: float = 1.0, *, valid=None):
     """Gradient of ``balance_loss``'s logits for grad_loss (CUDA fp32 scalar), from the forward's counts and tokens."""
     ensure_cuda_device(logits)
-    return _ops.balance_loss_backward(grad_loss.contiguous(), logits.contiguous(), counts, tokens, int(k),
-                                      float(coefficient), valid)
+    return _balance_loss_backward(grad_loss.contiguous(), logits.contiguous(), counts, tokens, k, coefficient, valid)
 
 
 def combine_rows(y, pair_row, T: int, kk: int):
