@@ -326,7 +326,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lead_tempty = mapa_shared(tempty_bar(0), 0);
     const bool vec = p.N % (16 / (int)sizeof(OutT)) == 0;
     uint32_t it = 0, grp = 0, tile = 0;
-    const float* slot = scales;
     bool ok = true;
     for (int u = cluster; ok && u < units; u += clusters, ++tile) {
       const Unit w = unit_of(p, u, 2, first);
@@ -339,51 +338,74 @@ __global__ void __launch_bounds__(THREADS, 1)
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-      for (int kb = 0; kb < p.kb; ++kb, ++it) {
-        const uint32_t buf = (it & 1) * 2 + half;
-        if (kb % GROUP == 0) {
-          ok = warp_wait(sfull_bar(grp % SLOTS), (grp / SLOTS) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
-          if (!ok) break;
-          slot = scales + grp % SLOTS * SLOT_FLOATS;
-        }
-        const float xa = slot[row_in_tile * GROUP + kb % GROUP];
-        const float* wb = slot + BM * GROUP + kb % GROUP;
-        const float b0 = wb[SWIGLU ? 0 : half * GROUP], b1 = SWIGLU ? wb[GROUP] : 0.f, b2 = SWIGLU ? wb[2 * GROUP] : 0.f;
-        ok = warp_wait(tfull_bar(buf), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t src = t_lane + (it & 1) * 2 * NACC;
-        // 32 and 16 columns in turn: one run is read while the other is added
-        uint32_t t[32], v[16];
-        tmem_ld_x32(src, t);
-        const float s0 = xa * b0, s1 = SWIGLU ? xa * b1 : s0, s2 = SWIGLU ? xa * b2 : s0;
-        auto scale_of = [&](int col) { return SWIGLU && col >= 64 ? (col - 64 < cut ? s1 : s2) : s0; };
-        auto add16 = [&](int col, const uint32_t* r) {
-          const float sc = scale_of(col);
+      // Runs of 16 and 32 columns in turn: one is read while the other is added. The first run of
+      // the next K block is read before the last one of this block is added, so that neither its
+      // wait nor its latency lies between two K blocks that are both there.
+      uint32_t t[32], v[16];
+      auto scale_for = [&](int col, float c0, float c1, float c2) { return SWIGLU && col >= 64 ? (col - 64 < cut ? c1 : c2) : c0; };
+      auto add16 = [&](int col, const uint32_t* r, float sc) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[col + i] = fmaf(sc, __uint_as_float(r[i]), acc[col + i]);
-        };
-        tmem_wait_ld();
-        tmem_ld_x16(src + 32, v);
-        add16(0, t), add16(16, t + 16);
-        tmem_wait_ld();
-        tmem_ld_x32(src + 48, t);
-        add16(32, v);
-        tmem_wait_ld();
-        tmem_ld_x16(src + 80, v);
-        add16(48, t), add16(64, t + 16);
-        tmem_wait_ld();
-        tmem_ld_x32(src + 96, t);
-        add16(80, v);
-        tmem_wait_ld();
-        tc_fence_before();
+        for (int i = 0; i < 16; ++i) acc[col + i] = fmaf(sc, __uint_as_float(r[i]), acc[col + i]);
+      };
+      ok = warp_wait(tfull_bar((it & 1) * 2 + half), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
+      for (int kb0 = 0; ok && kb0 < p.kb; kb0 += GROUP) {
+        const uint32_t sl = grp % SLOTS;
+        ok = warp_wait(sfull_bar(sl), (grp / SLOTS) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
+        if (!ok) break;
+        const float* slot = scales + sl * SLOT_FLOATS;
+        float s0[GROUP], s1[GROUP], s2[GROUP];
+        {
+          const float4 xa = *reinterpret_cast<const float4*>(slot + row_in_tile * GROUP);
+          const float4* wb = reinterpret_cast<const float4*>(slot + BM * GROUP);
+          const float4 w0 = wb[SWIGLU ? 0 : half];
+          s0[0] = xa.x * w0.x, s0[1] = xa.y * w0.y, s0[2] = xa.z * w0.z, s0[3] = xa.w * w0.w;
+          if (SWIGLU) {
+            const float4 w1 = wb[1], w2 = wb[2];
+            s1[0] = xa.x * w1.x, s1[1] = xa.y * w1.y, s1[2] = xa.z * w1.z, s1[3] = xa.w * w1.w;
+            s2[0] = xa.x * w2.x, s2[1] = xa.y * w2.y, s2[2] = xa.z * w2.z, s2[3] = xa.w * w2.w;
+          }
+        }
         __syncwarp();
-        if (lane == 0) arrive_remote(lead_tempty + 8u * buf);
-        add16(96, t), add16(112, t + 16);
-        if (kb % GROUP == GROUP - 1 || kb == p.kb - 1) {  // the group's scales have been read
-          __syncwarp();
-          if (lane == 0) mbar_arrive(sempty_bar(grp % SLOTS));
-          ++grp;
+        if (lane == 0) mbar_arrive(sempty_bar(sl));
+        ++grp;
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+          if (kb0 + j >= p.kb) break;
+          const uint32_t buf = (it & 1) * 2 + half;
+          const uint32_t src = t_lane + (it & 1) * 2 * NACC;
+          auto add = [&](int col, const uint32_t* r) {
+            add16(col, r, scale_for(col, s0[j], SWIGLU ? s1[j] : 0.f, SWIGLU ? s2[j] : 0.f));
+          };
+          tmem_wait_ld();
+          tmem_ld_x32(src + 16, t);
+          add(0, v);
+          tmem_wait_ld();
+          tmem_ld_x16(src + 48, v);
+          add(16, t), add(32, t + 16);
+          tmem_wait_ld();
+          tmem_ld_x32(src + 64, t);
+          add(48, v);
+          tmem_wait_ld();
+          tmem_ld_x16(src + 96, v);
+          add(64, t), add(80, t + 16);
+          tmem_wait_ld();
+          uint32_t last[16];
+          tmem_ld_x16(src + 112, last);
+          add(96, v);
+          tmem_wait_ld();
+          tc_fence_before();
+          if (lane == 0) arrive_remote(lead_tempty + 8u * buf);
+          ++it;
+          if (kb0 + j + 1 < p.kb) {
+            ok = warp_wait(tfull_bar(buf ^ 2), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
+            if (!ok) break;
+            tc_fence_after();
+            tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
+          }
+          add(112, last);
         }
       }
       if (!ok) break;
