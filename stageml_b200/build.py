@@ -38,6 +38,7 @@ CU_SOURCES = [
     "fp8.cu",
     "quantize_blocks.cu",
     "block_gemm.cu",
+    "block_skinny.cu",
     "block_norm.cu",
     "balance.cu",
     "block_capi.cu",

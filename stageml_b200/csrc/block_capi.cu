@@ -16,12 +16,16 @@ struct MoeBlocksBuffers {
   void* perm = nullptr;
   uint8_t* xq = nullptr;     // [rows_cap, H] codes of the permuted rows
   float* xs = nullptr;       // [rows_cap, ceil(H/128)]
+  float* h = nullptr;        // few rows: [rows_cap, I] silu(gate) * up in fp32
   uint8_t* hq = nullptr;     // [rows_cap, I] codes of silu(gate) * up
   float* hs = nullptr;       // [rows_cap, ceil(I/128)]
   void* y = nullptr;         // [rows_cap, H] weighted rows of the down projection
   int32_t* status = nullptr;
   size_t bytes = 0;
 };
+
+// At most kSkinnyRows tokens: no expert has more rows than that (a token names an expert once).
+bool moe_blocks_skinny(const stageml_moe_blocks_args* a) { return a->T <= kSkinnyRows; }
 
 void moe_blocks_carve(const stageml_moe_blocks_args* a, void* ws, MoeBlocksBuffers* b) {
   Carver c(ws);
@@ -32,6 +36,7 @@ void moe_blocks_carve(const stageml_moe_blocks_args* a, void* ws, MoeBlocksBuffe
   b->perm = c.take_bytes(permute_scratch_bytes(P, permute_num_keys(0, 0, 0, E_tot)));
   b->xq = c.take<uint8_t>(rows * a->H);
   b->xs = c.take<float>(rows * scale_blocks(a->H));
+  if (moe_blocks_skinny(a)) b->h = c.take<float>(rows * a->I);
   b->hq = c.take<uint8_t>(rows * a->I);
   b->hs = c.take<float>(rows * scale_blocks(a->I));
   b->y = c.take_bytes(rows * a->H * 2);
@@ -79,12 +84,15 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   int32_t* status = a->status ? a->status : b.status;
   PermuteScratch scr;
   permute_carve(b.perm, P, permute_num_keys(0, 0, 0, E_tot), &scr);
+  const int slots = a->k + a->n_shared;
+  const bool skinny = moe_blocks_skinny(a), pdl = pdl_enabled();
   SB_STAGE(STAGEML_STAGE_PERMUTE,
            launch_permute(a->topk_ids, a->ids_dtype, a->topk_weights, a->weights_dtype, nullptr, a->T, a->k,
-                          a->n_shared, E_tot, 0, 0, b.plan, status, scr, st));
+                          a->n_shared, E_tot, 0, 0, b.plan, status, scr, st, nullptr, pdl));
+  // few rows: codes by token, the product finds a plan row's token; else by plan row
   SB_STAGE(STAGEML_STAGE_GATHER_SHRINK,
-           launch_quantize_block_rows(a->x, a->act_dtype, b.plan.rows_cap, a->H, b.plan.row_token, b.plan.num_tiles,
-                                      b.xq, b.xs, st));
+           launch_quantize_block_rows(a->x, a->act_dtype, a->T, a->H, skinny ? nullptr : b.plan.pair_row,
+                                      skinny ? 0 : slots, b.xq, b.xs, st, pdl));
   BlockGemmLaunch g;
   g.a = b.xq;
   g.a_scale = b.xs;
@@ -99,7 +107,22 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   g.q_out = b.hq;
   g.q_scale = b.hs;
   g.status = status;
-  SB_STAGE(STAGEML_STAGE_GEMM_GATE_UP, launch_block_gemm(g, st));
+  g.pdl = pdl;
+  BlockSkinny sk;
+  if (skinny) {
+    sk.max_rows = a->T;
+    sk.row_map = b.plan.row_token;
+    sk.tile_group = b.plan.tile_group;
+    sk.group_counts = b.plan.group_counts;
+    sk.num_tiles = b.plan.num_tiles;
+    sk.tiles_cap = (int)std::min<int64_t>(b.plan.rows_cap / 128, E_tot);
+    g.out = b.h;
+    SB_STAGE(STAGEML_STAGE_GEMM_GATE_UP, launch_block_skinny(g, sk, st));
+    SB_STAGE(STAGEML_STAGE_SHRINK_H, launch_quantize_block_pairs(b.h, b.plan.pair_row, P, a->I, b.hq, b.hs, st, pdl));
+    sk.row_map = nullptr;
+  } else {
+    SB_STAGE(STAGEML_STAGE_GEMM_GATE_UP, launch_block_gemm(g, st));
+  }
   g.a = b.hq;
   g.a_scale = b.hs;
   g.b = a->down;
@@ -110,9 +133,9 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   g.row_scale = b.plan.row_weight;
   g.out = b.y;
   g.out_dtype = a->act_dtype;
-  SB_STAGE(STAGEML_STAGE_GEMM_DOWN, launch_block_gemm(g, st));
-  SB_STAGE(STAGEML_STAGE_COMBINE, launch_combine(b.y, b.plan.pair_row, a->T, a->k + a->n_shared, a->H,
-                                                 a->act_dtype == STAGEML_BF16, a->out, st));
+  SB_STAGE(STAGEML_STAGE_GEMM_DOWN, skinny ? launch_block_skinny(g, sk, st) : launch_block_gemm(g, st));
+  SB_STAGE(STAGEML_STAGE_COMBINE, launch_combine(b.y, b.plan.pair_row, a->T, slots, a->H,
+                                                 a->act_dtype == STAGEML_BF16, a->out, st, nullptr, pdl));
   return STAGEML_OK;
 }
 
@@ -185,7 +208,7 @@ int stageml_quantize_e4m3_blocks(const void* x, int dtype, int64_t batch, int64_
   SB_CHECK_ARG(is_float(dtype), "quantize_e4m3_blocks: x must be F32, BF16 or F16");
   if (batch == 0 || rows == 0 || cols == 0) return STAGEML_OK;
   SB_CHECK_ARG(x && q_out && scale_out, "quantize_e4m3_blocks: null pointer");
-  if (!tiles) return launch_quantize_block_rows(x, dtype, batch * rows, cols, nullptr, nullptr, q_out, scale_out, st);
+  if (!tiles) return launch_quantize_block_rows(x, dtype, batch * rows, cols, nullptr, 0, q_out, scale_out, st);
   SB_CHECK_ARG(batch * scale_blocks(rows) * scale_blocks(cols) <= 0x7fffffff, "quantize_e4m3_blocks: too many tiles");
   return launch_quantize_block_tiles(x, dtype, batch, rows, cols, q_out, scale_out, st);
 }
@@ -220,7 +243,13 @@ int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* 
   g.out = out;
   g.out_dtype = out_dtype;
   g.status = status;
-  SB_STAGE(STAGEML_STAGE_GEMM, launch_block_gemm(g, st));
+  if (M <= kSkinnyRows) {
+    BlockSkinny sk;
+    sk.max_rows = M;
+    SB_STAGE(STAGEML_STAGE_GEMM, launch_block_skinny(g, sk, st));
+  } else {
+    SB_STAGE(STAGEML_STAGE_GEMM, launch_block_gemm(g, st));
+  }
   return STAGEML_OK;
 }
 

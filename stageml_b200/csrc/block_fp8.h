@@ -13,11 +13,13 @@ inline int64_t scale_blocks(int64_t n) { return (n + kScaleBlock - 1) / kScaleBl
 // quantize_blocks.cu: e4m3 codes with one fp32 scale per 128 values of a row
 // (scale [rows, ceil(cols/128)]) or per 128 x 128 tile of each of `batch` matrices
 // (scale [batch, ceil(rows/128), ceil(cols/128)]).
-// row_of (rows mode, optional): output row r holds source row row_of[r]; rows with
-// row_of[r] < 0 and rows past 128 * (*num_tiles_dev) are left unwritten.
-int launch_quantize_block_rows(const void* x, int dtype, int64_t rows, int64_t cols, const int32_t* row_of,
-                               const int32_t* num_tiles_dev, uint8_t* q, float* scale, cudaStream_t stream,
-                               bool pdl = false);
+// slots > 0: source row r is written to the output rows out_row[slots * r + j], j < slots (a MoE
+// plan's pair_row; negative ones are left out).
+int launch_quantize_block_rows(const void* x, int dtype, int64_t rows, int64_t cols, const int32_t* out_row, int slots,
+                               uint8_t* q, float* scale, cudaStream_t stream, bool pdl = false);
+// fp32 rows row[p] of x (negative: skipped) to the same rows of q and scale; cols % 8 == 0.
+int launch_quantize_block_pairs(const float* x, const int32_t* row, int64_t pairs, int64_t cols, uint8_t* q,
+                                float* scale, cudaStream_t stream, bool pdl);
 int launch_quantize_block_tiles(const void* w, int dtype, int64_t batch, int64_t rows, int64_t cols, uint8_t* q,
                                 float* scale, cudaStream_t stream);
 
@@ -47,6 +49,19 @@ struct BlockGemmLaunch {
   int32_t* status = nullptr;
   bool pdl = false;
 };
+// block_skinny.cu: the same product for at most kSkinnyRows rows per weight group, streaming the
+// weights. swiglu: writes silu(gate) * up in fp32 to g.out. Grouped rows need the plan's tiles (a
+// group's rows all lie in one tile); row_map (optional) names the row of `a` of each plan row.
+constexpr int kSkinnyRows = 16;
+struct BlockSkinny {
+  int max_rows = 0;                       // at most kSkinnyRows; plain rows: their number
+  const int32_t* row_map = nullptr;
+  const int32_t* tile_group = nullptr;
+  const int32_t* group_counts = nullptr;
+  const int32_t* num_tiles = nullptr;
+  int tiles_cap = 0;
+};
+int launch_block_skinny(const BlockGemmLaunch& g, const BlockSkinny& s, cudaStream_t stream);
 int block_gemm_max_groups();
 int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream);
 

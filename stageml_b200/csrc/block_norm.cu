@@ -662,7 +662,7 @@ int launch_norm_residual(const stageml_norm_args& a, void* scratch, cudaStream_t
   const bool two_step = a.codes && !vectors(a);
   SB_TRY(launch_any(a, false, two_step ? static_cast<float*>(scratch) : nullptr, stream));
   if (two_step)
-    return launch_quantize_block_rows(scratch, STAGEML_F32, a.T, a.H, nullptr, nullptr, a.codes, a.code_scale, stream);
+    return launch_quantize_block_rows(scratch, STAGEML_F32, a.T, a.H, nullptr, 0, a.codes, a.code_scale, stream);
   return STAGEML_OK;
 }
 

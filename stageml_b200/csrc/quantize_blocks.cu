@@ -68,41 +68,89 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t c, int64_t col
   }
 }
 
+// A half-warp takes kUnits neighbouring blocks of the flattened (row, block) list per round, all
+// loaded before the first is encoded.
+constexpr int kUnits = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_block_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
-                                                                  const int32_t* __restrict__ row_of,
-                                                                  const int32_t* __restrict__ num_tiles_dev,
+                                                                  const int32_t* __restrict__ out_row, int slots,
                                                                   uint8_t* __restrict__ q, float* __restrict__ scale) {
   pdl_wait();
   pdl_trigger();
   const int64_t nb = (cols + 127) / 128;
-  if (num_tiles_dev) rows = min(rows, (int64_t)128 * *num_tiles_dev);
   const int64_t units = rows * nb;
-  const int sub = threadIdx.x & 15;
-  // whole warps run together (the shuffles): a warp's two halves take neighbouring units
-  const int64_t step = (int64_t)gridDim.x * 16;
-  for (int64_t u0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 5) * 2; u0 < units; u0 += step) {
-    const int64_t u = u0 + ((threadIdx.x >> 4) & 1);
-    const int64_t r = u / nb, c = (u - r * nb) * 128 + sub * 8;
-    int64_t src = u < units ? r : -1;
-    if (row_of && src >= 0) src = row_of[r];
-    float f[8];
-    if (src >= 0) {
-      load_cols<T, VEC>(x + src * cols, c, cols, f);
-    } else {
+  const int sub = threadIdx.x & 15, half = threadIdx.x >> 4;
+  const int64_t step = (int64_t)gridDim.x * 16 * kUnits;
+  // a warp's two halves go through the same rounds (the shuffles)
+  for (int64_t u0 = ((int64_t)blockIdx.x * 16 + (half & ~1)) * kUnits; u0 < units; u0 += step) {
+    float f[kUnits][8];
+    int64_t row[kUnits];
+    int64_t u = u0 + (half & 1) * kUnits;
+    int64_t r = u / nb, kb = u - r * nb;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    for (int i = 0; i < kUnits; ++i) {
+      row[i] = r * nb + kb < units ? r : -1;
+      if (row[i] >= 0) {
+        load_cols<T, VEC>(x + r * cols, kb * 128 + sub * 8, cols, f[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+      }
+      if (++kb == nb) kb = 0, ++r;
     }
-    uint32_t m = 0;
+    r = u / nb, kb = u - r * nb;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[i]));
+    for (int i = 0; i < kUnits; ++i) {
+      uint32_t m = 0;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (src < 0) continue;
-    const float s = scale_of(m);
-    store_codes<VEC>(q + r * cols, c, cols, encode8(f, s));
-    if (sub == 0) scale[u] = s;
+      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[i][e]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (row[i] >= 0) {
+        const float s = scale_of(m);
+        const uint2 code = encode8(f[i], s);
+        if (slots == 0) {
+          store_codes<VEC>(q + r * cols, kb * 128 + sub * 8, cols, code);
+          if (sub == 0) scale[r * nb + kb] = s;
+        } else {
+          for (int j = 0; j < slots; ++j) {
+            const int64_t d = out_row[r * slots + j];
+            if (d < 0) continue;
+            store_codes<VEC>(q + d * cols, kb * 128 + sub * 8, cols, code);
+            if (sub == 0) scale[d * nb + kb] = s;
+          }
+        }
+      }
+      if (++kb == nb) kb = 0, ++r;
+    }
   }
+}
+
+// fp32 rows row[p] (skipped when negative) of x, encoded in place of their own row of q; cols % 8 == 0.
+__global__ void __launch_bounds__(256) quantize_block_pairs_kernel(const float* __restrict__ x,
+                                                                   const int32_t* __restrict__ row, int64_t pairs,
+                                                                   int64_t cols, uint8_t* __restrict__ q,
+                                                                   float* __restrict__ scale) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t nb = (cols + 127) / 128, units = pairs * nb;
+  const int64_t u = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int sub = threadIdx.x & 15;
+  const int64_t p = u / nb, c = (u - p * nb) * 128 + sub * 8;
+  const int64_t r = u < units ? row[p] : -1;
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  if (r >= 0) load_cols<float, true>(x + r * cols, c, cols, f);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[i]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (r < 0) return;
+  const float s = scale_of(m);
+  store_codes<true>(q + r * cols, c, cols, encode8(f, s));
+  if (sub == 0) scale[r * nb + (c >> 7)] = s;
 }
 
 template <typename T, bool VEC>
@@ -152,17 +200,13 @@ bool vector_ok(const T* x, const uint8_t* q, int64_t cols) {
 }
 
 template <typename T>
-int run_rows(const void* xv, int64_t rows, int64_t cols, const int32_t* row_of, const int32_t* num_tiles_dev,
-             uint8_t* q, float* scale, cudaStream_t stream, bool pdl) {
+int run_rows(const void* xv, int64_t rows, int64_t cols, const int32_t* out_row, int slots, uint8_t* q, float* scale,
+             cudaStream_t stream, bool pdl) {
   const T* x = static_cast<const T*>(xv);
-  const int64_t groups = (rows * scale_blocks(cols) + 15) / 16;
+  const int64_t groups = (rows * scale_blocks(cols) + 16 * kUnits - 1) / (16 * kUnits);
   const dim3 grid((unsigned)std::min<int64_t>(groups, (int64_t)sm_count() * 32));
-  if (vector_ok(x, q, cols))
-    SB_CUDA_CHECK(launch_kernel(quantize_block_rows_kernel<T, true>, grid, dim3(256), 0, stream, pdl, x, rows, cols,
-                                row_of, num_tiles_dev, q, scale));
-  else
-    SB_CUDA_CHECK(launch_kernel(quantize_block_rows_kernel<T, false>, grid, dim3(256), 0, stream, pdl, x, rows, cols,
-                                row_of, num_tiles_dev, q, scale));
+  auto kernel = vector_ok(x, q, cols) ? quantize_block_rows_kernel<T, true> : quantize_block_rows_kernel<T, false>;
+  SB_CUDA_CHECK(launch_kernel(kernel, grid, dim3(256), 0, stream, pdl, x, rows, cols, out_row, slots, q, scale));
   count_launch();
   return STAGEML_OK;
 }
@@ -184,12 +228,22 @@ int run_tiles(const void* wv, int64_t batch, int64_t rows, int64_t cols, uint8_t
 
 }  // namespace
 
-int launch_quantize_block_rows(const void* x, int dtype, int64_t rows, int64_t cols, const int32_t* row_of,
-                               const int32_t* num_tiles_dev, uint8_t* q, float* scale, cudaStream_t stream, bool pdl) {
+int launch_quantize_block_rows(const void* x, int dtype, int64_t rows, int64_t cols, const int32_t* out_row, int slots,
+                               uint8_t* q, float* scale, cudaStream_t stream, bool pdl) {
   if (rows == 0 || cols == 0) return STAGEML_OK;
-  if (dtype == STAGEML_F32) return run_rows<float>(x, rows, cols, row_of, num_tiles_dev, q, scale, stream, pdl);
-  if (dtype == STAGEML_BF16) return run_rows<bf16>(x, rows, cols, row_of, num_tiles_dev, q, scale, stream, pdl);
-  return run_rows<f16>(x, rows, cols, row_of, num_tiles_dev, q, scale, stream, pdl);
+  if (dtype == STAGEML_F32) return run_rows<float>(x, rows, cols, out_row, slots, q, scale, stream, pdl);
+  if (dtype == STAGEML_BF16) return run_rows<bf16>(x, rows, cols, out_row, slots, q, scale, stream, pdl);
+  return run_rows<f16>(x, rows, cols, out_row, slots, q, scale, stream, pdl);
+}
+
+int launch_quantize_block_pairs(const float* x, const int32_t* row, int64_t pairs, int64_t cols, uint8_t* q,
+                                float* scale, cudaStream_t stream, bool pdl) {
+  if (pairs == 0 || cols == 0) return STAGEML_OK;
+  const int64_t units = pairs * scale_blocks(cols);
+  SB_CUDA_CHECK(launch_kernel(quantize_block_pairs_kernel, dim3((unsigned)((units + 15) / 16)), dim3(256), 0, stream,
+                              pdl, x, row, pairs, cols, q, scale));
+  count_launch();
+  return STAGEML_OK;
 }
 
 int launch_quantize_block_tiles(const void* w, int dtype, int64_t batch, int64_t rows, int64_t cols, uint8_t* q,
