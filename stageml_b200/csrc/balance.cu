@@ -15,8 +15,9 @@
 // Each lane sums its experts' p over its tokens in registers; a CTA adds them in a fixed
 // order in shared memory. Counts are integer atomics in shared memory. Batches of up to
 // kClusterValues logits run as one cluster whose first CTA adds the others' sums over
-// distributed shared memory and writes the loss: one launch. Longer ones write one partial
-// per CTA, added in CTA order by a second kernel. No floating-point atomics: the same bits
+// distributed shared memory and writes the loss: one launch. Longer ones run as many clusters,
+// each leaving one partial, which a second kernel adds in cluster order (one partial per CTA
+// made that kernel 32 us). No floating-point atomics: the same bits
 // on every run. Backward: the softmax again from the logits, one pass. Bound: HBM for long
 // batches (logits read twice, gradient written once), launches for short ones.
 #include "block_fp8.h"
@@ -26,7 +27,7 @@
 namespace sb {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxE = 256;
 constexpr int kClusterCtas = 8;                // portable cluster size
@@ -56,14 +57,40 @@ __device__ __forceinline__ void load4(const T* p, int e, int E, bool live, float
   }
 }
 
-// The token's logits on its lanes, then its softmax; 0 everywhere when no logit is above
-// -infinity (or the token does not count).
+// The token's logits on its lanes (-infinity when the token does not count), and its softmax, 0
+// everywhere when no logit is above -infinity.
 template <typename T, typename L, bool VEC>
-__device__ __forceinline__ void load_softmax(const T* __restrict__ logits, int64_t t, bool live, int E, int lane,
-                                             float (&x)[L::groups][4]) {
+__device__ __forceinline__ void load_logits(const T* __restrict__ logits, int64_t t, bool live, int E, int lane,
+                                            float (&x)[L::groups][4]) {
   const T* row = logits + t * E;
 #pragma unroll
   for (int j = 0; j < L::groups; ++j) load4<T, VEC>(row, (lane + L::lanes * j) * 4, E, live, x[j]);
+}
+
+// Sum over the token's experts. Up to 8 of them, every expert may be a chosen one (k = E); the
+// gradient then vanishes but for the rounding of these sums, so they are taken pairwise by expert
+// index (e with e + 4, then + 2, + 1) over separately rounded terms, as elementwise code takes them.
+template <typename L>
+__device__ __forceinline__ float token_sum(float (&v)[L::groups][4]) {
+  if constexpr (L::lanes <= 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (L::lanes == 2) v[0][i] = __fadd_rn(v[0][i], __shfl_xor_sync(0xffffffffu, v[0][i], 1));
+    return __fadd_rn(__fadd_rn(v[0][0], v[0][2]), __fadd_rn(v[0][1], v[0][3]));
+  } else {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += v[j][i];
+#pragma unroll
+    for (int o = L::lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+  }
+}
+
+template <typename L>
+__device__ __forceinline__ void softmax(float (&x)[L::groups][4]) {
   float m = -INFINITY;
 #pragma unroll
   for (int j = 0; j < L::groups; ++j)
@@ -72,21 +99,17 @@ __device__ __forceinline__ void load_softmax(const T* __restrict__ logits, int64
 #pragma unroll
   for (int o = L::lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float shift = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
+  float v[L::groups][4];
 #pragma unroll
   for (int j = 0; j < L::groups; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[j][i] = __expf(x[j][i] - shift);
-      s += x[j][i];
-    }
-#pragma unroll
-  for (int o = L::lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int i = 0; i < 4; ++i) v[j][i] = x[j][i] = L::lanes <= 2 ? expf(x[j][i] - shift) : __expf(x[j][i] - shift);
+  const float s = token_sum<L>(v);
   const float inv = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
   for (int j = 0; j < L::groups; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[j][i] *= inv;
+    for (int i = 0; i < 4; ++i) x[j][i] = L::lanes <= 2 && s != 0.f ? x[j][i] / s : x[j][i] * inv;
 }
 
 struct BalanceIn {
@@ -105,6 +128,17 @@ __device__ __forceinline__ void cta_sums(const T* __restrict__ logits, const Bal
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & (L::lanes - 1), sub = (threadIdx.x & 31) / L::lanes;
   for (int i = threadIdx.x; i <= kMaxE; i += kThreads) counts[i] = 0;
   __syncthreads();
+  // the slots of all tokens, apart from the softmax loop, whose loads they would hold up
+  const int64_t slots = in.T * in.k;
+  for (int64_t i = (int64_t)cta * kThreads + threadIdx.x; i < slots; i += (int64_t)ctas * kThreads) {
+    const int64_t e = in.ids_i64 ? static_cast<const int64_t*>(in.ids)[i] : static_cast<const int32_t*>(in.ids)[i];
+    if (in.valid && !in.valid[(uint32_t)i / (uint32_t)in.k]) continue;
+    if (e >= in.E) {
+      if (in.status) atomicCAS(in.status, 0, (int)kDevBadIndex);
+    } else if (e >= 0) {
+      atomicAdd(&counts[e], 1);
+    }
+  }
   float acc[L::groups][4];
 #pragma unroll
   for (int j = 0; j < L::groups; ++j)
@@ -112,27 +146,27 @@ __device__ __forceinline__ void cta_sums(const T* __restrict__ logits, const Bal
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
   int tokens = 0;
   const int64_t step = (int64_t)ctas * kWarps * L::per_warp;
-  for (int64_t t0 = ((int64_t)cta * kWarps + warp) * L::per_warp; t0 < in.T; t0 += step) {
-    const int64_t t = t0 + sub;
-    const bool live = t < in.T && (!in.valid || in.valid[t]);
+  auto counted = [&](int64_t t) { return t < in.T && (!in.valid || in.valid[t]); };
+  // the next tokens' logits are read while these are worked on
+  const int64_t t_first = ((int64_t)cta * kWarps + warp) * L::per_warp;
+  float next[L::groups][4];
+  bool next_live = counted(t_first + sub);
+  load_logits<T, L, VEC>(logits, t_first + sub, next_live, in.E, lane, next);
+  for (int64_t t0 = t_first; t0 < in.T; t0 += step) {
+    const bool live = next_live;
     float x[L::groups][4];
-    load_softmax<T, L, VEC>(logits, t, live, in.E, lane, x);
+#pragma unroll
+    for (int j = 0; j < L::groups; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j][i] = next[j][i];
+    next_live = counted(t0 + step + sub);
+    load_logits<T, L, VEC>(logits, t0 + step + sub, next_live, in.E, lane, next);
+    softmax<L>(x);
 #pragma unroll
     for (int j = 0; j < L::groups; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] += x[j][i];
-    if (live) {
-      for (int j = lane; j < in.k; j += L::lanes) {
-        const int64_t i = t * in.k + j;
-        const int64_t e = in.ids_i64 ? static_cast<const int64_t*>(in.ids)[i] : static_cast<const int32_t*>(in.ids)[i];
-        if (e >= in.E) {
-          if (in.status) atomicCAS(in.status, 0, (int)kDevBadIndex);
-        } else if (e >= 0) {
-          atomicAdd(&counts[e], 1);
-        }
-      }
-      tokens += lane == 0;
-    }
+    tokens += live && lane == 0;
   }
 #pragma unroll
   for (int o = L::lanes; o < 32; o <<= 1)
@@ -175,22 +209,25 @@ __device__ __forceinline__ void write_loss(const float* sums, const int32_t* cou
   }
 }
 
-// One cluster: every CTA its sums, the first CTA their totals in CTA order and the loss.
+// Every CTA its sums, the first CTA of a cluster their totals in CTA order; one cluster: then the
+// loss, several: one partial each (psum [clusters][E], pcount [clusters][E + 1]).
 template <typename T, typename L, bool VEC>
-__global__ void __launch_bounds__(kThreads)
-    balance_cluster_kernel(const T* __restrict__ logits, const BalanceIn in, float coefficient, float* loss,
-                           int32_t* counts_out, int32_t* tokens_out) {
+__global__ void __launch_bounds__(kThreads, 3)
+    balance_sums_kernel(const T* __restrict__ logits, const BalanceIn in, float coefficient, float* loss,
+                        int32_t* counts_out, int32_t* tokens_out, float* __restrict__ psum,
+                        int32_t* __restrict__ pcount, int cluster_ctas) {
   __shared__ float warp_sums[kWarps][kMaxE];
   __shared__ float sums[kMaxE];
   __shared__ int32_t counts[kMaxE + 1];
   cta_sums<T, L, VEC>(logits, in, blockIdx.x, gridDim.x, warp_sums, sums, counts);
-  if (gridDim.x > 1) {
+  const bool leader = cluster_ctas == 1 || cluster_ctarank() == 0;
+  if (cluster_ctas > 1) {
     cluster_sync_all();
-    if (blockIdx.x == 0) {
+    if (leader) {
       for (int e = threadIdx.x; e <= in.E; e += kThreads) {
         float s = e < in.E ? sums[e] : 0.f;
         int c = counts[e];
-        for (int r = 1; r < (int)gridDim.x; ++r) {
+        for (int r = 1; r < cluster_ctas; ++r) {
           uint32_t v;
           if (e < in.E) {
             asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(&sums[e]), r)) : "memory");
@@ -205,20 +242,15 @@ __global__ void __launch_bounds__(kThreads)
     }
     cluster_sync_all();  // the others stay until their sums have been read
   }
-  if (blockIdx.x == 0) write_loss(sums, counts, in.E, in.k, coefficient, loss, counts_out, tokens_out);
-}
-
-template <typename T, typename L, bool VEC>
-__global__ void __launch_bounds__(kThreads)
-    balance_partial_kernel(const T* __restrict__ logits, const BalanceIn in, float* __restrict__ psum,
-                           int32_t* __restrict__ pcount) {
-  __shared__ float warp_sums[kWarps][kMaxE];
-  __shared__ float sums[kMaxE];
-  __shared__ int32_t counts[kMaxE + 1];
-  cta_sums<T, L, VEC>(logits, in, blockIdx.x, gridDim.x, warp_sums, sums, counts);
+  if (!leader) return;
+  if ((int)gridDim.x == cluster_ctas) {
+    write_loss(sums, counts, in.E, in.k, coefficient, loss, counts_out, tokens_out);
+    return;
+  }
+  const int64_t cluster = blockIdx.x / cluster_ctas;
   for (int e = threadIdx.x; e <= in.E; e += kThreads) {
-    if (e < in.E) psum[(int64_t)blockIdx.x * in.E + e] = sums[e];
-    pcount[(int64_t)blockIdx.x * (in.E + 1) + e] = counts[e];
+    if (e < in.E) psum[cluster * in.E + e] = sums[e];
+    pcount[cluster * (in.E + 1) + e] = counts[e];
   }
 }
 
@@ -281,14 +313,14 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t t = t0 + sub;
     const bool live = t < T_ && (!valid || valid[t]);
     float x[L::groups][4];
-    load_softmax<T, L, VEC>(logits, t, live, E, lane, x);
-    float dot = 0.f;
+    load_logits<T, L, VEC>(logits, t, live, E, lane, x);
+    softmax<L>(x);
+    float v[L::groups][4];
 #pragma unroll
     for (int j = 0; j < L::groups; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dot = fmaf(x[j][i], f[j][i], dot);
-#pragma unroll
-    for (int o = L::lanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      for (int i = 0; i < 4; ++i) v[j][i] = __fmul_rn(x[j][i], f[j][i]);
+    const float dot = token_sum<L>(v);
     if (t >= T_) continue;
     T* out = grad + t * E;
 #pragma unroll
@@ -314,7 +346,7 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 3;
 
 // Calls f with the layout for E experts as a type.
 template <typename F>
@@ -324,8 +356,8 @@ int with_layout(int E, F&& f) {
   if (E <= 16) return f(Layout<4, 1>{});
   if (E <= 32) return f(Layout<8, 1>{});
   if (E <= 64) return f(Layout<8, 2>{});
-  if (E <= 128) return f(Layout<8, 4>{});
-  return f(Layout<8, 8>{});
+  if (E <= 128) return f(Layout<16, 2>{});
+  return f(Layout<16, 4>{});
 }
 
 int ctas_for(int64_t T, int E, int64_t most) {
@@ -334,7 +366,11 @@ int ctas_for(int64_t T, int E, int64_t most) {
   const int64_t per_cta = (int64_t)kWarps * per_warp;
   return (int)std::min<int64_t>((T + per_cta - 1) / per_cta, most);
 }
-int long_ctas(int64_t T, int E) { return ctas_for(T, E, (int64_t)sm_count() * kCtasPerSm); }
+// CTAs of a long batch, in whole clusters (at least two).
+int long_ctas(int64_t T, int E) {
+  const int n = ctas_for(T, E, (int64_t)sm_count() * kCtasPerSm);
+  return std::max(2, n / kClusterCtas) * kClusterCtas;
+}
 
 // 4 logits per load: E % 4 == 0 and the rows aligned to it.
 template <typename T>
@@ -352,33 +388,33 @@ struct ForwardOut {
 template <typename T, typename L, bool VEC>
 int forward_layout(const T* logits, const BalanceIn& in, float coefficient, const ForwardOut& o, void* scratch,
                    cudaStream_t stream) {
-  if (in.T * in.E <= kClusterValues) {
-    // a power of two of CTAs with a token group per warp, at least one
-    int ctas = 1;
-    while (ctas < kClusterCtas && ctas < ctas_for(in.T, in.E, kClusterCtas)) ctas <<= 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, balance_cluster_kernel<T, L, VEC>, logits, in, coefficient, o.loss, o.counts,
-                                     o.tokens));
-    count_launch();
-    return STAGEML_OK;
+  const bool one = in.T * in.E <= kClusterValues;
+  int cluster = kClusterCtas, grid = 0;
+  if (one) {  // a power of two of CTAs with a token group per warp, at least one
+    for (cluster = 1; cluster < kClusterCtas && cluster < ctas_for(in.T, in.E, kClusterCtas);) cluster <<= 1;
+    grid = cluster;
+  } else {
+    grid = long_ctas(in.T, in.E);
   }
-  const int grid = long_ctas(in.T, in.E);
+  const int clusters = grid / cluster;
   float* psum = static_cast<float*>(scratch);
-  int32_t* pcount = reinterpret_cast<int32_t*>(psum + (size_t)grid * in.E);
-  SB_CUDA_CHECK(launch_kernel(balance_partial_kernel<T, L, VEC>, dim3((unsigned)grid), dim3(kThreads), 0, stream, false,
-                              logits, in, psum, pcount));
+  int32_t* pcount = reinterpret_cast<int32_t*>(psum + (size_t)clusters * in.E);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, balance_sums_kernel<T, L, VEC>, logits, in, coefficient, o.loss, o.counts,
+                                   o.tokens, psum, pcount, cluster));
   count_launch();
+  if (one) return STAGEML_OK;
   SB_CUDA_CHECK(launch_kernel(balance_loss_kernel, dim3(1), dim3(1024), 0, stream, true, (const float*)psum,
-                              (const int32_t*)pcount, grid, in.E, in.k, coefficient, o.loss, o.counts, o.tokens));
+                              (const int32_t*)pcount, clusters, in.E, in.k, coefficient, o.loss, o.counts, o.tokens));
   count_launch();
   return STAGEML_OK;
 }
@@ -413,7 +449,7 @@ int backward(const float* grad_loss, const void* logits, const int32_t* counts, 
 }  // namespace
 
 size_t balance_scratch_bytes(int64_t T, int E) {
-  return T * E <= kClusterValues ? 0 : (size_t)long_ctas(T, E) * (2 * E + 1) * 4;
+  return T * E <= kClusterValues ? 0 : (size_t)(long_ctas(T, E) / kClusterCtas) * (2 * E + 1) * 4;
 }
 
 int launch_balance_loss(const void* logits, int dtype, const void* ids, int ids_i64, const uint8_t* valid, int64_t T,

@@ -20,8 +20,11 @@
 // to its store, 8 values per 16-byte load, or single values where the width or an address
 // is not a multiple of 8 values.
 //
-// Long batches: persistent CTAs whose next row arrives in shared memory by bulk copies
-// (two stages) while the current one is reduced, so HBM stays busy across the row sums.
+// Long batches: persistent CTAs that keep the channels' factors in shared memory as fp32
+// (w_post times a per-channel gate in one array, w_pre in another: read in their own types
+// every row, their loads, branches and conversions were half of the instructions) and whose
+// next row arrives in shared memory by bulk copies (two stages) while the current one is
+// reduced, so HBM stays busy across the row sums.
 //
 // Weight gradients: with y^ normalised (or y), the post weight and a per-channel gate have
 // gradients that are multiples, column by column, of the same sum over tokens
@@ -30,6 +33,7 @@
 // so at most two sums per column (S and dw_pre's) are kept, in the registers of the thread
 // that owns the column. Each CTA takes every gridDim-th row and writes its sums once; a second
 // kernel adds them in CTA order: no atomics, the same bits on every run. Bound: HBM.
+#include "block_codes.cuh"
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -39,7 +43,7 @@ namespace {
 
 constexpr int kMaxThreads = 512;
 constexpr int kMaxH = 16384;  // 512 threads x 32 values
-constexpr size_t kMaxRing = 200 * 1024;  // shared memory of a CTA's row ring
+constexpr size_t kMaxSmem = 224 * 1024;  // dynamic shared memory of a CTA
 
 template <int VEC, typename T>
 __device__ __forceinline__ void load_vals(const T* p, float (&f)[VEC]) {
@@ -99,8 +103,8 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, const
     store_vals<VEC>(static_cast<f16*>(p) + i, f);
 }
 
-// Sum of (a, b) over the row's threads: a warp (WARP) or the CTA. `red` has 64 floats;
-// consecutive calls alternate between its halves, so one barrier per call is enough.
+// Sums over the row's threads: a warp (WARP) or the CTA. `red` has 2 x 16 places; consecutive
+// calls alternate between its halves, so one barrier per call is enough.
 template <bool WARP>
 __device__ __forceinline__ float2 row_sum(float a, float b, float2* red, int& phase) {
 #pragma unroll
@@ -116,18 +120,113 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2* red, int& ph
   for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s.x += buf[i].x, s.y += buf[i].y;
   return s;
 }
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float a, float2* red, int& phase) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (WARP) return a;
+  float2* buf = red + (phase ^= 1) * 16;
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5].x = a;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += buf[i].x;
+  return s;
+}
 
-// Values of a row, from global memory or from the row's copy in shared memory.
+// Values of a row: from global memory, or (SMEM) from the row's copy at a shared-memory address.
+// The address is a 32-bit one, so that the loads are shared-memory loads (through a pointer
+// they were generic ones).
+__device__ __forceinline__ uint4 shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+template <typename T>
+struct RowIn {
+  const T* global;
+  uint32_t shared;
+};
 template <bool SMEM, int VEC, typename T>
-__device__ __forceinline__ void row_vals(const T* p, float (&f)[VEC]) {
+__device__ __forceinline__ void row_vals(const RowIn<T>& row, int c, float (&f)[VEC]) {
   if constexpr (!SMEM) {
-    load_vals<VEC>(p, f);
+    load_vals<VEC>(row.global + c, f);
   } else if constexpr (sizeof(T) == 2) {
-    unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
+    unpack8<T>(shared16(row.shared + 2 * c), f);
   } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    const uint4 a = shared16(row.shared + 4 * c), b = shared16(row.shared + 4 * c + 16);
+    f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
+    f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
   }
+}
+
+// The channels' factors: w_post times a per-channel gate (1 where neither is given) and w_pre,
+// from fp32 arrays in shared memory (STAGED) or from the parameters themselves.
+// Vectors of 8: the first four values of every eight in one plane, the others in a second, so that
+// the lanes of a 16-byte read are 16 bytes apart (32 apart they take two passes).
+template <bool STAGED>
+struct Factors {
+  const stageml_norm_args& a;
+  uint32_t y_at, z_at;
+  bool has_y;
+  template <int VEC>
+  __device__ __forceinline__ static int place(int c, int H) {
+    return VEC == 1 ? c : (c >> 3) * 4 + (c & 3) + (c & 4 ? H / 2 : 0);
+  }
+  template <int VEC>
+  __device__ __forceinline__ void stage(float* smem) {
+    has_y = a.post_weight || a.gate_mode == STAGEML_GATE_CHANNEL;
+    y_at = smem_u32(smem);
+    z_at = y_at + (has_y ? 4 * a.H : 0);
+    if (!STAGED) return;
+    float* z_factor = smem + (has_y ? a.H : 0);
+    for (int i = threadIdx.x; i < a.H; i += blockDim.x) {
+      if (has_y) smem[place<VEC>(i, a.H)] = from_params(i);
+      if (a.pre_weight) z_factor[place<VEC>(i, a.H)] = load_param1(a.pre_weight, a.pre_dtype, i);
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ float from_params(int c) const {
+    float f = a.post_weight ? load_param1(a.post_weight, a.post_dtype, c) : 1.f;
+    if (a.gate_mode == STAGEML_GATE_CHANNEL) f *= load_param1(a.gate, a.gate_dtype, c);
+    return f;
+  }
+  template <int VEC>
+  __device__ __forceinline__ void read(uint32_t at, int c, float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[0]) : "r"(at + 4 * c));
+    } else {
+      const uint4 lo = shared16(at + 2 * c), hi = shared16(at + 2 * a.H + 2 * c);
+      f[0] = __uint_as_float(lo.x), f[1] = __uint_as_float(lo.y), f[2] = __uint_as_float(lo.z), f[3] = __uint_as_float(lo.w);
+      f[4] = __uint_as_float(hi.x), f[5] = __uint_as_float(hi.y), f[6] = __uint_as_float(hi.z), f[7] = __uint_as_float(hi.w);
+    }
+  }
+  template <int VEC>
+  __device__ __forceinline__ void y(int c, float (&f)[VEC]) const {
+    if (STAGED && has_y) {
+      read<VEC>(y_at, c, f);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = 1.f;
+    if (STAGED) return;
+    if (a.post_weight) load_param<VEC>(a.post_weight, a.post_dtype, c, f);
+    if (a.gate_mode == STAGEML_GATE_CHANNEL) {
+      float g[VEC];
+      load_param<VEC>(a.gate, a.gate_dtype, c, g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] *= g[i];
+    }
+  }
+  template <int VEC>
+  __device__ __forceinline__ void z(int c, float (&f)[VEC]) const {
+    if (STAGED)
+      read<VEC>(z_at, c, f);
+    else
+      load_param<VEC>(a.pre_weight, a.pre_dtype, c, f);
+  }
+};
+size_t factor_bytes(const stageml_norm_args& a) {
+  return ((a.post_weight || a.gate_mode == STAGEML_GATE_CHANNEL ? 1 : 0) + (a.pre_weight ? 1 : 0)) * (size_t)a.H * 4;
 }
 
 // Two-stage ring of rows in dynamic shared memory, filled by bulk copies. Thread 0 issues
@@ -165,14 +264,14 @@ struct RowRing {
   }
   // An expired wait is recorded in the status word; the caller goes on (with wrong values),
   // so that the CTA's barriers still meet.
-  __device__ const uint8_t* wait(uint32_t n) {
+  __device__ uint32_t wait(uint32_t n) {
     mbar_wait(smem_u32(&full[n % kStages]), (n / kStages) & 1, abort_flag, status, kDefaultWaitNs,
               kDevTimeoutProducer);
-    return base + n % kStages * stage_bytes;
+    return smem_u32(base) + n % kStages * stage_bytes;
   }
 };
 
-template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING>
+template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stageml_norm_args a, float* z32) {
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
@@ -199,15 +298,16 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
     if (threadIdx.x == 0)
       for (int i = 0; i < kStages; ++i) fill(i);
   }
+  Factors<STAGED> factors{a};
+  factors.template stage<VEC>(reinterpret_cast<float*>(row_smem + (RING ? kStages * (r_bytes + y_bytes) : 0)));
   uint32_t count = 0;
   for (int64_t row = first; row < a.T; row += step, ++count) {
     const int64_t base = row * H;
-    const TR* r_row = static_cast<const TR*>(a.residual) + base;
-    const TY* y_row = static_cast<const TY*>(a.block_out) + base;
+    RowIn<TR> r_row{static_cast<const TR*>(a.residual) + base, 0};
+    RowIn<TY> y_row{static_cast<const TY*>(a.block_out) + base, 0};
     if constexpr (RING) {
-      const uint8_t* stage = ring.wait(count);
-      r_row = reinterpret_cast<const TR*>(stage);
-      y_row = reinterpret_cast<const TY*>(stage + r_bytes);
+      r_row.shared = ring.wait(count);
+      y_row.shared = r_row.shared + r_bytes;
     }
     float n[V][VEC];
     float sq = 0.f;
@@ -216,42 +316,30 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       const int c = (v * nt + tid) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) n[v][i] = 0.f;
-      if (a.block_out && c < H) row_vals<RING, VEC>(y_row + c, n[v]);
+      if (a.block_out && c < H) row_vals<RING, VEC>(y_row, c, n[v]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sq = fmaf(n[v][i], n[v][i], sq);
     }
-    if (a.block_out) {
-      float inv = 1.f;
-      if (a.post_weight) inv = rsqrtf(row_sum<WARP>(sq, 0.f, red, phase).x * inv_h + a.eps);
-      const float token_gate =
-          a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int c = (v * nt + tid) * VEC;
-        if (c >= H) continue;
-        float w[VEC];
-        if (a.post_weight) {
-          load_param<VEC>(a.post_weight, a.post_dtype, c, w);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) n[v][i] = n[v][i] * inv * w[i];
-        }
-        if (a.gate_mode == STAGEML_GATE_CHANNEL || a.gate_mode == STAGEML_GATE_FULL) {
-          load_param<VEC>(a.gate, a.gate_dtype, a.gate_mode == STAGEML_GATE_FULL ? base + c : c, w);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) n[v][i] *= w[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) n[v][i] *= token_gate;
-        }
-      }
-    }
+    float scale = a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
+    if (a.post_weight) scale *= rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
     sq = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
       if (c >= H) continue;
+      if (a.block_out) {
+        float w[VEC];
+        factors.template y<VEC>(c, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) n[v][i] *= scale * w[i];
+        if (a.gate_mode == STAGEML_GATE_FULL) {
+          load_param<VEC>(a.gate, a.gate_dtype, base + c, w);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) n[v][i] *= w[i];
+        }
+      }
       float r[VEC];
-      row_vals<RING, VEC>(r_row + c, r);
+      row_vals<RING, VEC>(r_row, c, r);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         n[v][i] = fmaf(a.residual_scale, r[i], n[v][i]);
@@ -261,7 +349,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
     }
     float inv = 0.f;
     if (a.pre_weight)
-      inv = rsqrtf(row_sum<WARP>(sq, 0.f, red, phase).x * inv_h + a.eps);
+      inv = rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
     else if (RING)
       __syncthreads();
     // the row's copy has been read by every thread (the barrier above)
@@ -274,26 +362,21 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       float w[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) w[i] = 0.f;
-      if (c < H) load_param<VEC>(a.pre_weight, a.pre_dtype, c, w);
+      if (c < H) factors.template z<VEC>(c, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] = n[v][i] * inv * w[i];
+      for (int i = 0; i < VEC; ++i) w[i] *= n[v][i] * inv;
       if constexpr (VEC == 8) {
         if (a.codes) {
-          // 16 neighbouring lanes hold one block of 128 columns
+          // 16 neighbouring lanes hold one block of 128 columns (w is 0 past the row's end)
           uint32_t m = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m = max(m, c < H ? __float_as_uint(w[i]) & 0x7fffffffu : 0u);
+          for (int i = 0; i < 8; ++i) m = max(m, c < H ? abs_bits(w[i]) : 0u);
 #pragma unroll
           for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          float s = __uint_as_float(m) / 448.0f;
-          s = s == 0.f ? 1.f : s;
+          const BlockScale s(m);
           if (c < H) {
-            uint32_t q[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              q[i] = __nv_cvt_float2_to_fp8x2(make_float2(w[2 * i] / s, w[2 * i + 1] / s), __NV_SATFINITE, __NV_E4M3);
-            *reinterpret_cast<uint2*>(a.codes + base + c) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-            if ((c & 127) == 0) a.code_scale[row * ((H + 127) / 128) + (c >> 7)] = s;
+            *reinterpret_cast<uint2*>(a.codes + base + c) = s.encode_signed8(w);
+            if ((c & 127) == 0) a.code_scale[row * ((H + 127) / 128) + (c >> 7)] = s.s;
           }
           continue;
         }
@@ -316,7 +399,7 @@ __host__ __device__ inline int n_sums_of(const stageml_norm_args& a) {
   return (has_block_sum(a) ? 1 : 0) + (a.pre_weight ? 1 : 0);
 }
 
-template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING>
+template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(const stageml_norm_args a, float* partial) {
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
@@ -327,7 +410,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
   const int H = a.H;
   const float inv_h = 1.f / (float)H;
   const bool post = a.post_weight != nullptr, pre = a.pre_weight != nullptr && a.grad_normed != nullptr;
-  const bool channel = a.gate_mode == STAGEML_GATE_CHANNEL, has_y = a.block_out != nullptr;
+  const bool has_y = a.block_out != nullptr;
   const uint32_t r_bytes = (uint32_t)H * sizeof(TR), y_bytes = (uint32_t)H * sizeof(TY);
   const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
@@ -347,6 +430,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
     if (threadIdx.x == 0)
       for (int i = 0; i < kStages; ++i) fill(i);
   }
+  Factors<STAGED> factors{a};
+  factors.template stage<VEC>(reinterpret_cast<float*>(row_smem + (RING ? 2 * kStages * (r_bytes + y_bytes) : 0)));
   float sum_y[V][VEC], sum_z[V][VEC];  // this thread's columns: S and dw_pre
 #pragma unroll
   for (int v = 0; v < V; ++v)
@@ -355,35 +440,25 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
   uint32_t count = 0;
   for (int64_t row = first; row < a.T; row += step, ++count) {
     const int64_t base = row * H;
-    const TR* r_row = static_cast<const TR*>(a.residual) + base;
-    const TR* dr_row = static_cast<const TR*>(a.grad_residual) + base;
-    const TY* y_row = static_cast<const TY*>(a.block_out) + base;
-    const TY* dz_row = static_cast<const TY*>(a.grad_normed) + base;
+    RowIn<TR> r_row{static_cast<const TR*>(a.residual) + base, 0}, dr_row{static_cast<const TR*>(a.grad_residual) + base, 0};
+    RowIn<TY> y_row{static_cast<const TY*>(a.block_out) + base, 0}, dz_row{static_cast<const TY*>(a.grad_normed) + base, 0};
     if constexpr (RING) {
-      const uint8_t* stage = ring.wait(count);
-      r_row = reinterpret_cast<const TR*>(stage);
-      dr_row = reinterpret_cast<const TR*>(stage + r_bytes);
-      y_row = reinterpret_cast<const TY*>(stage + 2 * r_bytes);
-      dz_row = reinterpret_cast<const TY*>(stage + 2 * r_bytes + y_bytes);
+      r_row.shared = ring.wait(count);
+      dr_row.shared = r_row.shared + r_bytes;
+      y_row.shared = dr_row.shared + r_bytes;
+      dz_row.shared = y_row.shared + y_bytes;
     }
     float y[V][VEC], n[V][VEC], d[V][VEC];
     float inv_y = 1.f;
     const float token_gate =
         a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
+    // a gate that is not part of the channels' factors
     auto gate_of = [&](int c, float (&g)[VEC]) {
-      if (channel || a.gate_mode == STAGEML_GATE_FULL) {
-        load_param<VEC>(a.gate, a.gate_dtype, channel ? c : base + c, g);
+      if (a.gate_mode == STAGEML_GATE_FULL) {
+        load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) g[i] = token_gate;
-      }
-    };
-    auto post_of = [&](int c, float (&w)[VEC]) {
-      if (post) {
-        load_param<VEC>(a.post_weight, a.post_dtype, c, w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) w[i] = 1.f;
       }
     };
     // y^ (or y), then n = r'
@@ -393,11 +468,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       const int c = (v * nt + tid) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[v][i] = 0.f;
-      if (c < H && has_y) row_vals<RING, VEC>(y_row + c, y[v]);
+      if (c < H && has_y) row_vals<RING, VEC>(y_row, c, y[v]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sq = fmaf(y[v][i], y[v][i], sq);
     }
-    if (post) inv_y = rsqrtf(row_sum<WARP>(sq, 0.f, red, phase).x * inv_h + a.eps);
+    if (post) inv_y = rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -406,10 +481,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       for (int i = 0; i < VEC; ++i) n[v][i] = d[v][i] = 0.f;
       if (c >= H) continue;
       float r[VEC];
-      row_vals<RING, VEC>(r_row + c, r);
+      row_vals<RING, VEC>(r_row, c, r);
       if (has_y) {
         float w[VEC], g[VEC];
-        post_of(c, w);
+        factors.template y<VEC>(c, w);
         gate_of(c, g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -421,8 +496,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       for (int i = 0; i < VEC; ++i) n[v][i] = fmaf(a.residual_scale, r[i], n[v][i]);
       if (pre) {
         float w[VEC];
-        row_vals<RING, VEC>(dz_row + c, d[v]);
-        load_param<VEC>(a.pre_weight, a.pre_dtype, c, w);
+        row_vals<RING, VEC>(dz_row, c, d[v]);
+        factors.template z<VEC>(c, w);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           s1 = fmaf(n[v][i], n[v][i], s1);
@@ -444,7 +519,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       if (c >= H) continue;
       if (pre) {
         float w[VEC];
-        load_param<VEC>(a.pre_weight, a.pre_dtype, c, w);
+        factors.template z<VEC>(c, w);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float nh = n[v][i] * inv_n;
@@ -454,7 +529,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       }
       if (a.grad_residual) {
         float dr[VEC];
-        row_vals<RING, VEC>(dr_row + c, dr);
+        row_vals<RING, VEC>(dr_row, c, dr);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) d[v][i] += dr[i];
       }
@@ -464,10 +539,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       store_vals<VEC>(static_cast<TR*>(a.d_residual) + base + c, t);
       if (!has_y) continue;
       float w[VEC], g[VEC];
-      post_of(c, w);
+      factors.template y<VEC>(c, w);
       gate_of(c, g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) t[i] = d[v][i] * y[v][i];  // dg = w_post t
+      for (int i = 0; i < VEC; ++i) t[i] = d[v][i] * y[v][i];  // a token's or full gate's dg = w_post t
       if (a.gate_mode == STAGEML_GATE_FULL) {
         float dg[VEC];
 #pragma unroll
@@ -477,7 +552,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         s4 = fmaf(w[i], t[i], s4);
-        sum_y[v][i] += channel ? t[i] : g[i] * t[i];
+        sum_y[v][i] = fmaf(g[i], t[i], sum_y[v][i]);  // g is 1 for a per-channel gate
         d[v][i] *= g[i] * w[i];  // the gradient of y^
         s3 = fmaf(d[v][i], y[v][i], s3);
       }
@@ -522,6 +597,7 @@ constexpr int kStrands = 16;
 __global__ void __launch_bounds__(32 * kStrands)
     norm_weight_sums_kernel(const stageml_norm_args a, const float* __restrict__ partial, int owners, int n_sums) {
   __shared__ float part[kStrands][33];
+  pdl_wait();
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const int64_t width = (int64_t)n_sums * a.H, i = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
@@ -580,13 +656,13 @@ int max_owners(const stageml_norm_args& a) {
   return (int)std::min<int64_t>(a.T + 7, (int64_t)sm_count() * rows_per_sm);
 }
 
-template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING>
+template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStream_t stream) {
-  auto kernel = norm_residual_kernel<TR, TY, VEC, V, WARP, RING>;
+  auto kernel = norm_residual_kernel<TR, TY, VEC, V, WARP, RING, STAGED>;
   int64_t grid = (a.T + s.rows_per_cta - 1) / s.rows_per_cta;
   size_t smem = 0;
-  if (RING) {
-    smem = (size_t)kStages * a.H * (sizeof(TR) + sizeof(TY));
+  if (STAGED) {
+    smem = (RING ? (size_t)kStages * a.H * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
     SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     grid = resident_ctas(kernel, s.threads, smem, a.T);
   }
@@ -595,13 +671,13 @@ int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStre
   return STAGEML_OK;
 }
 
-template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING>
+template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cudaStream_t stream) {
-  auto kernel = norm_residual_backward_kernel<TR, TY, VEC, V, WARP, RING>;
+  auto kernel = norm_residual_backward_kernel<TR, TY, VEC, V, WARP, RING, STAGED>;
   const int n_sums = n_sums_of(a);
   size_t smem = 0;
-  if (RING) {
-    smem = (size_t)kStages * a.H * 2 * (sizeof(TR) + sizeof(TY));
+  if (STAGED) {
+    smem = (RING ? (size_t)kStages * a.H * 2 * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
     SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
   const int grid = resident_ctas(kernel, s.threads, smem, (a.T + s.rows_per_cta - 1) / s.rows_per_cta);
@@ -610,7 +686,7 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
   if (n_sums) {
     const int64_t width = (int64_t)n_sums * a.H;
     SB_CUDA_CHECK(launch_kernel(norm_weight_sums_kernel, dim3((unsigned)((width + 31) / 32)), dim3(32 * kStrands), 0,
-                                stream, false, a, (const float*)partial, grid * s.rows_per_cta, n_sums));
+                                stream, true, a, (const float*)partial, grid * s.rows_per_cta, n_sums));
     count_launch();
   }
   return STAGEML_OK;
@@ -618,25 +694,29 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
 
 template <typename TR, typename TY>
 int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStream_t stream) {
-#define SB_NORM(VEC, V, WARP, RING, units) \
-  (backward ? run_backward<TR, TY, VEC, V, WARP, RING>(a, shape_of(units, V, WARP), scratch, stream) \
-            : run_forward<TR, TY, VEC, V, WARP, RING>(a, shape_of(units, V, WARP), scratch, stream))
+#define SB_NORM(VEC, V, WARP, RING, STAGED, units) \
+  (backward ? run_backward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, stream) \
+            : run_forward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, stream))
+  // Few rows run straight from global memory with as many threads per row as possible; more
+  // than two rows per SM are worth a CTA's staged factors.
+  const bool many = a.T > 2 * (int64_t)sm_count();
   if (vectors(a)) {
     const int units = a.H / 8;
-    if (units <= 32) return SB_NORM(8, 1, true, false, units);
-    // few rows: as many threads per row as possible, straight from global memory
-    const size_t stages = (size_t)kStages * a.H * (sizeof(TR) + sizeof(TY)) * (backward ? 2 : 1);
-    if (a.T <= sm_count() || stages > kMaxRing) {
-      if (units <= kMaxThreads) return SB_NORM(8, 1, false, false, units);
-      if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, false, units);
-      return SB_NORM(8, 4, false, false, units);
+    if (units <= 32) return SB_NORM(8, 1, true, false, false, units);
+    const size_t ring = (size_t)kStages * a.H * (sizeof(TR) + sizeof(TY)) * (backward ? 2 : 1) + factor_bytes(a);
+    if (!many || ring > kMaxSmem) {
+      if (units <= kMaxThreads) return SB_NORM(8, 1, false, false, false, units);
+      if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, false, false, units);
+      return SB_NORM(8, 4, false, false, false, units);
     }
-    if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, true, units);
-    return SB_NORM(8, 4, false, true, units);
+    if (units <= 256) return SB_NORM(8, 1, false, true, true, units);
+    if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, true, true, units);
+    return SB_NORM(8, 4, false, true, true, units);
   }
-  if (a.H <= 256) return SB_NORM(1, 8, true, false, a.H);
-  if (a.H <= 8 * kMaxThreads) return SB_NORM(1, 8, false, false, a.H);
-  return SB_NORM(1, 32, false, false, a.H);
+  if (a.H <= 256) return SB_NORM(1, 8, true, false, false, a.H);
+  if (a.H <= 8 * kMaxThreads)
+    return many ? SB_NORM(1, 8, false, false, true, a.H) : SB_NORM(1, 8, false, false, false, a.H);
+  return many ? SB_NORM(1, 32, false, false, true, a.H) : SB_NORM(1, 32, false, false, false, a.H);
 #undef SB_NORM
 }
 

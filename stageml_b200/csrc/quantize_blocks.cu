@@ -6,9 +6,10 @@
 // |x|, in which NaN > infinity > every number), so it is never hidden.
 //
 // One pass: a block's values stay in registers between the maximum and the encoding.
-// Rows: 16 lanes per block, 8 values per lane (one 16-byte load for 16-bit inputs), the
-// maximum by four shuffles. Tiles: one CTA per tile, 64 values per thread.
+// Rows: 8 or 16 lanes per block, the maximum by shuffles. Tiles: one CTA per tile, 64
+// values per thread.
 // Bound: HBM (2 or 4 bytes read and 1 written per value).
+#include "block_codes.cuh"
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -16,45 +17,25 @@
 namespace sb {
 namespace {
 
-// |v| as an integer that orders like |v|, NaN above infinity.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
-  const float s = __uint_as_float(amax_bits) / 448.0f;
-  return s == 0.f ? 1.f : s;
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  unpack8<T>(__ldg(reinterpret_cast<const uint4*>(p)), f);
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-}
-
 // 8 values of one row at columns [c, c + 8), zeros past the end. VEC: cols % 8 == 0
 // and the rows are aligned for 16-byte loads.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_cols(const T* row, int64_t c, int64_t cols, float (&f)[8]) {
+__device__ __forceinline__ void load_cols(const T* row, int64_t c, int64_t cols, Vals8<T>& v) {
   if (VEC && c < cols) {
-    load8<T>(row + c, f);
+    v.load(row + c);
   } else {
+    v.zero();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.f;
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) v.set(i, row[c + i]);
   }
 }
 
-__device__ __forceinline__ uint2 encode8(const float (&f)[8], float s) {
-  uint2 u;
-  uint16_t h[4];
+// The largest magnitude (bits) over the 16 lanes of a block.
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] / s, f[2 * i + 1] / s), __NV_SATFINITE, __NV_E4M3);
-  u.x = h[0] | (uint32_t)h[1] << 16;
-  u.y = h[2] | (uint32_t)h[3] << 16;
-  return u;
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
 }
 
 template <bool VEC>
@@ -68,8 +49,49 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t c, int64_t col
   }
 }
 
-// A half-warp takes kUnits neighbouring blocks of the flattened (row, block) list per round, all
+// Rows of whole blocks, in place: block u of the flattened tensor starts at 128 u and no row
+// index is needed. 8 lanes per block, 16 values each: the scale and the shuffles, which every
+// lane pays for per block, weigh half of what they do with 16 lanes (26 us instead of 17 for
+// 8192 x 4096 bf16 values; instructions bound that form, not HBM). All blocks of a round are
 // loaded before the first is encoded.
+constexpr int kFlat = 2;
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_block_flat_kernel(const T* __restrict__ x, int64_t units,
+                                                                  uint8_t* __restrict__ q, float* __restrict__ scale) {
+  pdl_wait();
+  pdl_trigger();
+  const int sub = threadIdx.x & 7;
+  const int64_t step = (int64_t)gridDim.x * 32;
+  for (int64_t u0 = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); u0 - (threadIdx.x >> 3) < units; u0 += step * kFlat) {
+    Vals8<T> v[kFlat][2];
+#pragma unroll
+    for (int i = 0; i < kFlat; ++i) {
+      const int64_t u = u0 + i * step;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (u < units)
+          v[i][h].load(x + u * 128 + sub * 16 + 8 * h);
+        else
+          v[i][h].zero();
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kFlat; ++i) {
+      const int64_t u = u0 + i * step;
+      uint32_t m = max(v[i][0].amax(), v[i][1].amax());
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (u >= units) continue;
+      const BlockScale s(m);
+      const uint2 lo = v[i][0].encode(s), hi = v[i][1].encode(s);
+      *reinterpret_cast<uint4*>(q + u * 128 + sub * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      if (sub == 0) scale[u] = s.s;
+    }
+  }
+}
+
+// Other rows, or rows that are written to other places (a MoE plan's): unit u is block u % nb of
+// row u / nb, 16 lanes per block, kUnits blocks per half-warp and round.
 constexpr int kUnits = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_block_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
@@ -77,51 +99,40 @@ __global__ void __launch_bounds__(256) quantize_block_rows_kernel(const T* __res
                                                                   uint8_t* __restrict__ q, float* __restrict__ scale) {
   pdl_wait();
   pdl_trigger();
-  const int64_t nb = (cols + 127) / 128;
+  const uint32_t nb = (uint32_t)((cols + 127) / 128);
   const int64_t units = rows * nb;
   const int sub = threadIdx.x & 15, half = threadIdx.x >> 4;
-  const int64_t step = (int64_t)gridDim.x * 16 * kUnits;
-  // a warp's two halves go through the same rounds (the shuffles)
-  for (int64_t u0 = ((int64_t)blockIdx.x * 16 + (half & ~1)) * kUnits; u0 < units; u0 += step) {
-    float f[kUnits][8];
-    int64_t row[kUnits];
-    int64_t u = u0 + (half & 1) * kUnits;
-    int64_t r = u / nb, kb = u - r * nb;
+  // unit i of a round: 16 neighbouring units per CTA, then the next 16
+  const int64_t step = (int64_t)gridDim.x * 16;
+  for (int64_t u0 = (int64_t)blockIdx.x * 16; u0 < units; u0 += step * kUnits) {
+    Vals8<T> v[kUnits];
+    uint32_t row[kUnits], col[kUnits];
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      row[i] = r * nb + kb < units ? r : -1;
-      if (row[i] >= 0) {
-        load_cols<T, VEC>(x + r * cols, kb * 128 + sub * 8, cols, f[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
-      }
-      if (++kb == nb) kb = 0, ++r;
+      const int64_t u = u0 + i * step + half;
+      v[i].zero();
+      if (u >= units) continue;
+      row[i] = (uint32_t)u / nb;
+      col[i] = ((uint32_t)u - row[i] * nb) * 128 + sub * 8;
+      load_cols<T, VEC>(x + row[i] * cols, col[i], cols, v[i]);
     }
-    r = u / nb, kb = u - r * nb;
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[i][e]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (row[i] >= 0) {
-        const float s = scale_of(m);
-        const uint2 code = encode8(f[i], s);
-        if (slots == 0) {
-          store_codes<VEC>(q + r * cols, kb * 128 + sub * 8, cols, code);
-          if (sub == 0) scale[r * nb + kb] = s;
-        } else {
-          for (int j = 0; j < slots; ++j) {
-            const int64_t d = out_row[r * slots + j];
-            if (d < 0) continue;
-            store_codes<VEC>(q + d * cols, kb * 128 + sub * 8, cols, code);
-            if (sub == 0) scale[d * nb + kb] = s;
-          }
+      const uint32_t m = block_max(v[i].amax());
+      if (u0 + i * step + half >= units) continue;
+      const BlockScale s(m);
+      const uint2 code = v[i].encode(s);
+      if (slots == 0) {
+        store_codes<VEC>(q + row[i] * cols, col[i], cols, code);
+        if (sub == 0) scale[(int64_t)row[i] * nb + (col[i] >> 7)] = s.s;
+      } else {
+        for (int j = 0; j < slots; ++j) {
+          const int64_t d = out_row[(int64_t)row[i] * slots + j];
+          if (d < 0) continue;
+          store_codes<VEC>(q + d * cols, col[i], cols, code);
+          if (sub == 0) scale[d * nb + (col[i] >> 7)] = s.s;
         }
       }
-      if (++kb == nb) kb = 0, ++r;
     }
   }
 }
@@ -138,19 +149,13 @@ __global__ void __launch_bounds__(256) quantize_block_pairs_kernel(const float* 
   const int sub = threadIdx.x & 15;
   const int64_t p = u / nb, c = (u - p * nb) * 128 + sub * 8;
   const int64_t r = u < units ? row[p] : -1;
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = 0.f;
-  if (r >= 0) load_cols<float, true>(x + r * cols, c, cols, f);
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[i]));
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  Vals8<float> v;
+  v.zero();
+  if (r >= 0) load_cols<float, true>(x + r * cols, c, cols, v);
+  const BlockScale s(block_max(v.amax()));
   if (r < 0) return;
-  const float s = scale_of(m);
-  store_codes<true>(q + r * cols, c, cols, encode8(f, s));
-  if (sub == 0) scale[r * nb + (c >> 7)] = s;
+  store_codes<true>(q + r * cols, c, cols, v.encode(s));
+  if (sub == 0) scale[r * nb + (c >> 7)] = s.s;
 }
 
 template <typename T, bool VEC>
@@ -163,34 +168,30 @@ __global__ void __launch_bounds__(256) quantize_block_tiles_kernel(const T* __re
   const int64_t r0 = t / nb * 128, c = t % nb * 128 + (threadIdx.x & 15) * 8;
   const T* src = w + b * rows * cols;
   uint8_t* dst = q + b * rows * cols;
-  float f[8][8];
+  Vals8<T> v[8];
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int64_t r = r0 + j * 16 + (threadIdx.x >> 4);
-    if (r < rows) {
-      load_cols<T, VEC>(src + r * cols, c, cols, f[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
-    }
+    if (r < rows)
+      load_cols<T, VEC>(src + r * cols, c, cols, v[j]);
+    else
+      v[j].zero();
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[j][i]));
+  for (int j = 0; j < 8; ++j) m = max(m, v[j].amax());
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, red[i]);
-  const float s = scale_of(m);
-  if (threadIdx.x == 0) scale[tile] = s;
+  const BlockScale s(m);
+  if (threadIdx.x == 0) scale[tile] = s.s;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int64_t r = r0 + j * 16 + (threadIdx.x >> 4);
-    if (r < rows) store_codes<VEC>(dst + r * cols, c, cols, encode8(f[j], s));
+    if (r < rows) store_codes<VEC>(dst + r * cols, c, cols, v[j].encode(s));
   }
 }
 
@@ -203,10 +204,17 @@ template <typename T>
 int run_rows(const void* xv, int64_t rows, int64_t cols, const int32_t* out_row, int slots, uint8_t* q, float* scale,
              cudaStream_t stream, bool pdl) {
   const T* x = static_cast<const T*>(xv);
-  const int64_t groups = (rows * scale_blocks(cols) + 16 * kUnits - 1) / (16 * kUnits);
-  const dim3 grid((unsigned)std::min<int64_t>(groups, (int64_t)sm_count() * 32));
-  auto kernel = vector_ok(x, q, cols) ? quantize_block_rows_kernel<T, true> : quantize_block_rows_kernel<T, false>;
-  SB_CUDA_CHECK(launch_kernel(kernel, grid, dim3(256), 0, stream, pdl, x, rows, cols, out_row, slots, q, scale));
+  const int64_t units = rows * scale_blocks(cols);
+  SB_CHECK_ARG(units <= 0x7fffffff, "quantize_e4m3_blocks: more than 2^31 blocks");
+  const bool vec = vector_ok(x, q, cols);
+  if (slots == 0 && cols % 128 == 0 && vec && reinterpret_cast<uintptr_t>(q) % 16 == 0) {
+    const dim3 grid((unsigned)std::min<int64_t>((units + 31) / 32, (int64_t)sm_count() * 32));
+    SB_CUDA_CHECK(launch_kernel(quantize_block_flat_kernel<T>, grid, dim3(256), 0, stream, pdl, x, units, q, scale));
+  } else {
+    const dim3 grid((unsigned)std::min<int64_t>((units + 15) / 16, (int64_t)sm_count() * 32));
+    auto kernel = vec ? quantize_block_rows_kernel<T, true> : quantize_block_rows_kernel<T, false>;
+    SB_CUDA_CHECK(launch_kernel(kernel, grid, dim3(256), 0, stream, pdl, x, rows, cols, out_row, slots, q, scale));
+  }
   count_launch();
   return STAGEML_OK;
 }
