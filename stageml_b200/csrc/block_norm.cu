@@ -20,11 +20,12 @@
 // to its store, 8 values per 16-byte load, or single values where the width or an address
 // is not a multiple of 8 values.
 //
-// Long batches: persistent CTAs that keep the channels' factors in shared memory as fp32
-// (w_post times a per-channel gate in one array, w_pre in another: read in their own types
-// every row, their loads, branches and conversions were half of the instructions) and whose
-// next row arrives in shared memory by bulk copies (two stages) while the current one is
-// reduced, so HBM stays busy across the row sums.
+// Long batches: persistent CTAs that keep the channels' factors as fp32 (w_post times a
+// per-channel gate in one array, w_pre in another), the forward in the registers of the
+// columns' threads, the backward, whose column sums are there, in shared memory; read in their
+// own types every row, their loads, branches and conversions were half of the instructions.
+// The next rows arrive in shared memory by bulk copies (a ring of rows) while the current one
+// is reduced, so HBM stays busy across the row sums.
 //
 // Weight gradients: with y^ normalised (or y), the post weight and a per-channel gate have
 // gradients that are multiples, column by column, of the same sum over tokens
@@ -116,8 +117,13 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2* red, int& ph
   float2* buf = red + (phase ^= 1) * 16;
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = make_float2(a, b);
   __syncthreads();
-  float2 s = make_float2(0.f, 0.f);
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s.x += buf[i].x, s.y += buf[i].y;
+  const int lane = threadIdx.x & 15;
+  float2 s = lane < (int)(blockDim.x >> 5) ? buf[lane] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+    s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+  }
   return s;
 }
 template <bool WARP>
@@ -128,8 +134,10 @@ __device__ __forceinline__ float row_sum(float a, float2* red, int& phase) {
   float2* buf = red + (phase ^= 1) * 16;
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5].x = a;
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += buf[i].x;
+  const int lane = threadIdx.x & 15;
+  float s = lane < (int)(blockDim.x >> 5) ? buf[lane].x : 0.f;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
@@ -158,6 +166,42 @@ __device__ __forceinline__ void row_vals(const RowIn<T>& row, int c, float (&f)[
     f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
   }
 }
+
+// A row's values held as they were loaded: eight 16-bit values take four registers, and the
+// kernels that hold several rows' worth run out of registers before anything else.
+template <int VEC, typename T>
+struct Held {
+  float f[VEC];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = 0.f;
+  }
+  template <bool SMEM>
+  __device__ __forceinline__ void load(const RowIn<T>& row, int c) {
+    row_vals<SMEM, VEC>(row, c, f);
+  }
+  __device__ __forceinline__ void floats(float (&v)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = f[i];
+  }
+};
+template <typename T>
+struct Held16 {
+  uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  template <bool SMEM>
+  __device__ __forceinline__ void load(const RowIn<T>& row, int c) {
+    if constexpr (SMEM)
+      u = shared16(row.shared + 2 * c);
+    else
+      u = __ldg(reinterpret_cast<const uint4*>(row.global + c));
+  }
+  __device__ __forceinline__ void floats(float (&v)[8]) const { unpack8<T>(u, v); }
+};
+template <>
+struct Held<8, bf16> : Held16<bf16> {};
+template <>
+struct Held<8, f16> : Held16<f16> {};
 
 // The channels' factors: w_post times a per-channel gate (1 where neither is given) and w_pre,
 // from fp32 arrays in shared memory (STAGED) or from the parameters themselves.
@@ -229,20 +273,21 @@ size_t factor_bytes(const stageml_norm_args& a) {
   return ((a.post_weight || a.gate_mode == STAGEML_GATE_CHANNEL ? 1 : 0) + (a.pre_weight ? 1 : 0)) * (size_t)a.H * 4;
 }
 
-// Two-stage ring of rows in dynamic shared memory, filled by bulk copies. Thread 0 issues
-// the copies of row i + 2 once every thread has read row i.
-constexpr int kStages = 2;
+// Ring of rows in dynamic shared memory, filled by bulk copies. Thread 0 issues the copies of
+// row i + STAGES once every thread has read row i.
+constexpr int kForwardStages = 3, kBackwardStages = 2;
+template <int STAGES>
 struct RowRing {
   uint8_t* base;
   uint32_t stage_bytes;
-  uint64_t* full;          // [kStages]
+  uint64_t* full;          // [STAGES]
   volatile int* abort_flag;
   int32_t* status;
 
   __device__ void init(uint8_t* smem, uint32_t bytes, uint64_t* bars, int* flag, int32_t* st) {
     base = smem, stage_bytes = bytes, full = bars, abort_flag = flag, status = st;
     if (threadIdx.x == 0) {
-      for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&full[i]), 1);
+      for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&full[i]), 1);
       *flag = 0;
       fence_barrier_init();
     }
@@ -251,8 +296,8 @@ struct RowRing {
   // The copies of the n-th row of this CTA (thread 0); null sources are left out.
   __device__ void fill(uint32_t n, const void* const (&src)[4], const uint32_t (&bytes)[4]) {
     fence_proxy_async_smem();  // the stage's reads (ordered by the caller's barrier) come first
-    const uint32_t bar = smem_u32(&full[n % kStages]);
-    uint32_t dst = smem_u32(base) + n % kStages * stage_bytes, total = 0;
+    const uint32_t bar = smem_u32(&full[n % STAGES]);
+    uint32_t dst = smem_u32(base) + n % STAGES * stage_bytes, total = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) total += src[i] ? bytes[i] : 0;
     mbar_arrive_expect_tx(bar, total);
@@ -265,17 +310,19 @@ struct RowRing {
   // An expired wait is recorded in the status word; the caller goes on (with wrong values),
   // so that the CTA's barriers still meet.
   __device__ uint32_t wait(uint32_t n) {
-    mbar_wait(smem_u32(&full[n % kStages]), (n / kStages) & 1, abort_flag, status, kDefaultWaitNs,
+    mbar_wait(smem_u32(&full[n % STAGES]), (n / STAGES) & 1, abort_flag, status, kDefaultWaitNs,
               kDevTimeoutProducer);
-    return smem_u32(base) + n % kStages * stage_bytes;
+    return smem_u32(base) + n % STAGES * stage_bytes;
   }
 };
 
-template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
+// HELD: persistent CTAs, the factors of a thread's columns in its registers.
+template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool HELD>
 __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stageml_norm_args a, float* z32) {
+  constexpr int STAGES = kForwardStages;
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
-  __shared__ uint64_t bars[kStages];
+  __shared__ uint64_t bars[STAGES];
   __shared__ int flag;
   int phase = 0;
   const int nt = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
@@ -284,7 +331,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
   const uint32_t r_bytes = (uint32_t)H * sizeof(TR), y_bytes = (uint32_t)H * sizeof(TY);
   const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
-  RowRing ring;
+  RowRing<STAGES> ring;
   auto fill = [&](uint32_t n) {
     const int64_t row = first + n * step;
     if (row >= a.T) return;
@@ -296,10 +343,21 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
   if constexpr (RING) {
     ring.init(row_smem, r_bytes + y_bytes, bars, &flag, a.status);
     if (threadIdx.x == 0)
-      for (int i = 0; i < kStages; ++i) fill(i);
+      for (int i = 0; i < STAGES; ++i) fill(i);
   }
-  Factors<STAGED> factors{a};
-  factors.template stage<VEC>(reinterpret_cast<float*>(row_smem + (RING ? kStages * (r_bytes + y_bytes) : 0)));
+  const Factors<false> factors{a, 0, 0, false};
+  float fy[V][VEC], fz[V][VEC];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * nt + tid) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) fy[v][i] = fz[v][i] = 0.f;
+      if (c >= H) continue;
+      factors.template y<VEC>(c, fy[v]);
+      if (a.pre_weight) factors.template z<VEC>(c, fz[v]);
+    }
+  }
   uint32_t count = 0;
   for (int64_t row = first; row < a.T; row += step, ++count) {
     const int64_t base = row * H;
@@ -328,21 +386,21 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       const int c = (v * nt + tid) * VEC;
       if (c >= H) continue;
       if (a.block_out) {
-        float w[VEC];
-        factors.template y<VEC>(c, w);
+        if constexpr (!HELD) factors.template y<VEC>(c, fy[v]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) n[v][i] *= scale * w[i];
+        for (int i = 0; i < VEC; ++i) n[v][i] *= fy[v][i];
         if (a.gate_mode == STAGEML_GATE_FULL) {
-          load_param<VEC>(a.gate, a.gate_dtype, base + c, w);
+          float g[VEC];
+          load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) n[v][i] *= w[i];
+          for (int i = 0; i < VEC; ++i) n[v][i] *= g[i];
         }
       }
       float r[VEC];
       row_vals<RING, VEC>(r_row, c, r);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        n[v][i] = fmaf(a.residual_scale, r[i], n[v][i]);
+        n[v][i] = fmaf(n[v][i], scale, a.residual_scale * r[i]);
         sq = fmaf(n[v][i], n[v][i], sq);
       }
       store_vals<VEC>(static_cast<TR*>(a.new_residual) + base + c, n[v]);
@@ -354,20 +412,22 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       __syncthreads();
     // the row's copy has been read by every thread (the barrier above)
     if constexpr (RING)
-      if (threadIdx.x == 0) fill(count + kStages);
+      if (threadIdx.x == 0) fill(count + STAGES);
     if (!a.pre_weight) continue;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
+      if constexpr (!HELD) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) fz[v][i] = 0.f;
+        if (c < H) factors.template z<VEC>(c, fz[v]);
+      }
       float w[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] = 0.f;
-      if (c < H) factors.template z<VEC>(c, w);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] *= n[v][i] * inv;
+      for (int i = 0; i < VEC; ++i) w[i] = n[v][i] * inv * fz[v][i];
       if constexpr (VEC == 8) {
         if (a.codes) {
-          // 16 neighbouring lanes hold one block of 128 columns (w is 0 past the row's end)
+          // 16 neighbouring lanes hold one block of 128 columns
           uint32_t m = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) m = max(m, c < H ? abs_bits(w[i]) : 0u);
@@ -400,10 +460,11 @@ __host__ __device__ inline int n_sums_of(const stageml_norm_args& a) {
 }
 
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
-__global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(const stageml_norm_args a, float* partial) {
+__global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_residual_backward_kernel(const stageml_norm_args a, float* partial) {
+  constexpr int STAGES = kBackwardStages;
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
-  __shared__ uint64_t bars[kStages];
+  __shared__ uint64_t bars[STAGES];
   __shared__ int flag;
   int phase = 0;
   const int nt = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
@@ -414,7 +475,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
   const uint32_t r_bytes = (uint32_t)H * sizeof(TR), y_bytes = (uint32_t)H * sizeof(TY);
   const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
-  RowRing ring;
+  RowRing<STAGES> ring;
   auto fill = [&](uint32_t n) {
     const int64_t row = first + n * step;
     if (row >= a.T) return;
@@ -428,10 +489,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
   if constexpr (RING) {
     ring.init(row_smem, 2 * (r_bytes + y_bytes), bars, &flag, a.status);
     if (threadIdx.x == 0)
-      for (int i = 0; i < kStages; ++i) fill(i);
+      for (int i = 0; i < STAGES; ++i) fill(i);
   }
   Factors<STAGED> factors{a};
-  factors.template stage<VEC>(reinterpret_cast<float*>(row_smem + (RING ? 2 * kStages * (r_bytes + y_bytes) : 0)));
+  factors.template stage<VEC>(reinterpret_cast<float*>(row_smem + (RING ? 2 * STAGES * (r_bytes + y_bytes) : 0)));
   float sum_y[V][VEC], sum_z[V][VEC];  // this thread's columns: S and dw_pre
 #pragma unroll
   for (int v = 0; v < V; ++v)
@@ -448,133 +509,143 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_residual_backward_kernel(
       y_row.shared = dr_row.shared + r_bytes;
       dz_row.shared = y_row.shared + y_bytes;
     }
-    float y[V][VEC], n[V][VEC], d[V][VEC];
+    Held<VEC, TY> y_in[V], dz_in[V];
+    float n[V][VEC], d[V][VEC];
+    // With f the channel's factor and g a gate that is not part of it: n = a r + f g y inv_y.
+    const bool full = a.gate_mode == STAGEML_GATE_FULL;
+    const float token_gate = a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
     float inv_y = 1.f;
-    const float token_gate =
-        a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
-    // a gate that is not part of the channels' factors
-    auto gate_of = [&](int c, float (&g)[VEC]) {
-      if (a.gate_mode == STAGEML_GATE_FULL) {
-        load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) g[i] = token_gate;
-      }
-    };
-    // y^ (or y), then n = r'
     float sq = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
+      y_in[v].zero();
+      if (c < H && has_y) y_in[v].template load<RING>(y_row, c);
+      float y[VEC];
+      y_in[v].floats(y);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) y[v][i] = 0.f;
-      if (c < H && has_y) row_vals<RING, VEC>(y_row, c, y[v]);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sq = fmaf(y[v][i], y[v][i], sq);
+      for (int i = 0; i < VEC; ++i) sq = fmaf(y[i], y[i], sq);
     }
     if (post) inv_y = rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
+    const float y_scale = inv_y * token_gate;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) n[v][i] = d[v][i] = 0.f;
+      for (int i = 0; i < VEC; ++i) n[v][i] = 0.f;
+      dz_in[v].zero();
       if (c >= H) continue;
-      float r[VEC];
-      row_vals<RING, VEC>(r_row, c, r);
       if (has_y) {
-        float w[VEC], g[VEC];
-        factors.template y<VEC>(c, w);
-        gate_of(c, g);
+        float f[VEC], y[VEC];
+        factors.template y<VEC>(c, f);
+        y_in[v].floats(y);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          y[v][i] *= inv_y;
-          n[v][i] = g[i] * (y[v][i] * w[i]);
+        for (int i = 0; i < VEC; ++i) n[v][i] = y[i] * f[i];
+        if (full) {
+          load_param<VEC>(a.gate, a.gate_dtype, base + c, f);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) n[v][i] *= f[i];
         }
       }
+      float r[VEC];
+      row_vals<RING, VEC>(r_row, c, r);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) n[v][i] = fmaf(a.residual_scale, r[i], n[v][i]);
+      for (int i = 0; i < VEC; ++i) n[v][i] = fmaf(n[v][i], y_scale, a.residual_scale * r[i]);
       if (pre) {
-        float w[VEC];
-        row_vals<RING, VEC>(dz_row, c, d[v]);
-        factors.template z<VEC>(c, w);
+        float f[VEC], dz[VEC];
+        dz_in[v].template load<RING>(dz_row, c);
+        dz_in[v].floats(dz);
+        factors.template z<VEC>(c, f);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           s1 = fmaf(n[v][i], n[v][i], s1);
-          s2 = fmaf(d[v][i] * w[i], n[v][i], s2);
+          s2 = fmaf(dz[i] * f[i], n[v][i], s2);
         }
       }
     }
-    float inv_n = 0.f, mean = 0.f;
+    float inv_n = 0.f, c_n = 0.f;
     if (pre) {
       const float2 s = row_sum<WARP>(s1, s2, red, phase);
       inv_n = rsqrtf(s.x * inv_h + a.eps);
-      mean = s.y * inv_n * inv_h;  // mean(dn n^)
+      c_n = s.y * inv_h * inv_n * inv_n * inv_n;  // n^ mean(dn n^) inv_n = n c_n
     }
-    // d, then the gradients that need no further row sum
-    float s3 = 0.f, s4 = 0.f;
+    // d, dr and the column sums; then d becomes p = f g d inv_y, the part of dy that needs no
+    // further row sum: dy = p - y inv_y^2 mean(p y)
+    float s3 = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) d[v][i] = 0.f;
       if (c >= H) continue;
+      float t[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) t[i] = 0.f;
+      if (a.grad_residual) row_vals<RING, VEC>(dr_row, c, t);
       if (pre) {
-        float w[VEC];
-        factors.template z<VEC>(c, w);
+        float f[VEC], dz[VEC];
+        factors.template z<VEC>(c, f);
+        dz_in[v].floats(dz);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float nh = n[v][i] * inv_n;
-          sum_z[v][i] = fmaf(d[v][i], nh, sum_z[v][i]);
-          d[v][i] = inv_n * (d[v][i] * w[i] - nh * mean);
+          const float e = dz[i] * inv_n;
+          sum_z[v][i] = fmaf(e, n[v][i], sum_z[v][i]);
+          d[v][i] = fmaf(e, f[i], fmaf(-c_n, n[v][i], t[i]));
         }
-      }
-      if (a.grad_residual) {
-        float dr[VEC];
-        row_vals<RING, VEC>(dr_row, c, dr);
+      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d[v][i] += dr[i];
+        for (int i = 0; i < VEC; ++i) d[v][i] = t[i];
       }
-      float t[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) t[i] = a.residual_scale * d[v][i];
       store_vals<VEC>(static_cast<TR*>(a.d_residual) + base + c, t);
       if (!has_y) continue;
-      float w[VEC], g[VEC];
-      factors.template y<VEC>(c, w);
-      gate_of(c, g);
+      float f[VEC], y[VEC];
+      factors.template y<VEC>(c, f);
+      y_in[v].floats(y);
+      if (full) {
+        float g[VEC];
+        load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) t[i] = d[v][i] * y[v][i];  // a token's or full gate's dg = w_post t
-      if (a.gate_mode == STAGEML_GATE_FULL) {
-        float dg[VEC];
+        for (int i = 0; i < VEC; ++i) {
+          const float e = d[v][i] * inv_y, p = e * f[i];
+          t[i] = p * y[i];  // dg
+          sum_y[v][i] = fmaf(e * g[i], y[i], sum_y[v][i]);
+          d[v][i] = p * g[i];
+          s3 = fmaf(d[v][i], y[i], s3);
+        }
+        store_param<VEC>(a.d_gate, a.gate_dtype, base + c, t);
+      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) dg[i] = w[i] * t[i];
-        store_param<VEC>(a.d_gate, a.gate_dtype, base + c, dg);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        s4 = fmaf(w[i], t[i], s4);
-        sum_y[v][i] = fmaf(g[i], t[i], sum_y[v][i]);  // g is 1 for a per-channel gate
-        d[v][i] *= g[i] * w[i];  // the gradient of y^
-        s3 = fmaf(d[v][i], y[v][i], s3);
+        for (int i = 0; i < VEC; ++i) {  // without the token's gate, which multiplies the sums
+          const float e = d[v][i] * inv_y;
+          sum_y[v][i] = fmaf(e * token_gate, y[i], sum_y[v][i]);
+          d[v][i] = e * f[i];
+          s3 = fmaf(d[v][i], y[i], s3);
+        }
       }
     }
+    float c_y = 0.f;
     if (has_y && (post || a.gate_mode == STAGEML_GATE_TOKEN)) {
-      const float2 s = row_sum<WARP>(s3, s4, red, phase);
-      s3 = s.x * inv_h;
-      if (a.gate_mode == STAGEML_GATE_TOKEN && tid == 0) store_param1(a.d_gate, a.gate_dtype, row, s.y);
+      s3 = row_sum<WARP>(s3, red, phase);
+      if (a.gate_mode == STAGEML_GATE_TOKEN && tid == 0) store_param1(a.d_gate, a.gate_dtype, row, s3);
+      if (post) c_y = s3 * token_gate * inv_h * inv_y * inv_y;
     } else if (RING) {
       __syncthreads();
     }
     // the row's copies have been read by every thread (the barrier above)
     if constexpr (RING)
-      if (threadIdx.x == 0) fill(count + kStages);
+      if (threadIdx.x == 0) fill(count + STAGES);
     if (!has_y) continue;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
       if (c >= H) continue;
-      float t[VEC];
+      float t[VEC], y[VEC];
+      y_in[v].floats(y);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) t[i] = post ? inv_y * (d[v][i] - y[v][i] * s3) : d[v][i];
+      for (int i = 0; i < VEC; ++i) t[i] = fmaf(-c_y, y[i], token_gate * d[v][i]);
       store_vals<VEC>(static_cast<TY*>(a.d_block_out) + base + c, t);
     }
   }
@@ -662,7 +733,7 @@ int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStre
   int64_t grid = (a.T + s.rows_per_cta - 1) / s.rows_per_cta;
   size_t smem = 0;
   if (STAGED) {
-    smem = (RING ? (size_t)kStages * a.H * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
+    smem = RING ? (size_t)kForwardStages * a.H * (sizeof(TR) + sizeof(TY)) : 0;
     SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     grid = resident_ctas(kernel, s.threads, smem, a.T);
   }
@@ -677,7 +748,7 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
   const int n_sums = n_sums_of(a);
   size_t smem = 0;
   if (STAGED) {
-    smem = (RING ? (size_t)kStages * a.H * 2 * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
+    smem = (RING ? (size_t)kBackwardStages * a.H * 2 * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
     SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
   const int grid = resident_ctas(kernel, s.threads, smem, (a.T + s.rows_per_cta - 1) / s.rows_per_cta);
@@ -703,13 +774,14 @@ int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStre
   if (vectors(a)) {
     const int units = a.H / 8;
     if (units <= 32) return SB_NORM(8, 1, true, false, false, units);
-    const size_t ring = (size_t)kStages * a.H * (sizeof(TR) + sizeof(TY)) * (backward ? 2 : 1) + factor_bytes(a);
+    const size_t row = a.H * (sizeof(TR) + sizeof(TY));
+    const size_t ring = backward ? 2 * kBackwardStages * row + factor_bytes(a) : kForwardStages * row;
     if (!many || ring > kMaxSmem) {
       if (units <= kMaxThreads) return SB_NORM(8, 1, false, false, false, units);
       if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, false, false, units);
       return SB_NORM(8, 4, false, false, false, units);
     }
-    if (units <= 256) return SB_NORM(8, 1, false, true, true, units);
+    if (units <= (backward ? kMaxThreads : 256)) return SB_NORM(8, 1, false, true, true, units);
     if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, true, true, units);
     return SB_NORM(8, 4, false, true, true, units);
   }
