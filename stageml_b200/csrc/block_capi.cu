@@ -148,11 +148,11 @@ int norm_validate(const stageml_norm_args* a, bool backward, bool check_ptrs) {
   SB_CHECK_ARG(is_float(a->resid_dtype) && is_float(a->block_dtype), "norm_residual: dtypes must be F32, BF16 or F16");
   SB_CHECK_ARG(a->resid_dtype == STAGEML_F32 || a->block_dtype == a->resid_dtype,
                "norm_residual: a 16-bit residual needs block rows of its own dtype");
-  SB_CHECK_ARG(a->block_out || (!a->post_weight && a->gate_mode == STAGEML_GATE_NONE),
+  SB_CHECK_ARG(a->block_out || a->T == 0 || (!a->post_weight && a->gate_mode == STAGEML_GATE_NONE),
                "norm_residual: post_weight and gate need block_out");
   SB_CHECK_ARG(a->gate_mode >= STAGEML_GATE_NONE && a->gate_mode <= STAGEML_GATE_FULL, "norm_residual: gate mode %d",
                a->gate_mode);
-  SB_CHECK_ARG((a->gate_mode == STAGEML_GATE_NONE) == (a->gate == nullptr), "norm_residual: gate and gate_mode disagree");
+  SB_CHECK_ARG(a->T == 0 || (a->gate_mode == STAGEML_GATE_NONE) == (a->gate == nullptr), "norm_residual: gate and gate_mode disagree");
   SB_CHECK_ARG((!a->post_weight || is_float(a->post_dtype)) && (!a->gate || is_float(a->gate_dtype)) &&
                    (!a->pre_weight || is_float(a->pre_dtype)),
                "norm_residual: weights must be F32, BF16 or F16");
