@@ -227,32 +227,35 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const 
   return w;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_row16(T* dst, const float* v, int valid, bool vec) {
-  if (vec && valid >= 16) {
-    if (sizeof(T) == 2) {
-      float lo[8], hi[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) lo[i] = v[i], hi[i] = v[8 + i];
-      reinterpret_cast<uint4*>(dst)[0] = pack8<T>(lo);
-      reinterpret_cast<uint4*>(dst)[1] = pack8<T>(hi);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < valid) dst[i] = from_f32<T>(v[i]);
-  }
+// Four lanes hold a row each, in four pieces of 16 bytes; afterwards lane i of the four holds piece
+// i of the four rows (v[r] of row r). A thread of the epilogue owns a row, and a warp's store of one
+// piece per row touches 32 lines, one per clock; transposed it touches 8 (64 bytes of each row).
+__device__ __forceinline__ void transpose_pieces(uint4 (&v)[4]) {
+  const bool hi = threadIdx.x & 2, odd = threadIdx.x & 1;
+  auto swap = [](uint4& a, uint4& b, bool up, int mask) {  // up: a goes, else b
+    uint4 t = up ? a : b;
+    t.x = __shfl_xor_sync(0xffffffffu, t.x, mask);
+    t.y = __shfl_xor_sync(0xffffffffu, t.y, mask);
+    t.z = __shfl_xor_sync(0xffffffffu, t.z, mask);
+    t.w = __shfl_xor_sync(0xffffffffu, t.w, mask);
+    (up ? a : b) = t;
+  };
+  swap(v[0], v[2], hi, 2);
+  swap(v[1], v[3], hi, 2);
+  swap(v[0], v[1], odd, 1);
+  swap(v[2], v[3], odd, 1);
 }
-template <>
-__device__ __forceinline__ void store_row16<float>(float* dst, const float* v, int valid, bool vec) {
-  if (vec && valid >= 16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+
+// 16 bytes of outputs from the sums.
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* f) {
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   } else {
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < valid) dst[i] = v[i];
+    for (int i = 0; i < 8; ++i) v[i] = f[i];
+    return pack8<T>(v);
   }
 }
 
@@ -331,6 +334,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Unit w = unit_of(p, u, 2, first);
       const int64_t row = (int64_t)(w.m + rank) * BM + row_in_tile;
       const bool row_ok = rank < w.tiles && row < p.rows;
+      const int64_t row4 = row - (lane & 3);  // this lane's four rows of the epilogue
+      const int rows4 = rank < w.tiles ? (int)max((int64_t)0, min((int64_t)4, p.rows - row4)) : 0;
       // The up rows start at N inside the group, so a tile's up columns can straddle two 128-row
       // scale blocks: the columns below `cut` take the first, the others the second. N % 16 == 0,
       // so 16 columns share a scale.
@@ -431,36 +436,55 @@ __global__ void __launch_bounds__(THREADS, 1)
         // h never leaves in another form, so its codes may come from the reciprocal: the quotient
         // is off by an ulp of fp32 at most, 2^-20 of an e4m3 step
         const float inv = 1.f / s;
-        if (row_ok) {
-          uint8_t* q = p.q_out + row * p.N + n0;
+        uint4 codes[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (n0 + 16 * c < p.N) {  // N % 16 == 0: 16 columns are inside or outside
-              uint32_t v[4];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float* f = acc + 16 * c + 4 * i;
-                const uint32_t lo =
-                    __nv_cvt_float2_to_fp8x2(make_float2(f[0] * inv, f[1] * inv), __NV_SATFINITE, __NV_E4M3);
-                const uint32_t hi =
-                    __nv_cvt_float2_to_fp8x2(make_float2(f[2] * inv, f[3] * inv), __NV_SATFINITE, __NV_E4M3);
-                v[i] = lo | hi << 16;
-              }
-              *reinterpret_cast<uint4*>(q + 16 * c) = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int i = 0; i < 4; ++i) {
+            const float* f = acc + 16 * c + 4 * i;
+            const uint32_t lo =
+                __nv_cvt_float2_to_fp8x2(make_float2(f[0] * inv, f[1] * inv), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi =
+                __nv_cvt_float2_to_fp8x2(make_float2(f[2] * inv, f[3] * inv), __NV_SATFINITE, __NV_E4M3);
+            v[i] = lo | hi << 16;
+          }
+          codes[c] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        transpose_pieces(codes);
+        const int n = n0 + 16 * (lane & 3);
+        if (n < p.N) {  // N % 16 == 0: 16 columns are inside or outside
+          uint8_t* q = p.q_out + row4 * p.N + n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < rows4) *reinterpret_cast<uint4*>(q + (int64_t)r * p.N) = codes[r];
+        }
+        if (row_ok && half == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s;
+      } else {
+        constexpr int PIECE = 16 / (int)sizeof(OutT);
+        const int n0 = w.n * BN + 128 * half;
+        const float rs = row_ok && p.row_scale ? p.row_scale[row] : 1.f;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] *= rs;
+        if (vec) {
+          OutT* out = static_cast<OutT*>(p.out) + row4 * p.N + n0 + PIECE * (lane & 3);
+#pragma unroll
+          for (int c = 0; c < 128; c += 4 * PIECE) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = pack16<OutT>(acc + c + PIECE * i);
+            transpose_pieces(v);
+            if (n0 + c + PIECE * (lane & 3) < p.N) {  // N % PIECE == 0
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (r < rows4) *reinterpret_cast<uint4*>(out + (int64_t)r * p.N + c) = v[r];
             }
           }
-          if (half == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s;
-        }
-      } else if (row_ok) {
-        const int n0 = w.n * BN + 128 * half;
-        const float rs = p.row_scale ? p.row_scale[row] : 1.f;
-        OutT* out = static_cast<OutT*>(p.out) + row * p.N + n0;
+        } else if (row_ok) {
+          OutT* out = static_cast<OutT*>(p.out) + row * p.N + n0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int valid = p.N - (n0 + 16 * c);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[16 * c + i] *= rs;
-          if (valid > 0) store_row16<OutT>(out + 16 * c, acc + 16 * c, valid, vec);
+          for (int i = 0; i < 128; ++i)
+            if (n0 + i < p.N) out[i] = from_f32<OutT>(acc[i]);
         }
       }
     }

@@ -34,6 +34,8 @@
 // so at most two sums per column (S and dw_pre's) are kept, in the registers of the thread
 // that owns the column. Each CTA takes every gridDim-th row and writes its sums once; a second
 // kernel adds them in CTA order: no atomics, the same bits on every run. Bound: HBM.
+#include <atomic>
+
 #include "block_codes.cuh"
 #include "block_fp8.h"
 #include "common.cuh"
@@ -316,10 +318,15 @@ struct RowRing {
   }
 };
 
+// Without a ring every input of a row is loaded before its first sum, while the values fit in
+// registers: one memory latency per row instead of one per phase.
+__host__ __device__ constexpr bool eager_loads(bool ring, int values) { return !ring && values <= 8; }
+
 // HELD: persistent CTAs, the factors of a thread's columns in its registers.
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool HELD>
 __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stageml_norm_args a, float* z32) {
   constexpr int STAGES = kForwardStages;
+  constexpr bool EAGER = eager_loads(RING, V * VEC);
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
   __shared__ uint64_t bars[STAGES];
@@ -368,6 +375,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       y_row.shared = r_row.shared + r_bytes;
     }
     float n[V][VEC];
+    Held<VEC, TR> r_in[EAGER ? V : 1];
     float sq = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -375,9 +383,13 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
 #pragma unroll
       for (int i = 0; i < VEC; ++i) n[v][i] = 0.f;
       if (a.block_out && c < H) row_vals<RING, VEC>(y_row, c, n[v]);
+      if constexpr (EAGER)
+        if (c < H) r_in[v].template load<false>(r_row, c);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sq = fmaf(n[v][i], n[v][i], sq);
-    }
     float scale = a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
     if (a.post_weight) scale *= rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
     sq = 0.f;
@@ -397,7 +409,10 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
         }
       }
       float r[VEC];
-      row_vals<RING, VEC>(r_row, c, r);
+      if constexpr (EAGER)
+        r_in[v].floats(r);
+      else
+        row_vals<RING, VEC>(r_row, c, r);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         n[v][i] = fmaf(n[v][i], scale, a.residual_scale * r[i]);
@@ -460,8 +475,10 @@ __host__ __device__ inline int n_sums_of(const stageml_norm_args& a) {
 }
 
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
-__global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_residual_backward_kernel(const stageml_norm_args a, float* partial) {
+__global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V * VEC <= 4) ? 2 : 1)
+    norm_residual_backward_kernel(const stageml_norm_args a, float* partial) {
   constexpr int STAGES = kBackwardStages;
+  constexpr bool EAGER = eager_loads(RING, V * VEC);
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
   __shared__ uint64_t bars[STAGES];
@@ -510,6 +527,7 @@ __global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_resi
       dz_row.shared = y_row.shared + y_bytes;
     }
     Held<VEC, TY> y_in[V], dz_in[V];
+    Held<VEC, TR> r_in[EAGER ? V : 1], dr_in[EAGER ? V : 1];
     float n[V][VEC], d[V][VEC];
     // With f the channel's factor and g a gate that is not part of it: n = a r + f g y inv_y.
     const bool full = a.gate_mode == STAGEML_GATE_FULL;
@@ -521,6 +539,17 @@ __global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_resi
       const int c = (v * nt + tid) * VEC;
       y_in[v].zero();
       if (c < H && has_y) y_in[v].template load<RING>(y_row, c);
+      if constexpr (EAGER) {
+        dz_in[v].zero(), dr_in[v].zero();
+        if (c < H) {
+          r_in[v].template load<false>(r_row, c);
+          if (pre) dz_in[v].template load<false>(dz_row, c);
+          if (a.grad_residual) dr_in[v].template load<false>(dr_row, c);
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
       float y[VEC];
       y_in[v].floats(y);
 #pragma unroll
@@ -534,7 +563,7 @@ __global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_resi
       const int c = (v * nt + tid) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) n[v][i] = 0.f;
-      dz_in[v].zero();
+      if constexpr (!EAGER) dz_in[v].zero();
       if (c >= H) continue;
       if (has_y) {
         float f[VEC], y[VEC];
@@ -549,12 +578,15 @@ __global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_resi
         }
       }
       float r[VEC];
-      row_vals<RING, VEC>(r_row, c, r);
+      if constexpr (EAGER)
+        r_in[v].floats(r);
+      else
+        row_vals<RING, VEC>(r_row, c, r);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) n[v][i] = fmaf(n[v][i], y_scale, a.residual_scale * r[i]);
       if (pre) {
         float f[VEC], dz[VEC];
-        dz_in[v].template load<RING>(dz_row, c);
+        if constexpr (!EAGER) dz_in[v].template load<RING>(dz_row, c);
         dz_in[v].floats(dz);
         factors.template z<VEC>(c, f);
 #pragma unroll
@@ -582,7 +614,10 @@ __global__ void __launch_bounds__(kMaxThreads, RING && V == 1 ? 2 : 1) norm_resi
       float t[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) t[i] = 0.f;
-      if (a.grad_residual) row_vals<RING, VEC>(dr_row, c, t);
+      if constexpr (EAGER)
+        dr_in[v].floats(t);
+      else if (a.grad_residual)
+        row_vals<RING, VEC>(dr_row, c, t);
       if (pre) {
         float f[VEC], dz[VEC];
         factors.template z<VEC>(c, f);
@@ -712,13 +747,25 @@ Shape shape_of(int units, int per, bool warp) {
 }
 
 // Persistent CTAs of a kernel of `threads` threads and `smem` bytes: as many as fit in an SM's
-// registers and shared memory, at most `rows`.
+// registers and shared memory, at most `rows`. The kernel may then be launched with up to kMaxSmem.
+// The two calls cost 2 to 3 us; `last` keeps the kernel's latest answer with the device, threads and
+// bytes that it is for.
 template <typename K>
-int resident_ctas(K kernel, int threads, size_t smem, int64_t rows) {
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem) != cudaSuccess || per_sm < 1)
-    per_sm = 1;
-  return (int)std::min<int64_t>(rows, (int64_t)sm_count() * per_sm);
+int resident_ctas(std::atomic<uint64_t>& last, K kernel, int threads, size_t smem, int64_t rows, int* grid) {
+  int dev = 0, per_sm = 0;
+  SB_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t key = (uint64_t)(dev + 1) << 48 | (uint64_t)threads << 32 | (uint64_t)smem << 8;
+  const uint64_t known = last.load(std::memory_order_relaxed);
+  if ((known & ~uint64_t(0xff)) == key) {
+    per_sm = (int)(known & 0xff);
+  } else {
+    SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem));
+    SB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    per_sm = std::max(per_sm, 1);
+    last.store(key | (uint64_t)per_sm, std::memory_order_relaxed);
+  }
+  *grid = (int)std::min<int64_t>(rows, (int64_t)sm_count() * per_sm);
+  return STAGEML_OK;
 }
 
 // The most owners of column sums (workspace): 2048 threads per SM.
@@ -730,12 +777,12 @@ int max_owners(const stageml_norm_args& a) {
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStream_t stream) {
   auto kernel = norm_residual_kernel<TR, TY, VEC, V, WARP, RING, STAGED>;
-  int64_t grid = (a.T + s.rows_per_cta - 1) / s.rows_per_cta;
+  static std::atomic<uint64_t> resident{0};
+  int grid = (int)((a.T + s.rows_per_cta - 1) / s.rows_per_cta);
   size_t smem = 0;
   if (STAGED) {
     smem = RING ? (size_t)kForwardStages * a.H * (sizeof(TR) + sizeof(TY)) : 0;
-    SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    grid = resident_ctas(kernel, s.threads, smem, a.T);
+    SB_TRY(resident_ctas(resident, kernel, s.threads, smem, a.T, &grid));
   }
   SB_CUDA_CHECK(launch_kernel(kernel, dim3((unsigned)grid), dim3(s.threads), smem, stream, false, a, z32));
   count_launch();
@@ -747,11 +794,11 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
   auto kernel = norm_residual_backward_kernel<TR, TY, VEC, V, WARP, RING, STAGED>;
   const int n_sums = n_sums_of(a);
   size_t smem = 0;
-  if (STAGED) {
+  if (STAGED)
     smem = (RING ? (size_t)kBackwardStages * a.H * 2 * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
-    SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  }
-  const int grid = resident_ctas(kernel, s.threads, smem, (a.T + s.rows_per_cta - 1) / s.rows_per_cta);
+  static std::atomic<uint64_t> resident{0};
+  int grid = 0;
+  SB_TRY(resident_ctas(resident, kernel, s.threads, smem, (a.T + s.rows_per_cta - 1) / s.rows_per_cta, &grid));
   SB_CUDA_CHECK(launch_kernel(kernel, dim3((unsigned)grid), dim3(s.threads), smem, stream, false, a, partial));
   count_launch();
   if (n_sums) {
@@ -786,6 +833,8 @@ int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStre
     return SB_NORM(8, 4, false, true, true, units);
   }
   if (a.H <= 256) return SB_NORM(1, 8, true, false, false, a.H);
+  if (a.H <= 4 * kMaxThreads)
+    return many ? SB_NORM(1, 4, false, false, true, a.H) : SB_NORM(1, 4, false, false, false, a.H);
   if (a.H <= 8 * kMaxThreads)
     return many ? SB_NORM(1, 8, false, false, true, a.H) : SB_NORM(1, 8, false, false, false, a.H);
   return many ? SB_NORM(1, 32, false, false, true, a.H) : SB_NORM(1, 32, false, false, false, a.H);

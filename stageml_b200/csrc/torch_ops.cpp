@@ -11,6 +11,7 @@
 // current CUDA stream; workspaces come from the caching allocator.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -55,8 +56,14 @@ void check_cuda(const Tensor& t, const char* name, const Tensor& ref) {
 
 const void* opt_ptr(const c10::optional<Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
+// An uninitialised contiguous tensor on ref's device, without the dispatcher's way there (0.5 us of a call
+// whose kernel may take 3).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& ref) {
+  return at::detail::empty_cuda(sizes, dtype, ref.device(), c10::nullopt);
+}
+
 Tensor workspace(size_t bytes, const Tensor& ref) {
-  return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, ref.options().dtype(at::kByte));
+  return fresh({(int64_t)std::max<size_t>(bytes, 16)}, at::kByte, ref);
 }
 
 // Per-device status word that kernels write data-dependent errors into.
@@ -440,8 +447,8 @@ std::tuple<Tensor, Tensor> quantize_e4m3_blocks(const Tensor& x, bool tiles) {
   auto sizes = x.sizes().vec();
   sizes.back() = blocks128(cols);
   if (tiles) sizes[sizes.size() - 2] = blocks128(rows);
-  auto q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  auto s = at::empty(sizes, x.options().dtype(at::kFloat));
+  auto q = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
+  auto s = fresh(sizes, at::kFloat, x);
   check_rc(stageml_quantize_e4m3_blocks(x.data_ptr(), dtype_code(x), batch, rows, cols, tiles ? 1 : 0,
                                         static_cast<uint8_t*>(q.data_ptr()), s.data_ptr<float>(), cur_stream()),
            "quantize_e4m3_blocks");
@@ -467,7 +474,7 @@ Tensor block_matmul(const Tensor& x, const Tensor& x_scale, const Tensor& w, con
                   w_scale.size(1) == blocks128(K),
               "block_matmul: w_scale must be fp32 [ceil(N/128), ceil(K/128)], got ", w_scale.sizes());
   c10::cuda::CUDAGuard guard(x.device());
-  auto out = at::empty({M, N}, x.options().dtype(out_dtype));
+  auto out = fresh({M, N}, out_dtype, x);
   check_float_dtype(out, "block_matmul: out_dtype");
   const size_t bytes = stageml_block_matmul_workspace_bytes((int)M, (int)N, (int)K);
   Tensor ws = bytes ? workspace(bytes, x) : Tensor();
@@ -512,7 +519,7 @@ Tensor moe_forward_blocks(const Tensor& x, const Tensor& gate_up, const Tensor& 
     k = topk_ids->size(1);
   }
   c10::cuda::CUDAGuard guard(x.device());
-  auto out = at::empty({T, H}, x.options());
+  auto out = fresh({T, H}, x.scalar_type(), x);
   stageml_moe_blocks_args a{};
   a.T = (int)T;
   a.H = (int)H;
@@ -626,17 +633,17 @@ std::vector<Tensor> norm_residual(const c10::optional<Tensor>& block_out, const 
   c10::cuda::CUDAGuard guard(residual.device());
   std::vector<Tensor> out;
   out.reserve(3);
-  out.push_back(at::empty(residual.sizes(), residual.options()));
+  out.push_back(fresh(residual.sizes(), residual.scalar_type(), residual));
   a.new_residual = out[0].data_ptr();
   if (quantize) {
     auto sizes = residual.sizes().vec();
     sizes.back() = blocks128(a.H);
-    out.push_back(at::empty(residual.sizes(), residual.options().dtype(at::kFloat8_e4m3fn)));
-    out.push_back(at::empty(sizes, residual.options().dtype(at::kFloat)));
+    out.push_back(fresh(residual.sizes(), at::kFloat8_e4m3fn, residual));
+    out.push_back(fresh(sizes, at::kFloat, residual));
     a.codes = static_cast<uint8_t*>(out[1].data_ptr());
     a.code_scale = out[2].data_ptr<float>();
   } else if (pre_weight.has_value()) {
-    out.push_back(at::empty(residual.sizes(), residual.options().dtype(bd)));
+    out.push_back(fresh(residual.sizes(), bd, residual));
     a.normed = out[1].data_ptr();
   }
   const size_t bytes = stageml_norm_residual_workspace_bytes(&a, 0);
@@ -671,7 +678,7 @@ std::vector<Tensor> norm_residual_backward(const c10::optional<Tensor>& grad_res
   std::vector<Tensor> out;
   out.reserve(5);
   auto add = [&](const Tensor& like) {
-    out.push_back(at::empty(like.sizes(), like.options()));
+    out.push_back(fresh(like.sizes(), like.scalar_type(), like));
     return out.back().data_ptr();
   };
   a.d_residual = add(residual);
@@ -706,9 +713,9 @@ std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, const Tens
   TORCH_CHECK(E >= 1 && E <= 256 && k >= 1 && k <= 8, "balance_loss: E=", E, " must be in 1..256 and k=", k, " in 1..8");
   const uint8_t* v = valid_ptr(valid, logits);
   c10::cuda::CUDAGuard guard(logits.device());
-  auto loss = at::empty({}, logits.options().dtype(at::kFloat));
-  auto counts = at::empty({E}, logits.options().dtype(at::kInt));
-  auto tokens = at::empty({}, logits.options().dtype(at::kInt));
+  auto loss = fresh({}, at::kFloat, logits);
+  auto counts = fresh({E}, at::kInt, logits);
+  auto tokens = fresh({}, at::kInt, logits);
   const size_t bytes = stageml_balance_workspace_bytes(T, (int)E);
   Tensor w = bytes ? workspace(bytes, logits) : Tensor();
   check_rc(stageml_balance_loss(logits.data_ptr(), dtype_code(logits), topk_ids.data_ptr(), dtype_code(topk_ids), v, T,
@@ -731,7 +738,7 @@ Tensor balance_loss_backward(const Tensor& grad_loss, const Tensor& logits, cons
               "balance_loss_backward: counts int32 [E] and tokens int32 [1] of the forward");
   const uint8_t* v = valid_ptr(valid, logits);
   c10::cuda::CUDAGuard guard(logits.device());
-  auto grad = at::empty_like(logits);
+  auto grad = fresh(logits.sizes(), logits.scalar_type(), logits);
   check_rc(stageml_balance_loss_backward(grad_loss.data_ptr<float>(), logits.data_ptr(), dtype_code(logits),
                                          counts.data_ptr<int32_t>(), tokens.data_ptr<int32_t>(), v, logits.size(0),
                                          (int)logits.size(1), (int)k, (float)coefficient, grad.data_ptr(), cur_stream()),
