@@ -25,7 +25,13 @@
 // h = silu(gate) * up in fp32 and writes it as e4m3 codes with one scale per (row, 128
 // columns), the next product's operand, so h never exists in 16 bits.
 //
+// Plain products of few tiles: clusters of two or four pairs, each with its share of a tile's K blocks;
+// the sums meet over distributed shared memory, in a fixed order, and each pair stores its share of
+// the columns.
+//
 // Every wait is bounded. No load is multicast.
+#include <atomic>
+
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -57,8 +63,9 @@ constexpr int SLOT_FLOATS = (BM + 4) * GROUP;
 constexpr int MAX_GROUPS = 1024;
 constexpr int kBandUnits = 8;            // plain rows: row units that share a pass over the columns
 constexpr int BAR_BYTES = 512;
+constexpr int TURN_PITCH = 17;           // floats per row of a math warp's 32 x 16 turning area
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + BAR_BYTES + 2 * 2 * BM * 4 /*row maxima*/ +
-                           SLOTS * SLOT_FLOATS * 4 + (MAX_GROUPS + 1) * 4;
+                           SLOTS * SLOT_FLOATS * 4 + 2 * HALF_WARPS * 32 * TURN_PITCH * 4 + (MAX_GROUPS + 1) * 4;
 static_assert(BUFS == 4, "two halves, two K blocks in flight");
 static_assert(SMEM_BYTES <= 232448, "shared memory per block");
 static_assert((2 * STAGES + 2 * BUFS + 2 + 2 * SLOTS) * 8 + 16 <= BAR_BYTES, "barrier area");
@@ -259,8 +266,102 @@ __device__ __forceinline__ uint4 pack16(const float* f) {
   }
 }
 
-// OutT: output element (plain); SWIGLU writes codes and ignores it.
-template <typename OutT, bool SWIGLU>
+// Stores W columns of a row per thread, the warp's 32 rows four by four (rows4 of `row`'s four exist);
+// where the rows do not start at 16 bytes, 16 columns at a time through `turn`, so that a warp's store
+// is of two rows' 16 columns (a thread storing its own row: 300 x 500 x 1536 in 44 us).
+template <typename OutT, int W>
+__device__ __forceinline__ void store_columns(const Params& p, float* v, float factor, int64_t row, int rows4, int n0,
+                                              float* turn) {
+  constexpr int PIECE = 16 / (int)sizeof(OutT);
+#pragma unroll
+  for (int i = 0; i < W; ++i) v[i] *= factor;
+  const int mine = threadIdx.x & 3;
+  if (p.N % PIECE == 0) {
+    OutT* out = static_cast<OutT*>(p.out) + (row - mine) * p.N + n0 + PIECE * mine;
+#pragma unroll
+    for (int c = 0; c < W; c += 4 * PIECE) {
+      uint4 u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = pack16<OutT>(v + c + PIECE * i);
+      transpose_pieces(u);
+      if (n0 + c + PIECE * mine < p.N) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r < rows4) *reinterpret_cast<uint4*>(out + (int64_t)r * p.N + c) = u[r];
+      }
+    }
+  } else {
+    const int lane = threadIdx.x & 31;
+    const int64_t row0 = row - lane;
+#pragma unroll
+    for (int c = 0; c < W; c += 16) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) turn[lane * TURN_PITCH + i] = v[c + i];
+      __syncwarp();
+      const int n = n0 + c + (lane & 15);
+      OutT* out = static_cast<OutT*>(p.out) + (row0 + (lane >> 4)) * p.N + n;
+#pragma unroll 4
+      for (int r = 0; r < 32; r += 2, out += 2 * (int64_t)p.N) {
+        const float f = turn[(r + (lane >> 4)) * TURN_PITCH + (lane & 15)];
+        // rows4 of the lane that owns this row tells whether it exists
+        const int there = __shfl_sync(0xffffffffu, rows4, r + (lane >> 4));
+        if (n < p.N && there > ((r + (lane >> 4)) & 3)) *out = from_f32<OutT>(f);
+      }
+    }
+  }
+}
+
+// The sums of a cluster's S pairs, each over its share of K: pair q ends with the tile's q-th 128 / S
+// columns of each half. The others' sums of them arrive in the operand stages, which nothing reads
+// any more once every pair has come to the first barrier ([pair][half][4 columns][row] in 16 bytes,
+// so that a warp writes 512 bytes in a row). Its own sums first, then the others' in their order: the same
+// bits every time.
+template <int S>
+__device__ __forceinline__ void join_splits(const float* acc, float* own, uint32_t stage, int rank, int split, int half,
+                                            int row) {
+  constexpr int W = 128 / S;
+  static_assert(S * 2 * W * BM * 4 <= STAGES * STAGE_BYTES, "exchange area");
+  auto place = [&](int from, int c) { return (uint32_t)((((from * 2 + half) * (W / 4) + c / 4) * BM + row) * 16); };
+  __syncwarp();
+  cluster_sync_all();
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    if (q == split) continue;
+    const uint32_t dst = mapa_shared(stage, 2 * q + rank);
+#pragma unroll
+    for (int c = 0; c < W; c += 4)
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + place(split, c)),
+                   "f"(acc[q * W + c]), "f"(acc[q * W + c + 1]), "f"(acc[q * W + c + 2]), "f"(acc[q * W + c + 3])
+                   : "memory");
+  }
+#pragma unroll
+  for (int c = 0; c < W; ++c) {
+    own[c] = acc[c];
+#pragma unroll
+    for (int q = 1; q < S; ++q) own[c] = split == q ? acc[q * W + c] : own[c];
+  }
+  __syncwarp();
+  cluster_sync_all();
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    if (q == split) continue;
+#pragma unroll
+    for (int c = 0; c < W; c += 4) {
+      float f[4];
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                   : "r"(stage + place(q, c))
+                   : "memory");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) own[c + i] += f[i];
+    }
+  }
+}
+
+// OutT: output element (plain); SWIGLU writes codes and ignores it. SPLITS pairs of a cluster share a
+// tile's K blocks; a cluster then has one tile.
+template <typename OutT, bool SWIGLU, int SPLITS>
 __global__ void __launch_bounds__(THREADS, 1)
     block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                            const Params p) {
@@ -273,7 +374,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t abort_flag = smem_u32(tmem_slot + 1);
   uint32_t* row_max = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + BAR_BYTES);  // [2][2][128]
   float* scales = reinterpret_cast<float*>(row_max + 2 * 2 * BM);                                 // [SLOTS][SLOT_FLOATS]
-  int32_t* first = reinterpret_cast<int32_t*>(scales + SLOTS * SLOT_FLOATS);                      // [groups + 1]
+  float* turns = scales + SLOTS * SLOT_FLOATS;                                                    // [math warps][32][17]
+  int32_t* first = reinterpret_cast<int32_t*>(turns + 2 * HALF_WARPS * 32 * TURN_PITCH);          // [groups + 1]
   auto full_bar = [&](int s) { return smem_u32(&bars[s]); };                // both CTAs' copies (even CTA)
   auto empty_bar = [&](int s) { return smem_u32(&bars[STAGES + s]); };
   auto tfull_bar = [&](int i) { return smem_u32(&bars[2 * STAGES + i]); };
@@ -283,8 +385,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto sfull_bar = [&](uint32_t i) { return smem_u32(&bars[2 * STAGES + 2 * BUFS + 2 + i]); };
   auto sempty_bar = [&](uint32_t i) { return smem_u32(&bars[2 * STAGES + 2 * BUFS + 2 + SLOTS + i]); };
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
-  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const int cta = (int)cluster_ctarank(), rank = SPLITS == 1 ? cta : cta & 1;
+  const int lead = SPLITS == 1 ? 0 : cta - rank, split = SPLITS == 1 ? 0 : cta >> 1;
+  const int cluster = blockIdx.x / (2 * SPLITS), clusters = gridDim.x / (2 * SPLITS);
+  const int kb_begin = SPLITS == 1 ? 0 : p.kb * split / SPLITS;
+  const int kb_count = SPLITS == 1 ? p.kb : p.kb * (split + 1) / SPLITS - kb_begin;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -326,16 +431,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int row_in_tile = quarter * 32 + lane;
     // this thread's lane of its half's accumulator: all 128 columns (SwiGLU: 64 gate, the same 64 up)
     const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * NACC;
-    const uint32_t lead_tempty = mapa_shared(tempty_bar(0), 0);
-    const bool vec = p.N % (16 / (int)sizeof(OutT)) == 0;
+    const uint32_t lead_tempty = mapa_shared(tempty_bar(0), lead);
     uint32_t it = 0, grp = 0, tile = 0;
-    bool ok = true;
+    bool ok = true, joined = false;
     for (int u = cluster; ok && u < units; u += clusters, ++tile) {
       const Unit w = unit_of(p, u, 2, first);
       const int64_t row = (int64_t)(w.m + rank) * BM + row_in_tile;
       const bool row_ok = rank < w.tiles && row < p.rows;
-      const int64_t row4 = row - (lane & 3);  // this lane's four rows of the epilogue
-      const int rows4 = rank < w.tiles ? (int)max((int64_t)0, min((int64_t)4, p.rows - row4)) : 0;
       // The up rows start at N inside the group, so a tile's up columns can straddle two 128-row
       // scale blocks: the columns below `cut` take the first, the others the second. N % 16 == 0,
       // so 16 columns share a scale.
@@ -356,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) break;
       tc_fence_after();
       tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
-      for (int kb0 = 0; ok && kb0 < p.kb; kb0 += GROUP) {
+      for (int kb0 = 0; ok && kb0 < kb_count; kb0 += GROUP) {
         const uint32_t sl = grp % SLOTS;
         ok = warp_wait(sfull_bar(sl), (grp / SLOTS) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
         if (!ok) break;
@@ -378,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ++grp;
 #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
-          if (kb0 + j >= p.kb) break;
+          if (kb0 + j >= kb_count) break;
           const uint32_t buf = (it & 1) * 2 + half;
           const uint32_t src = t_lane + (it & 1) * 2 * NACC;
           auto add = [&](int col, const uint32_t* r) {
@@ -404,7 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_before();
           if (lane == 0) arrive_remote(lead_tempty + 8u * buf);
           ++it;
-          if (kb0 + j + 1 < p.kb) {
+          if (kb0 + j + 1 < kb_count) {
             ok = warp_wait(tfull_bar(buf ^ 2), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
             if (!ok) break;
             tc_fence_after();
@@ -414,6 +516,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if (!ok) break;
+      const int64_t row4 = row - (lane & 3);  // the first of the four rows that four lanes store together
+      const int rows4 = rank < w.tiles ? (int)max((int64_t)0, min((int64_t)4, p.rows - row4)) : 0;
       if (SWIGLU) {
         const int n0 = w.n * 128 + 64 * half;
         uint32_t m = 0;
@@ -461,32 +565,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (row_ok && half == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s;
       } else {
-        constexpr int PIECE = 16 / (int)sizeof(OutT);
         const int n0 = w.n * BN + 128 * half;
+        float* turn = turns + (warp - MATH_WARP0) * 32 * TURN_PITCH;
         const float rs = row_ok && p.row_scale ? p.row_scale[row] : 1.f;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) acc[i] *= rs;
-        if (vec) {
-          OutT* out = static_cast<OutT*>(p.out) + row4 * p.N + n0 + PIECE * (lane & 3);
-#pragma unroll
-          for (int c = 0; c < 128; c += 4 * PIECE) {
-            uint4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = pack16<OutT>(acc + c + PIECE * i);
-            transpose_pieces(v);
-            if (n0 + c + PIECE * (lane & 3) < p.N) {  // N % PIECE == 0
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (r < rows4) *reinterpret_cast<uint4*>(out + (int64_t)r * p.N + c) = v[r];
-            }
-          }
-        } else if (row_ok) {
-          OutT* out = static_cast<OutT*>(p.out) + row * p.N + n0;
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (n0 + i < p.N) out[i] = from_f32<OutT>(acc[i]);
+        if constexpr (SPLITS == 1) {
+          store_columns<OutT, 128>(p, acc, rs, row, rows4, n0, turn);
+        } else {
+          constexpr int W = 128 / SPLITS;
+          joined = true;
+          float own[W];
+          join_splits<SPLITS>(acc, own, smem_u32(smem), rank, split, half, row_in_tile);
+          store_columns<OutT, W>(p, own, rs, row, rows4, n0 + W * split, turn);
         }
       }
+    }
+    if (SPLITS > 1 && !joined) {  // an expired wait: the other pairs still meet this one
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONTROL_REGS));
@@ -497,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tma_prefetch_desc(&tm_b);
       const uint64_t pol_a = l2_policy_evict_last(), pol_b = l2_policy_evict_normal();
       const uint32_t base = smem_u32(smem);
-      const uint32_t lead_full = mapa_shared(full_bar(0), 0);
+      const uint32_t lead_full = mapa_shared(full_bar(0), lead);
       uint32_t s = 0, phase = 0, filled = 0;  // filled: bit i = stage i has been filled
       bool ok = true;
       for (int u = cluster; ok && u < units; u += clusters) {
@@ -509,7 +605,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int a0 = (w.m + rank) * BM;
         const bool live = rank < w.tiles;  // an idle half multiplies what its stage holds; nobody stores it
         const uint32_t bytes = (w.tiles * A_BYTES) + 4 * B_HALF_BYTES;  // of both CTAs
-        for (int kb = 0; kb < p.kb; ++kb) {
+        for (int kb = kb_begin; kb < kb_begin + kb_count; ++kb) {
           ok = lane_wait(empty_bar(s), phase ^ 1, empty_bar(s), phase ^ 1, abort_flag, p.status, kDevTimeoutProducer);
           if (!ok) break;
           const uint32_t dst = base + s * STAGE_BYTES, bar = lead_full + 8u * s;
@@ -540,12 +636,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (rank == 0 && elect_one()) {
       constexpr uint32_t idesc = idesc_e4m3(2 * BM, NACC);
       const uint32_t half = warp >> 1;
+      const uint16_t both = (uint16_t)(3 << lead);
       const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
       const uint32_t b_off = (A_BYTES + half * B_HALF_BYTES) >> 4;
       uint32_t s = 0, phase = 0, it = 0;
       bool ok = true;
       for (int u = cluster; ok && u < units; u += clusters) {
-        for (int kb = 0; kb < p.kb; ++kb, ++it) {
+        for (int kb = 0; kb < kb_count; ++kb, ++it) {
           const uint32_t buf = (it & 1) * 2 + half;
           ok = lane_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, full_bar(s), phase, abort_flag, p.status, kDevTimeoutMma);
           if (!ok) break;
@@ -554,8 +651,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
             mma_f8_pair(tmem_base + buf * NACC, ad + 2 * k, bd + 2 * k, idesc, k > 0 ? 1u : 0u);
-          tc_commit_pair_both(tfull_bar(buf), 0x3);
-          tc_commit_pair_both(empty_bar(s), 0x3);
+          tc_commit_pair_both(tfull_bar(buf), both);
+          tc_commit_pair_both(empty_bar(s), both);
           if (++s == STAGES) s = 0, phase ^= 1;
         }
       }
@@ -579,7 +676,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int block = 2 * w.n + (lane & 1);
       if (SWIGLU) block = lane == 0 ? w.n : ((p.N + w.n * 128) >> 7) + (lane == 2);
       const float* sb = p.b_scale + ((int64_t)w.group * p.b_blocks + min(block, p.b_blocks - 1)) * p.kb;
-      for (int kb = 0; kb < p.kb; kb += GROUP, ++grp) {
+      for (int kb = kb_begin; kb < kb_begin + kb_count; kb += GROUP, ++grp) {
         const uint32_t sl = grp % SLOTS;
         ok = warp_wait(sempty_bar(sl), ((grp / SLOTS) & 1) ^ 1, abort_flag, p.status, kDevTimeoutProducer);
         if (!ok) break;
@@ -592,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane < 3) copy_async<16>(dst + 16 * BM, sb + kb, true);
         } else {
 #pragma unroll 1
-          for (int j = 0; j < GROUP && kb + j < p.kb; ++j) {
+          for (int j = 0; j < GROUP && kb + j < kb_begin + kb_count; ++j) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               copy_async<4>(dst + 512 * i + 4 * j, 32 * i < valid ? sa + (int64_t)(32 * i) * p.kb + kb + j : p.a_scale,
@@ -605,6 +702,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  if (SPLITS > 1) {  // the math warps' exchange
+    __syncwarp();
+    cluster_sync_all();
+    cluster_sync_all();
+  }
   }
   __syncwarp();
   tc_fence_before();
@@ -615,18 +717,18 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <typename OutT, bool SWIGLU>
+template <typename OutT, bool SWIGLU, int SPLITS = 1>
 int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int clusters, bool pdl, cudaStream_t stream) {
-  auto kernel = block_gemm_pair_kernel<OutT, SWIGLU>;
+  auto kernel = block_gemm_pair_kernel<OutT, SWIGLU, SPLITS>;
   SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * clusters);
+  cfg.gridDim = dim3(2 * SPLITS * clusters);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = 2 * SPLITS;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -635,6 +737,52 @@ int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int 
   SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, p));
   count_launch();
   return STAGEML_OK;
+}
+
+template <typename OutT>
+int run_plain(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int clusters, int splits, bool pdl,
+              cudaStream_t stream) {
+  if (splits == 4) return run_pair<OutT, false, 4>(ta, tb, p, clusters, pdl, stream);
+  if (splits == 2) return run_pair<OutT, false, 2>(ta, tb, p, clusters, pdl, stream);
+  return run_pair<OutT, false>(ta, tb, p, clusters, pdl, stream);
+}
+
+// Clusters of SPLITS pairs that the device runs at one time (not all of its SMs: a cluster lies in
+// one of its processing clusters). Asked for once per device.
+template <int SPLITS>
+int resident_clusters() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if ((n = known[dev].load(std::memory_order_relaxed)) != 0) return n;
+  auto kernel = block_gemm_pair_kernel<bf16, false, SPLITS>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * SPLITS);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2 * SPLITS;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess)
+    return 0;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Pairs per tile: where the tiles leave SMs idle, several pairs share a tile's K blocks. A K block
+// takes a pair 0.4 us on an idle device and the exchange 2 us, so 12 blocks are worth it (64 x 4096
+// outputs over 8, 16, 32, 112 blocks: 9.8, 13.1, 19.8, 52 us alone, 9.8, 11.7, 15.2, 32 us in two;
+// 300 x 1000 over 32: 19.9 alone, 15.2 in two, 13.3 in four), while all clusters run at one time
+// (64 x 4096 in 16 clusters of eight CTAs: 25 us, in two turns).
+int splits_for(int64_t units, int kb) {
+  if (kb < 12) return 1;
+  if (units <= resident_clusters<4>()) return 4;
+  if (units <= resident_clusters<2>()) return 2;
+  return 1;
 }
 
 }  // namespace
@@ -652,7 +800,6 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   p.n_tiles = g.swiglu ? (int)scale_blocks(g.N) : (g.N + BN - 1) / BN;
   p.a_scale = g.a_scale;
   p.b_scale = g.b_scale;
-  p.vec_scales = p.kb % GROUP == 0 && (reinterpret_cast<uintptr_t>(g.a_scale) | reinterpret_cast<uintptr_t>(g.b_scale)) % 16 == 0;
   p.group_offsets = g.group_offsets;
   p.groups = g.groups;
   p.rows = g.a_rows;
@@ -661,21 +808,25 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   p.q_out = g.q_out;
   p.q_scale = g.q_scale;
   p.status = g.status;
-  CUtensorMap ta, tb;
-  SB_TRY(make_tmap_2d(&ta, g.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.a_rows, (uint64_t)g.K, (uint64_t)g.K, BM,
-                      BK, 128));
-  SB_TRY(make_tmap_2d(&tb, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.groups * p.b_group_rows, (uint64_t)g.K,
-                      (uint64_t)g.K, 64, BK, 128));
   // row units: every group can end in a unit of one tile
   const int64_t tiles = (g.a_rows + BM - 1) / BM;
   const int64_t row_units = g.group_offsets ? std::min<int64_t>(tiles, tiles / 2 + g.groups) : (tiles + 1) / 2;
   const int64_t units = row_units * p.n_tiles;
   SB_CHECK_ARG(units <= 0x7fffffff, "block_gemm: too many tiles");
-  const int clusters = (int)std::min<int64_t>(units, sm_count() / 2);
+  const int pairs = sm_count() / 2;
+  const int splits = g.group_offsets || g.swiglu ? 1 : splits_for(units, p.kb);
+  p.vec_scales = p.kb % (GROUP * splits) == 0 &&
+                 (reinterpret_cast<uintptr_t>(g.a_scale) | reinterpret_cast<uintptr_t>(g.b_scale)) % 16 == 0;
+  CUtensorMap ta, tb;
+  SB_TRY(make_tmap_2d(&ta, g.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.a_rows, (uint64_t)g.K, (uint64_t)g.K, BM,
+                      BK, 128));
+  SB_TRY(make_tmap_2d(&tb, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.groups * p.b_group_rows, (uint64_t)g.K,
+                      (uint64_t)g.K, 64, BK, 128));
+  const int clusters = (int)std::min<int64_t>(units, pairs);
   if (g.swiglu) return run_pair<bf16, true>(ta, tb, p, clusters, g.pdl, stream);
-  if (g.out_dtype == STAGEML_F32) return run_pair<float, false>(ta, tb, p, clusters, g.pdl, stream);
-  if (g.out_dtype == STAGEML_BF16) return run_pair<bf16, false>(ta, tb, p, clusters, g.pdl, stream);
-  return run_pair<f16, false>(ta, tb, p, clusters, g.pdl, stream);
+  if (g.out_dtype == STAGEML_F32) return run_plain<float>(ta, tb, p, clusters, splits, g.pdl, stream);
+  if (g.out_dtype == STAGEML_BF16) return run_plain<bf16>(ta, tb, p, clusters, splits, g.pdl, stream);
+  return run_plain<f16>(ta, tb, p, clusters, splits, g.pdl, stream);
 }
 
 }  // namespace sb

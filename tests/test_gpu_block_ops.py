@@ -163,6 +163,18 @@ def test_block_matmul(ops, m, n, k, out):
     close(y, dequant(x, xs, 1) @ dequant(w, ws, 128).t())
 
 
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n,k", [(17, 130, 1536), (64, 4096, 1552), (300, 500, 2048), (257, 1001, 1616), (500, 4095, 2064),
+                                   (33, 8, 14336), (2048, 1027, 272)])
+def test_block_matmul_shared_k_and_odd_widths(ops, m, n, k, out):
+    """Few tiles with a long K, whose blocks several CTA pairs share, and rows that do not start at 16 bytes."""
+    x, xs, w, ws = operands(m, n, k, seed=m + n + k)
+    y = ops.block_matmul(x, xs, w, ws, out_dtype=out)
+    close(y, dequant(x, xs, 1) @ dequant(w, ws, 128).t())
+    for _ in range(3):
+        assert torch.equal(ops.block_matmul(x, xs, w, ws, out_dtype=out), y)
+
+
 @pytest.mark.parametrize("m", [1, 16, 17, 400])
 def test_block_matmul_rows_do_not_mix(ops, m):
     """A row of NaN codes, or of an infinite scale, stays in its own output row."""
