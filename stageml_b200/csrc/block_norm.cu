@@ -45,13 +45,22 @@ namespace sb {
 namespace {
 
 constexpr int kMaxThreads = 512;
+constexpr int kWarpRows = 8, kWarpWidth = 256;  // rows of a warp each: per CTA, and up to this width
 constexpr int kMaxH = 16384;  // 512 threads x 32 values
 constexpr size_t kMaxSmem = 224 * 1024;  // dynamic shared memory of a CTA
 
 template <int VEC, typename T>
 __device__ __forceinline__ void load_vals(const T* p, float (&f)[VEC]) {
   if constexpr (VEC == 1) {
-    f[0] = to_f32<T>(*p);
+    // read-only as the vectors: a plain load would wait for the stores before it. By its bits: the
+    // 16-bit types' own __ldg is a pure expression to the compiler, which may run it where the branch
+    // around it (a null parameter, a column past the end) says not to.
+    if constexpr (sizeof(T) == 2) {
+      const unsigned short u = __ldg(reinterpret_cast<const unsigned short*>(p));
+      f[0] = to_f32<T>(*reinterpret_cast<const T*>(&u));
+    } else {
+      f[0] = __ldg(p);
+    }
   } else if constexpr (sizeof(T) == 2) {
     unpack8<T>(__ldg(reinterpret_cast<const uint4*>(p)), f);
   } else {
@@ -94,6 +103,63 @@ __device__ __forceinline__ void store_param1(void* p, int dtype, int64_t i, floa
     static_cast<bf16*>(p)[i] = from_f32<bf16>(v);
   else
     static_cast<f16*>(p)[i] = from_f32<f16>(v);
+}
+
+// A thread's columns of a parameter, (v nt + tid) VEC and on for each v, 0 past the row's end. The
+// branch on the type stands outside the loads: a branch per load made each wait for the one before
+// (a row of 13831 columns in 26 us).
+template <int VEC, int V, typename T>
+__device__ __forceinline__ void load_columns(const T* p, int tid, int nt, int H, float (&f)[V][VEC]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (v * nt + tid) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[v][i] = 0.f;
+    if (c < H) load_vals<VEC>(p + c, f[v]);
+  }
+}
+template <int VEC, int V>
+__device__ __forceinline__ void load_columns(const void* p, int dtype, int64_t base, int tid, int nt, int H,
+                                             float (&f)[V][VEC]) {
+  if (dtype == STAGEML_F32)
+    load_columns<VEC, V>(static_cast<const float*>(p) + base, tid, nt, H, f);
+  else if (dtype == STAGEML_BF16)
+    load_columns<VEC, V>(static_cast<const bf16*>(p) + base, tid, nt, H, f);
+  else
+    load_columns<VEC, V>(static_cast<const f16*>(p) + base, tid, nt, H, f);
+}
+
+// The channels' factors of a thread's columns: w_post times a per-channel gate (1 where neither is
+// given) and w_pre (0 without).
+template <int VEC, int V>
+__device__ __forceinline__ void load_y_factors(const stageml_norm_args& a, int tid, int nt, int H, float (&f)[V][VEC]) {
+  if (a.post_weight) {
+    load_columns<VEC, V>(a.post_weight, a.post_dtype, 0, tid, nt, H, f);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[v][i] = 1.f;
+  }
+  if (a.gate_mode == STAGEML_GATE_CHANNEL) {
+    float g[V][VEC];
+    load_columns<VEC, V>(a.gate, a.gate_dtype, 0, tid, nt, H, g);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[v][i] *= g[v][i];
+  }
+}
+template <int VEC, int V>
+__device__ __forceinline__ void load_z_factors(const stageml_norm_args& a, int tid, int nt, int H, float (&f)[V][VEC]) {
+  if (a.pre_weight) {
+    load_columns<VEC, V>(a.pre_weight, a.pre_dtype, 0, tid, nt, H, f);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[v][i] = 0.f;
+  }
 }
 
 template <int VEC>
@@ -225,16 +291,24 @@ struct Factors {
     z_at = y_at + (has_y ? 4 * a.H : 0);
     if (!STAGED) return;
     float* z_factor = smem + (has_y ? a.H : 0);
-    for (int i = threadIdx.x; i < a.H; i += blockDim.x) {
-      if (has_y) smem[place<VEC>(i, a.H)] = from_params(i);
-      if (a.pre_weight) z_factor[place<VEC>(i, a.H)] = load_param1(a.pre_weight, a.pre_dtype, i);
+    constexpr int V = 8 / VEC;  // 8 values per thread and turn
+    for (int at = 0; at < a.H; at += 8 * blockDim.x) {
+      const int tid = at / VEC + threadIdx.x;
+      float fy[V][VEC], fz[V][VEC];
+      if (has_y) load_y_factors<VEC, V>(a, tid, blockDim.x, a.H, fy);
+      if (a.pre_weight) load_z_factors<VEC, V>(a, tid, blockDim.x, a.H, fz);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = (v * blockDim.x + tid) * VEC;
+        if (c >= a.H) continue;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (has_y) smem[place<VEC>(c + i, a.H)] = fy[v][i];
+          if (a.pre_weight) z_factor[place<VEC>(c + i, a.H)] = fz[v][i];
+        }
+      }
     }
     __syncthreads();
-  }
-  __device__ __forceinline__ float from_params(int c) const {
-    float f = a.post_weight ? load_param1(a.post_weight, a.post_dtype, c) : 1.f;
-    if (a.gate_mode == STAGEML_GATE_CHANNEL) f *= load_param1(a.gate, a.gate_dtype, c);
-    return f;
   }
   template <int VEC>
   __device__ __forceinline__ void read(uint32_t at, int c, float (&f)[VEC]) const {
@@ -352,18 +426,10 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
     if (threadIdx.x == 0)
       for (int i = 0; i < STAGES; ++i) fill(i);
   }
-  const Factors<false> factors{a, 0, 0, false};
   float fy[V][VEC], fz[V][VEC];
   if constexpr (HELD) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = (v * nt + tid) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) fy[v][i] = fz[v][i] = 0.f;
-      if (c >= H) continue;
-      factors.template y<VEC>(c, fy[v]);
-      if (a.pre_weight) factors.template z<VEC>(c, fz[v]);
-    }
+    load_y_factors<VEC, V>(a, tid, nt, H, fy);
+    load_z_factors<VEC, V>(a, tid, nt, H, fz);
   }
   uint32_t count = 0;
   for (int64_t row = first; row < a.T; row += step, ++count) {
@@ -386,10 +452,22 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       if constexpr (EAGER)
         if (c < H) r_in[v].template load<false>(r_row, c);
     }
+    if constexpr (!HELD) {
+      load_y_factors<VEC, V>(a, tid, nt, H, fy);
+      if constexpr (EAGER) load_z_factors<VEC, V>(a, tid, nt, H, fz);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sq = fmaf(n[v][i], n[v][i], sq);
+    if (a.block_out && a.gate_mode == STAGEML_GATE_FULL) {
+      float g[V][VEC];
+      load_columns<VEC, V>(a.gate, a.gate_dtype, base, tid, nt, H, g);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) n[v][i] *= g[v][i];
+    }
     float scale = a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
     if (a.post_weight) scale *= rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
     sq = 0.f;
@@ -398,15 +476,8 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       const int c = (v * nt + tid) * VEC;
       if (c >= H) continue;
       if (a.block_out) {
-        if constexpr (!HELD) factors.template y<VEC>(c, fy[v]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) n[v][i] *= fy[v][i];
-        if (a.gate_mode == STAGEML_GATE_FULL) {
-          float g[VEC];
-          load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) n[v][i] *= g[i];
-        }
       }
       float r[VEC];
       if constexpr (EAGER)
@@ -429,14 +500,10 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
     if constexpr (RING)
       if (threadIdx.x == 0) fill(count + STAGES);
     if (!a.pre_weight) continue;
+    if constexpr (!HELD && !EAGER) load_z_factors<VEC, V>(a, tid, nt, H, fz);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
-      if constexpr (!HELD) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) fz[v][i] = 0.f;
-        if (c < H) factors.template z<VEC>(c, fz[v]);
-      }
       float w[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) w[i] = n[v][i] * inv * fz[v][i];
@@ -530,7 +597,7 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
     Held<VEC, TR> r_in[EAGER ? V : 1], dr_in[EAGER ? V : 1];
     float n[V][VEC], d[V][VEC];
     // With f the channel's factor and g a gate that is not part of it: n = a r + f g y inv_y.
-    const bool full = a.gate_mode == STAGEML_GATE_FULL;
+    const bool full = has_y && a.gate_mode == STAGEML_GATE_FULL;
     const float token_gate = a.gate_mode == STAGEML_GATE_TOKEN ? load_param1(a.gate, a.gate_dtype, row) : 1.f;
     float inv_y = 1.f;
     float sq = 0.f;
@@ -555,14 +622,20 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sq = fmaf(y[i], y[i], sq);
     }
+    if (full) {
+      load_columns<VEC, V>(a.gate, a.gate_dtype, base, tid, nt, H, n);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) n[v][i] = has_y ? 1.f : 0.f;
+    }
     if (post) inv_y = rsqrtf(row_sum<WARP>(sq, red, phase) * inv_h + a.eps);
     const float y_scale = inv_y * token_gate;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) n[v][i] = 0.f;
       if constexpr (!EAGER) dz_in[v].zero();
       if (c >= H) continue;
       if (has_y) {
@@ -570,12 +643,7 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
         factors.template y<VEC>(c, f);
         y_in[v].floats(y);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) n[v][i] = y[i] * f[i];
-        if (full) {
-          load_param<VEC>(a.gate, a.gate_dtype, base + c, f);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) n[v][i] *= f[i];
-        }
+        for (int i = 0; i < VEC; ++i) n[v][i] *= y[i] * f[i];
       }
       float r[VEC];
       if constexpr (EAGER)
@@ -605,6 +673,9 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
     // d, dr and the column sums; then d becomes p = f g d inv_y, the part of dy that needs no
     // further row sum: dy = p - y inv_y^2 mean(p y)
     float s3 = 0.f;
+    float gates[VEC == 1 ? V : 1][VEC];
+    if constexpr (VEC == 1)
+      if (full) load_columns<VEC, V>(a.gate, a.gate_dtype, base, tid, nt, H, gates);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * nt + tid) * VEC;
@@ -641,7 +712,10 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
       y_in[v].floats(y);
       if (full) {
         float g[VEC];
-        load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
+        if constexpr (VEC == 1)
+          g[0] = gates[v][0];
+        else
+          load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float e = d[v][i] * inv_y, p = e * f[i];
@@ -685,9 +759,31 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
     }
   }
   if (n_sums_of(a) == 0) return;
-  // one row of sums per CTA, or per warp of a CTA of warp rows
-  const int64_t owner = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  float* out = partial + owner * n_sums_of(a) * H;
+  float* out = partial + (int64_t)blockIdx.x * n_sums_of(a) * H;
+  if constexpr (WARP) {
+    // the warps' sums are added first: an owner per warp left the second kernel thousands of rows
+    __shared__ float warps[kWarpRows][kWarpWidth];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      if (which == 0 ? !has_block_sum(a) : !a.pre_weight) continue;
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = (v * nt + tid) * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (c < H) warps[threadIdx.x >> 5][c + i] = which == 0 ? sum_y[v][i] : sum_z[v][i];
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < H; c += blockDim.x) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarpRows; ++w) s += warps[w][c];
+        out[(which == 1 && has_block_sum(a) ? H : 0) + c] = s;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (v * nt + tid) * VEC;
@@ -742,7 +838,7 @@ bool vectors(const stageml_norm_args& a) {
 
 // Threads for `units` loads per row, `per` of them per thread.
 Shape shape_of(int units, int per, bool warp) {
-  if (warp) return {256, 8};
+  if (warp) return {32 * kWarpRows, kWarpRows};
   return {std::min(kMaxThreads, ((units + per - 1) / per + 31) / 32 * 32), 1};
 }
 
@@ -759,7 +855,8 @@ int resident_ctas(std::atomic<uint64_t>& last, K kernel, int threads, size_t sme
   if ((known & ~uint64_t(0xff)) == key) {
     per_sm = (int)(known & 0xff);
   } else {
-    SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem));
+    if (smem > 40 * 1024)  // 48 KB with the static part need no leave
+      SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem));
     SB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
     per_sm = std::max(per_sm, 1);
     last.store(key | (uint64_t)per_sm, std::memory_order_relaxed);
@@ -768,11 +865,8 @@ int resident_ctas(std::atomic<uint64_t>& last, K kernel, int threads, size_t sme
   return STAGEML_OK;
 }
 
-// The most owners of column sums (workspace): 2048 threads per SM.
-int max_owners(const stageml_norm_args& a) {
-  const int rows_per_sm = a.H <= 256 ? 64 : 32;  // warps of warp rows; CTAs of at least 64 threads
-  return (int)std::min<int64_t>(a.T + 7, (int64_t)sm_count() * rows_per_sm);
-}
+// The most owners of column sums (workspace): CTAs of at least 64 threads, 2048 threads per SM.
+int max_owners(const stageml_norm_args& a) { return (int)std::min<int64_t>(a.T, (int64_t)sm_count() * 32); }
 
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStream_t stream) {
@@ -798,13 +892,15 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
     smem = (RING ? (size_t)kBackwardStages * a.H * 2 * (sizeof(TR) + sizeof(TY)) : 0) + factor_bytes(a);
   static std::atomic<uint64_t> resident{0};
   int grid = 0;
-  SB_TRY(resident_ctas(resident, kernel, s.threads, smem, (a.T + s.rows_per_cta - 1) / s.rows_per_cta, &grid));
+  // a warp takes four rows or more, for fewer rows of sums
+  const int64_t ctas = WARP ? (a.T + 4 * kWarpRows - 1) / (4 * kWarpRows) : a.T;
+  SB_TRY(resident_ctas(resident, kernel, s.threads, smem, ctas, &grid));
   SB_CUDA_CHECK(launch_kernel(kernel, dim3((unsigned)grid), dim3(s.threads), smem, stream, false, a, partial));
   count_launch();
   if (n_sums) {
     const int64_t width = (int64_t)n_sums * a.H;
     SB_CUDA_CHECK(launch_kernel(norm_weight_sums_kernel, dim3((unsigned)((width + 31) / 32)), dim3(32 * kStrands), 0,
-                                stream, true, a, (const float*)partial, grid * s.rows_per_cta, n_sums));
+                                stream, true, a, (const float*)partial, grid, n_sums));
     count_launch();
   }
   return STAGEML_OK;
@@ -816,11 +912,12 @@ int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStre
   (backward ? run_backward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, stream) \
             : run_forward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, stream))
   // Few rows run straight from global memory with as many threads per row as possible; more
-  // than two rows per SM are worth a CTA's staged factors.
+  // than two rows per SM are worth a CTA's staged factors, and so is one row of the scalar backward,
+  // which reads them three times.
   const bool many = a.T > 2 * (int64_t)sm_count();
   if (vectors(a)) {
     const int units = a.H / 8;
-    if (units <= 32) return SB_NORM(8, 1, true, false, false, units);
+    if (a.H <= kWarpWidth) return SB_NORM(8, 1, true, false, false, units);
     const size_t row = a.H * (sizeof(TR) + sizeof(TY));
     const size_t ring = backward ? 2 * kBackwardStages * row + factor_bytes(a) : kForwardStages * row;
     if (!many || ring > kMaxSmem) {
@@ -832,12 +929,14 @@ int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStre
     if (units <= 2 * kMaxThreads) return SB_NORM(8, 2, false, true, true, units);
     return SB_NORM(8, 4, false, true, true, units);
   }
-  if (a.H <= 256) return SB_NORM(1, 8, true, false, false, a.H);
-  if (a.H <= 4 * kMaxThreads)
-    return many ? SB_NORM(1, 4, false, false, true, a.H) : SB_NORM(1, 4, false, false, false, a.H);
-  if (a.H <= 8 * kMaxThreads)
-    return many ? SB_NORM(1, 8, false, false, true, a.H) : SB_NORM(1, 8, false, false, false, a.H);
-  return many ? SB_NORM(1, 32, false, false, true, a.H) : SB_NORM(1, 32, false, false, false, a.H);
+  if (a.H <= kWarpWidth) return SB_NORM(1, 8, true, false, false, a.H);
+#define SB_NORM_SCALAR(V) \
+  (many || backward ? SB_NORM(1, V, false, false, true, a.H) \
+                    : run_forward<TR, TY, 1, V, false, false, false>(a, shape_of(a.H, V, false), scratch, stream))
+  if (a.H <= 4 * kMaxThreads) return SB_NORM_SCALAR(4);
+  if (a.H <= 8 * kMaxThreads) return SB_NORM_SCALAR(8);
+  return SB_NORM_SCALAR(32);
+#undef SB_NORM_SCALAR
 #undef SB_NORM
 }
 
