@@ -49,12 +49,12 @@ struct BlockGemmLaunch {
   int32_t* status = nullptr;
   bool pdl = false;
 };
-// block_skinny.cu: the same product for at most kSkinnyRows rows per weight group, streaming the
-// weights. swiglu: writes silu(gate) * up in fp32 to g.out. Grouped rows need the plan's tiles (a
-// group's rows all lie in one tile); row_map (optional) names the row of `a` of each plan row.
+// block_skinny.cu: the same product for few rows per weight group, streaming the weights once per 8 or
+// 16 rows. swiglu: writes silu(gate) * up in fp32 to g.out. Grouped rows need the plan's tiles and
+// offsets; row_map (optional) names the row of `a` of each plan row.
 constexpr int kSkinnyRows = 16;
 struct BlockSkinny {
-  int max_rows = 0;                       // at most kSkinnyRows; plain rows: their number
+  int max_rows = 0;  // plain rows: their number, at most kSkinnyRows; grouped: up to 8 or more per group expected
   const int32_t* row_map = nullptr;
   const int32_t* tile_group = nullptr;
   const int32_t* group_counts = nullptr;

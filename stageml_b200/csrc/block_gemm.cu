@@ -65,7 +65,7 @@ constexpr int kBandUnits = 8;            // plain rows: row units that share a p
 constexpr int BAR_BYTES = 512;
 constexpr int TURN_PITCH = 17;           // floats per row of a math warp's 32 x 16 turning area
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + BAR_BYTES + 2 * 2 * BM * 4 /*row maxima*/ +
-                           SLOTS * SLOT_FLOATS * 4 + 2 * HALF_WARPS * 32 * TURN_PITCH * 4 + (MAX_GROUPS + 1) * 4;
+                           SLOTS * SLOT_FLOATS * 4 + 2 * HALF_WARPS * 32 * TURN_PITCH * 4 + 2 * (MAX_GROUPS + 1) * 4;
 static_assert(BUFS == 4, "two halves, two K blocks in flight");
 static_assert(SMEM_BYTES <= 232448, "shared memory per block");
 static_assert((2 * STAGES + 2 * BUFS + 2 + 2 * SLOTS) * 8 + 16 <= BAR_BYTES, "barrier area");
@@ -178,15 +178,17 @@ struct Unit {
   int tiles;        // row tiles of the unit
 };
 
-// first[g] = row units of the groups before g (grouped rows), in shared memory; returns the
-// number of row units. One warp.
-__device__ __forceinline__ void group_units(const Params& p, int step, int32_t* first) {
+// first[g] = row units of the groups before g, begin[g] = their row tiles (grouped rows), in shared
+// memory: read from global memory for each unit, they were 0.7 us of every role's unit. One warp.
+__device__ __forceinline__ void group_units(const Params& p, int step, int32_t* first, int32_t* begin) {
   const int lane = threadIdx.x & 31;
+  for (int g = lane; g <= p.groups; g += 32) begin[g] = p.group_offsets[g] / BM;
+  __syncwarp();
   int base = 0;
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
     const int g = g0 + lane;
     int c = 0;
-    if (g < p.groups) c = ((p.group_offsets[g + 1] - p.group_offsets[g]) / BM + step - 1) / step;
+    if (g < p.groups) c = (begin[g + 1] - begin[g] + step - 1) / step;
     int s = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -202,7 +204,7 @@ __device__ __forceinline__ void group_units(const Params& p, int step, int32_t* 
 // Unit u -> row tiles and column tile. All column tiles of a weight group's row units (or of
 // a band of plain row units) come before the next group, row units fastest, so that the
 // CTAs at work at one time share weight tiles and the group's rows stay in L2.
-__device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const int32_t* first) {
+__device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const int32_t* first, const int32_t* begins) {
   Unit w;
   if (p.group_offsets) {
     const int r = u / p.n_tiles;
@@ -214,7 +216,7 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const 
       else
         hi = mid - 1;
     }
-    const int begin = p.group_offsets[lo] / BM, tiles = p.group_offsets[lo + 1] / BM - begin;
+    const int begin = begins[lo], tiles = begins[lo + 1] - begin;
     const int cnt = first[lo + 1] - first[lo], local = u - first[lo] * p.n_tiles;
     w.group = lo;
     w.n = local / cnt;
@@ -376,6 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   float* scales = reinterpret_cast<float*>(row_max + 2 * 2 * BM);                                 // [SLOTS][SLOT_FLOATS]
   float* turns = scales + SLOTS * SLOT_FLOATS;                                                    // [math warps][32][17]
   int32_t* first = reinterpret_cast<int32_t*>(turns + 2 * HALF_WARPS * 32 * TURN_PITCH);          // [groups + 1]
+  int32_t* begins = first + MAX_GROUPS + 1;                                                       // [groups + 1]
   auto full_bar = [&](int s) { return smem_u32(&bars[s]); };                // both CTAs' copies (even CTA)
   auto empty_bar = [&](int s) { return smem_u32(&bars[STAGES + s]); };
   auto tfull_bar = [&](int i) { return smem_u32(&bars[2 * STAGES + i]); };
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish_pair();
   }
-  if (warp == 2 && p.group_offsets) group_units(p, 2, first);
+  if (warp == 2 && p.group_offsets) group_units(p, 2, first, begins);
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t it = 0, grp = 0, tile = 0;
     bool ok = true, joined = false;
     for (int u = cluster; ok && u < units; u += clusters, ++tile) {
-      const Unit w = unit_of(p, u, 2, first);
+      const Unit w = unit_of(p, u, 2, first, begins);
       const int64_t row = (int64_t)(w.m + rank) * BM + row_in_tile;
       const bool row_ok = rank < w.tiles && row < p.rows;
       // The up rows start at N inside the group, so a tile's up columns can straddle two 128-row
@@ -597,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t s = 0, phase = 0, filled = 0;  // filled: bit i = stage i has been filled
       bool ok = true;
       for (int u = cluster; ok && u < units; u += clusters) {
-        const Unit w = unit_of(p, u, 2, first);
+        const Unit w = unit_of(p, u, 2, first, begins);
         const int n0 = w.n * (SWIGLU ? 128 : BN);
         // B rows of half 0; half 1 is `next` rows on
         const int b0 = w.group * p.b_group_rows + n0 + rank * (SWIGLU ? p.N : 64);
@@ -669,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t grp = 0;
     bool ok = true;
     for (int u = cluster; ok && u < units; u += clusters) {
-      const Unit w = unit_of(p, u, 2, first);
+      const Unit w = unit_of(p, u, 2, first, begins);
       const int64_t row0 = (int64_t)(w.m + rank) * BM + lane;
       const int valid = rank < w.tiles ? (int)min((int64_t)BM, p.rows - row0) : 0;  // row 32 i + lane: 32 i < valid
       const float* sa = p.a_scale + (valid > 0 ? row0 : 0) * p.kb;

@@ -1,5 +1,5 @@
-// The block-scaled e4m3 product for a few rows (at most 16 per weight group): one token of
-// a decode step, or the expert rows of a small batch. It streams the weights once:
+// The block-scaled e4m3 product for a few rows: one token of a decode step, or the expert rows of
+// a small batch. It streams the weights, once per 8 or 16 rows of a weight group:
 //
 //   out[m, n] = row_scale[m] * sum_kb sx[m, kb] * sw[n / 128, kb] * (sum_{k in kb} x[m, k] w[n, k])
 //
@@ -11,7 +11,10 @@
 // for both operands, so nothing is shuffled. Rows are the N side (8 or 16 of them). The
 // matrix unit is far from its limit here; tcgen05 would only add its set-up time: the same
 // 1 x 4096 x 4096 product took 18 us on the pair kernel, bound by one accumulator round trip
-// per K block.
+// per K block, and takes 5 here. Measured over 64 experts of 2048 x 1408 with six per token: 8, 16
+// and 32 tokens in 114, 163 and 197 us, weights at 3.5 to 4 TB/s. Loading the next unit's weights
+// before the sums of this one meet was no faster (111, 159 and 191 us) and slowed long
+// rows down (8 experts of 4096 x 14336, 8 tokens: 319 us, not 293).
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -32,8 +35,9 @@ struct SkinnyParams {
   int w_group_rows, w_blocks;
   int units_n;                // column units per group
   int rows;                   // plain rows; grouped: from the counts
-  const int32_t* tile_group;  // grouped: 128-row tile -> group, each group with rows has one tile
+  const int32_t* tile_group;  // grouped: 128-row tile -> group
   const int32_t* group_counts;
+  const int32_t* group_offsets;  // first row of each group
   const int32_t* num_tiles;
   int tiles_cap;
   const float* row_scale;
@@ -80,8 +84,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) block_skinny_kernel(const Skin
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int tile = u / p.units_n, n0 = (u - tile * p.units_n) * kUnitRows;
     const int group = p.tile_group ? p.tile_group[tile] : 0;
-    const int all_rows = p.tile_group ? p.group_counts[group] : p.rows;
-    // one round but for ids that name an expert several times per token
+    const int all_rows =
+        p.tile_group ? min(128, p.group_counts[group] - (tile * 128 - p.group_offsets[group])) : p.rows;
     for (int first = 0; first < all_rows; first += NT * 8) {
     const int rows = min(all_rows - first, NT * 8);
     const int64_t row0 = (int64_t)tile * 128 + first;
@@ -217,6 +221,7 @@ int launch_block_skinny(const BlockGemmLaunch& g, const BlockSkinny& s, cudaStre
   p.rows = s.max_rows;
   p.tile_group = s.tile_group;
   p.group_counts = s.group_counts;
+  p.group_offsets = g.group_offsets;
   p.num_tiles = s.num_tiles;
   p.tiles_cap = s.tiles_cap;
   p.row_scale = g.row_scale;

@@ -291,6 +291,20 @@ def test_moe_forward_blocks_routing_edges(ops, t):
     assert none.shape == (0, h)
 
 
+@pytest.mark.parametrize("t,e,k,shared", [(17, 64, 4, 1), (100, 128, 4, 0), (128, 64, 2, 2), (43, 64, 6, 0)])
+@pytest.mark.parametrize("skew", [False, True])
+def test_moe_forward_blocks_few_rows_per_expert(ops, t, e, k, shared, skew):
+    """More than 16 tokens, few per expert on average; skewed, all slots name one expert (several row tiles)."""
+    h, i = 144, 80
+    gu, gus, dn, dns = layer_weights(e + shared, h, i, seed=5)
+    x = randn(t, h, seed=6, dtype=BF16)
+    ids = torch.full((t, k), e - 3, device=DEV, dtype=torch.int32) if skew else \
+        randn(t, e, seed=7).topk(k, 1).indices.to(torch.int32)
+    w = torch.rand(t, k, generator=torch.Generator(device=DEV).manual_seed(8), device=DEV)
+    y = ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w, n_shared=shared)
+    close(y, ref_layer(x, gu, gus, dn, dns, ids, w, shared), LAYER_TOL[BF16])
+
+
 @pytest.mark.parametrize("t", [3, 150])
 def test_moe_forward_blocks_bad_ids_are_dropped_and_reported(ops, t):
     e, h, i = 4, 128, 128
