@@ -282,6 +282,7 @@ __device__ __forceinline__ void store_columns(const Params& p, float* v, float f
     OutT* out = static_cast<OutT*>(p.out) + (row - mine) * p.N + n0 + PIECE * mine;
 #pragma unroll
     for (int c = 0; c < W; c += 4 * PIECE) {
+      if (n0 + c >= p.N) break;
       uint4 u[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] = pack16<OutT>(v + c + PIECE * i);
@@ -297,6 +298,7 @@ __device__ __forceinline__ void store_columns(const Params& p, float* v, float f
     const int64_t row0 = row - lane;
 #pragma unroll
     for (int c = 0; c < W; c += 16) {
+      if (n0 + c >= p.N) break;
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 16; ++i) turn[lane * TURN_PITCH + i] = v[c + i];
