@@ -376,12 +376,9 @@ int stageml_quantize_e4m3_blocks(const void* x, int dtype, int64_t batch, int64_
 
 /* out[m, n] = sum_kb x_scale[m, kb] * w_scale[n / 128, kb] * sum_{k in block kb} x[m, k] * w[n, k]
  * x [M, K] e4m3, x_scale [M, ceil(K/128)]; w [N, K] e4m3, w_scale [ceil(N/128), ceil(K/128)];
- * out [M, N] F32/BF16/F16, fp32 sums rounded once. K a multiple of 16 (16-byte rows), any M, N.
- * The workspace holds the partial sums of calls with few rows, whose K is split over CTAs. */
-size_t stageml_block_matmul_workspace_bytes(int M, int N, int K);
+ * out [M, N] F32/BF16/F16, fp32 sums rounded once. K a multiple of 16 (16-byte rows), any M, N. */
 int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int M, int N,
-                         int K, int out_dtype, void* out, int32_t* status, void* workspace, size_t workspace_bytes,
-                         stageml_stream_t stream);
+                         int K, int out_dtype, void* out, int32_t* status, stageml_stream_t stream);
 
 /* The routed SwiGLU feed-forward layer on block-scaled weights (the computation of
  * stageml_moe_forward without LoRA, with both products on e4m3 operands):

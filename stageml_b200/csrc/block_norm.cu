@@ -33,7 +33,12 @@
 //   dg = w_post S,
 // so at most two sums per column (S and dw_pre's) are kept, in the registers of the thread
 // that owns the column. Each CTA takes every gridDim-th row and writes its sums once; a second
-// kernel adds them in CTA order: no atomics, the same bits on every run. Bound: HBM.
+// kernel adds them in CTA order: no atomics, the same bits on every run.
+//
+// Bound: HBM for the forward (8192 x 4096 bf16 in 45 us, 268 MB: 6.0 TB/s); the backward (112 us,
+// 336 MB, 3.0 TB/s) by the issue slots, 70 % of which its arithmetic takes: two norms recomputed and
+// two differentiated per element. Widths that are not multiples of 8 take scalar loads (777 x 2047,
+// fp32 stream: forward 8, backward 17 us) and beyond 4096 columns more registers than there are.
 #include <atomic>
 
 #include "block_codes.cuh"
@@ -460,7 +465,9 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sq = fmaf(n[v][i], n[v][i], sq);
-    if (a.block_out && a.gate_mode == STAGEML_GATE_FULL) {
+    // with held factors the full gate's few vectors are loaded one by one below: together they take the
+    // registers of a third CTA per SM (8192 x 4096 in 51 us, not 45)
+    if (!(HELD && VEC == 8) && a.block_out && a.gate_mode == STAGEML_GATE_FULL) {
       float g[V][VEC];
       load_columns<VEC, V>(a.gate, a.gate_dtype, base, tid, nt, H, g);
 #pragma unroll
@@ -478,6 +485,12 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       if (a.block_out) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) n[v][i] *= fy[v][i];
+        if (HELD && VEC == 8 && a.gate_mode == STAGEML_GATE_FULL) {
+          float g[VEC];
+          load_param<VEC>(a.gate, a.gate_dtype, base + c, g);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) n[v][i] *= g[i];
+        }
       }
       float r[VEC];
       if constexpr (EAGER)
@@ -804,8 +817,13 @@ __global__ void __launch_bounds__(32 * kStrands)
   const int64_t width = (int64_t)n_sums * a.H, i = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
   if (i < width) {
-#pragma unroll 8
-    for (int c = strand; c < owners; c += kStrands) s += __ldg(partial + c * width + i);
+    for (int at = strand; at < owners; at += 8 * kStrands) {  // eight loads at a time, the last turn's too
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = at + j * kStrands;
+        s += c < owners ? __ldg(partial + c * width + i) : 0.f;
+      }
+    }
   }
   part[strand][lane] = s;
   __syncthreads();

@@ -476,12 +476,9 @@ Tensor block_matmul(const Tensor& x, const Tensor& x_scale, const Tensor& w, con
   c10::cuda::CUDAGuard guard(x.device());
   auto out = fresh({M, N}, out_dtype, x);
   check_float_dtype(out, "block_matmul: out_dtype");
-  const size_t bytes = stageml_block_matmul_workspace_bytes((int)M, (int)N, (int)K);
-  Tensor ws = bytes ? workspace(bytes, x) : Tensor();
   check_rc(stageml_block_matmul(static_cast<const uint8_t*>(x.data_ptr()), x_scale.data_ptr<float>(),
                                 static_cast<const uint8_t*>(w.data_ptr()), w_scale.data_ptr<float>(), (int)M, (int)N,
-                                (int)K, dtype_code(out), out.data_ptr(), status_word(x), bytes ? ws.data_ptr() : nullptr,
-                                bytes, cur_stream()),
+                                (int)K, dtype_code(out), out.data_ptr(), status_word(x), cur_stream()),
            "block_matmul");
   return out;
 }

@@ -15,11 +15,11 @@ P = 4096  # a non-null, 16-byte aligned address; never dereferenced
     (lambda L: L.stageml_quantize_e4m3_blocks(P, capi.I32, 1, 4, 128, 0, P, P, None), "F32, BF16 or F16"),
     (lambda L: L.stageml_quantize_e4m3_blocks(P, capi.F32, 1, -4, 128, 0, P, P, None), "negative"),
     (lambda L: L.stageml_quantize_e4m3_blocks(None, capi.F32, 1, 4, 128, 0, P, P, None), "null"),
-    (lambda L: L.stageml_block_matmul(P, P, P, P, 4, 4, 24, capi.BF16, P, None, None, 0, None), "multiple of 16"),
-    (lambda L: L.stageml_block_matmul(P, P, P, P, 4, 4, 32, capi.E4M3, P, None, None, 0, None), "out_dtype"),
-    (lambda L: L.stageml_block_matmul(P, None, P, P, 4, 4, 32, capi.BF16, P, None, None, 0, None), "null"),
-    (lambda L: L.stageml_block_matmul(P + 8, P, P, P, 4, 4, 32, capi.BF16, P, None, None, 0, None), "aligned"),
-    (lambda L: L.stageml_block_matmul(P, P, P, P, -1, 4, 32, capi.BF16, P, None, None, 0, None), "bad sizes"),
+    (lambda L: L.stageml_block_matmul(P, P, P, P, 4, 4, 24, capi.BF16, P, None, None), "multiple of 16"),
+    (lambda L: L.stageml_block_matmul(P, P, P, P, 4, 4, 32, capi.E4M3, P, None, None), "out_dtype"),
+    (lambda L: L.stageml_block_matmul(P, None, P, P, 4, 4, 32, capi.BF16, P, None, None), "null"),
+    (lambda L: L.stageml_block_matmul(P + 8, P, P, P, 4, 4, 32, capi.BF16, P, None, None), "aligned"),
+    (lambda L: L.stageml_block_matmul(P, P, P, P, -1, 4, 32, capi.BF16, P, None, None), "bad sizes"),
     (lambda L: L.stageml_balance_loss(P, capi.F32, P, capi.I32, None, 4, 300, 2, 1.0, P, P, P, None, None, 0, None), "256"),
     (lambda L: L.stageml_balance_loss(P, capi.F32, P, capi.I32, None, 4, 8, 9, 1.0, P, P, P, None, None, 0, None), "1..8"),
     (lambda L: L.stageml_balance_loss(P, capi.F32, P, capi.F32, None, 4, 8, 2, 1.0, P, P, P, None, None, 0, None), "int32"),
@@ -35,7 +35,7 @@ def test_bad_calls_are_refused(call, text):
 def test_nothing_to_do_is_ok():
     lib = load_capi()
     assert lib.stageml_quantize_e4m3_blocks(None, capi.F32, 1, 0, 128, 0, None, None, None) == capi.OK
-    assert lib.stageml_block_matmul(None, None, None, None, 0, 64, 128, capi.BF16, None, None, None, 0, None) == capi.OK
+    assert lib.stageml_block_matmul(None, None, None, None, 0, 64, 128, capi.BF16, None, None, None) == capi.OK
     assert lib.stageml_balance_loss_backward(None, None, capi.F32, None, None, None, 0, 8, 2, 1.0, None, None) == capi.OK
 
 
