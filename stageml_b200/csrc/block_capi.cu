@@ -30,10 +30,10 @@ struct MoeBlocksBuffers {
 bool moe_blocks_sparse(const stageml_moe_blocks_args* a) { return (int64_t)a->T * a->k <= 4 * (int64_t)a->E; }
 
 // Streaming products instead of tensor-core tiles. 64 experts of 2048 x 1408, six per token, two
-// shared: 17 tokens in 170 us (tiles: 223), 32 in 197 (243), 42 in 210 (tiles at 43: 243). The tiles
-// take the same time for any number of rows up to 128 per expert, the streams once more per 8 rows.
+// shared: 17 tokens in 170 us, 32 in 197, 42 in 210. The tiles take the same time for any number of
+// rows up to 128 per expert (43 to 128 tokens in 194 to 199 us), the streams once more per 8 rows.
 bool moe_blocks_skinny(const stageml_moe_blocks_args* a) {
-  return a->T <= kSkinnyRows || (a->T <= 128 && moe_blocks_sparse(a));
+  return a->T <= kSkinnyRows || (a->T <= 128 && (int64_t)a->T * a->k <= 2 * (int64_t)a->E);
 }
 
 void moe_blocks_carve(const stageml_moe_blocks_args* a, void* ws, MoeBlocksBuffers* b) {

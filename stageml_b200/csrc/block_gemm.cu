@@ -20,6 +20,11 @@
 // issue slots per K block, 256 of them the additions, and every warp pays its own waits.
 // The control warps give registers to the math warps. Persistent clusters.
 //
+// A unit of one row tile (a short batch, the odd last tile of an expert) is narrow: 64 rows per CTA,
+// MMAs of M = 128, whose accumulators hold columns [0, 64) of a half in lanes 0..63 and [64, 128) in
+// lanes 64..127: 64 sums per thread, half the work of a pair with an idle CTA. 64 experts of 2048 x
+// 1408 with at most 128 rows each in 197 us, from 250; 64 x 4096 x 4096 in 12 us, from 15.
+//
 // SwiGLU: half h of a tile is 64 gate rows and the matching 64 up rows of B, so a thread
 // holds the gate and up values of the same columns; the epilogue forms
 // h = silu(gate) * up in fp32 and writes it as e4m3 codes with one scale per (row, 128
@@ -282,10 +287,15 @@ __device__ __forceinline__ void store_columns(const Params& p, float* v, float f
 #pragma unroll
   for (int i = 0; i < W; ++i) v[i] *= factor;
   const int mine = threadIdx.x & 3;
-  if (p.N % PIECE == 0) {
+  if (W < 4 * PIECE && p.N % PIECE == 0) {
+    OutT* out = static_cast<OutT*>(p.out) + row * p.N + n0;
+#pragma unroll
+    for (int c = 0; c < W; c += PIECE)
+      if (rows4 > mine && n0 + c < p.N) *reinterpret_cast<uint4*>(out + c) = pack16<OutT>(v + c);
+  } else if (p.N % PIECE == 0) {
     OutT* out = static_cast<OutT*>(p.out) + (row - mine) * p.N + n0 + PIECE * mine;
 #pragma unroll
-    for (int c = 0; c < W; c += 4 * PIECE) {
+    for (int c = 0; c + 4 * PIECE <= W; c += 4 * PIECE) {
       if (n0 + c >= p.N) break;
       uint4 u[4];
 #pragma unroll
@@ -325,10 +335,10 @@ __device__ __forceinline__ void store_columns(const Params& p, float* v, float f
 // any more once every pair has come to the first barrier ([pair][half][4 columns][row] in 16 bytes,
 // so that a warp writes 512 bytes in a row). Its own sums first, then the others' in their order: the same
 // bits every time.
-template <int S>
+template <int S, int COLS>
 __device__ __forceinline__ void join_splits(const float* acc, float* own, uint32_t stage, int rank, int split, int half,
                                             int row) {
-  constexpr int W = 128 / S;
+  constexpr int W = COLS / S;
   static_assert(S * 2 * W * BM * 4 <= STAGES * STAGE_BYTES, "exchange area");
   auto place = [&](int from, int c) { return (uint32_t)((((from * 2 + half) * (W / 4) + c / 4) * BM + row) * 16); };
   __syncwarp();
@@ -367,12 +377,17 @@ __device__ __forceinline__ void join_splits(const float* acc, float* own, uint32
   }
 }
 
+template <int N>
+struct Columns {
+  static constexpr int value = N;
+};
+
 // OutT: output element (plain); SWIGLU writes codes and ignores it. SPLITS pairs of a cluster share a
 // tile's K blocks; a cluster then has one tile.
 template <typename OutT, bool SWIGLU, int SPLITS>
 __global__ void __launch_bounds__(THREADS, 1)
     block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                           const Params p) {
+                           const __grid_constant__ CUtensorMap tm_b32, const Params p) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
@@ -445,105 +460,128 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true, joined = false;
     for (int u = cluster; ok && u < units; u += clusters, ++tile) {
       const Unit w = unit_of(p, u, 2, first, begins);
-      const int64_t row = (int64_t)(w.m + rank) * BM + row_in_tile;
-      const bool row_ok = rank < w.tiles && row < p.rows;
+      // One row tile: 64 rows per CTA, lanes 64..127 the same rows' later columns (`side`).
+      const bool narrow = w.tiles == 1;
+      const int side = narrow ? quarter >> 1 : 0;
       // The up rows start at N inside the group, so a tile's up columns can straddle two 128-row
       // scale blocks: the columns below `cut` take the first, the others the second. N % 16 == 0,
       // so 16 columns share a scale.
-      const int cut = SWIGLU ? 128 - ((p.N + w.n * 128) & 127) - 64 * half : 0;
+      const int cut = SWIGLU ? 128 - ((p.N + w.n * 128) & 127) - 64 * half - 32 * side : 0;
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
       // Runs of 16 and 32 columns in turn: one is read while the other is added. The first run of
       // the next K block is read before the last one of this block is added, so that neither its
       // wait nor its latency lies between two K blocks that are both there.
-      uint32_t t[32], v[16];
-      auto scale_for = [&](int col, float c0, float c1, float c2) { return SWIGLU && col >= 64 ? (col - 64 < cut ? c1 : c2) : c0; };
-      auto add16 = [&](int col, const uint32_t* r, float sc) {
+      auto sum_blocks = [&](auto width) {
+        constexpr int COLS = decltype(width)::value;  // of this thread: 128, or 64 of a narrow unit
+        uint32_t t[32], v[16];
+        auto scale_for = [&](int col, float c0, float c1, float c2) {
+          return SWIGLU && col >= COLS / 2 ? (col - COLS / 2 < cut ? c1 : c2) : c0;
+        };
+        auto add16 = [&](int col, const uint32_t* r, float sc) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[col + i] = fmaf(sc, __uint_as_float(r[i]), acc[col + i]);
+          for (int i = 0; i < 16; ++i) acc[col + i] = fmaf(sc, __uint_as_float(r[i]), acc[col + i]);
+        };
+        if (!warp_wait(tfull_bar((it & 1) * 2 + half), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue)) return false;
+        tc_fence_after();
+        tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
+        for (int kb0 = 0; kb0 < kb_count; kb0 += GROUP) {
+          const uint32_t sl = grp % SLOTS;
+          if (!warp_wait(sfull_bar(sl), (grp / SLOTS) & 1, abort_flag, p.status, kDevTimeoutEpilogue)) return false;
+          const float* slot = scales + sl * SLOT_FLOATS;
+          float s0[GROUP], s1[GROUP], s2[GROUP];
+          {
+            const float4 xa = *reinterpret_cast<const float4*>(slot + row_in_tile * GROUP);
+            const float4* wb = reinterpret_cast<const float4*>(slot + BM * GROUP);
+            const float4 w0 = wb[SWIGLU ? 0 : half];
+            s0[0] = xa.x * w0.x, s0[1] = xa.y * w0.y, s0[2] = xa.z * w0.z, s0[3] = xa.w * w0.w;
+            if (SWIGLU) {
+              const float4 w1 = wb[1], w2 = wb[2];
+              s1[0] = xa.x * w1.x, s1[1] = xa.y * w1.y, s1[2] = xa.z * w1.z, s1[3] = xa.w * w1.w;
+              s2[0] = xa.x * w2.x, s2[1] = xa.y * w2.y, s2[2] = xa.z * w2.z, s2[3] = xa.w * w2.w;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty_bar(sl));
+          ++grp;
+#pragma unroll
+          for (int j = 0; j < GROUP; ++j) {
+            if (kb0 + j >= kb_count) break;
+            const uint32_t buf = (it & 1) * 2 + half;
+            const uint32_t src = t_lane + (it & 1) * 2 * NACC;
+            auto add = [&](int col, const uint32_t* r) {
+              add16(col, r, scale_for(col, s0[j], SWIGLU ? s1[j] : 0.f, SWIGLU ? s2[j] : 0.f));
+            };
+            uint32_t last[16];
+            tmem_wait_ld();
+            tmem_ld_x32(src + 16, t);
+            add(0, v);
+            tmem_wait_ld();
+            if constexpr (COLS == 128) {
+              tmem_ld_x16(src + 48, v);
+              add(16, t), add(32, t + 16);
+              tmem_wait_ld();
+              tmem_ld_x32(src + 64, t);
+              add(48, v);
+              tmem_wait_ld();
+              tmem_ld_x16(src + 96, v);
+              add(64, t), add(80, t + 16);
+              tmem_wait_ld();
+              tmem_ld_x16(src + 112, last);
+              add(96, v);
+            } else {
+              tmem_ld_x16(src + 48, last);
+              add(16, t), add(32, t + 16);
+            }
+            tmem_wait_ld();
+            tc_fence_before();
+            if (lane == 0) arrive_remote(lead_tempty + 8u * buf);
+            ++it;
+            if (kb0 + j + 1 < kb_count) {
+              if (!warp_wait(tfull_bar(buf ^ 2), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue)) return false;
+              tc_fence_after();
+              tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
+            }
+            add(COLS - 16, last);
+          }
+        }
+        return true;
       };
-      ok = warp_wait(tfull_bar((it & 1) * 2 + half), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
+      ok = narrow ? sum_blocks(Columns<64>{}) : sum_blocks(Columns<128>{});
       if (!ok) break;
-      tc_fence_after();
-      tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
-      for (int kb0 = 0; ok && kb0 < kb_count; kb0 += GROUP) {
-        const uint32_t sl = grp % SLOTS;
-        ok = warp_wait(sfull_bar(sl), (grp / SLOTS) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
-        if (!ok) break;
-        const float* slot = scales + sl * SLOT_FLOATS;
-        float s0[GROUP], s1[GROUP], s2[GROUP];
-        {
-          const float4 xa = *reinterpret_cast<const float4*>(slot + row_in_tile * GROUP);
-          const float4* wb = reinterpret_cast<const float4*>(slot + BM * GROUP);
-          const float4 w0 = wb[SWIGLU ? 0 : half];
-          s0[0] = xa.x * w0.x, s0[1] = xa.y * w0.y, s0[2] = xa.z * w0.z, s0[3] = xa.w * w0.w;
-          if (SWIGLU) {
-            const float4 w1 = wb[1], w2 = wb[2];
-            s1[0] = xa.x * w1.x, s1[1] = xa.y * w1.y, s1[2] = xa.z * w1.z, s1[3] = xa.w * w1.w;
-            s2[0] = xa.x * w2.x, s2[1] = xa.y * w2.y, s2[2] = xa.z * w2.z, s2[3] = xa.w * w2.w;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sempty_bar(sl));
-        ++grp;
-#pragma unroll
-        for (int j = 0; j < GROUP; ++j) {
-          if (kb0 + j >= kb_count) break;
-          const uint32_t buf = (it & 1) * 2 + half;
-          const uint32_t src = t_lane + (it & 1) * 2 * NACC;
-          auto add = [&](int col, const uint32_t* r) {
-            add16(col, r, scale_for(col, s0[j], SWIGLU ? s1[j] : 0.f, SWIGLU ? s2[j] : 0.f));
-          };
-          tmem_wait_ld();
-          tmem_ld_x32(src + 16, t);
-          add(0, v);
-          tmem_wait_ld();
-          tmem_ld_x16(src + 48, v);
-          add(16, t), add(32, t + 16);
-          tmem_wait_ld();
-          tmem_ld_x32(src + 64, t);
-          add(48, v);
-          tmem_wait_ld();
-          tmem_ld_x16(src + 96, v);
-          add(64, t), add(80, t + 16);
-          tmem_wait_ld();
-          uint32_t last[16];
-          tmem_ld_x16(src + 112, last);
-          add(96, v);
-          tmem_wait_ld();
-          tc_fence_before();
-          if (lane == 0) arrive_remote(lead_tempty + 8u * buf);
-          ++it;
-          if (kb0 + j + 1 < kb_count) {
-            ok = warp_wait(tfull_bar(buf ^ 2), (it >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
-            if (!ok) break;
-            tc_fence_after();
-            tmem_ld_x16(t_lane + (it & 1) * 2 * NACC, v);
-          }
-          add(112, last);
-        }
-      }
-      if (!ok) break;
+      const int64_t row = narrow ? (int64_t)w.m * BM + 64 * rank + (row_in_tile & 63)
+                                 : (int64_t)(w.m + rank) * BM + row_in_tile;
+      const bool row_ok = row < p.rows;
       const int64_t row4 = row - (lane & 3);  // the first of the four rows that four lanes store together
-      const int rows4 = rank < w.tiles ? (int)max((int64_t)0, min((int64_t)4, p.rows - row4)) : 0;
+      const int rows4 = (int)max((int64_t)0, min((int64_t)4, p.rows - row4));
       if (SWIGLU) {
-        const int n0 = w.n * 128 + 64 * half;
+        // a thread's 64 columns of h from its 64 gate and 64 up sums, or 32 of a narrow unit
+        const int n0 = w.n * 128 + 64 * half + 32 * side;
         uint32_t m = 0;
+        auto activate = [&](auto width) {  // h takes the gate values' place
+          constexpr int COLS = decltype(width)::value / 2;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {  // h takes the gate values' place
-          acc[i] = n0 + i < p.N ? __fdividef(acc[i], 1.f + __expf(-acc[i])) * acc[64 + i] : 0.f;
-          m = max(m, __float_as_uint(acc[i]) & 0x7fffffffu);
-        }
-        // the row's maximum over both halves; two buffers, so that one barrier per tile is enough
-        // (a warp writes a buffer again only after every warp has read it and come to the next tile)
-        uint32_t* mine = row_max + (tile & 1) * 2 * BM + row_in_tile;
-        mine[half * BM] = m;
+          for (int i = 0; i < COLS; ++i) {
+            acc[i] = n0 + i < p.N ? __fdividef(acc[i], 1.f + __expf(-acc[i])) * acc[COLS + i] : 0.f;
+            m = max(m, __float_as_uint(acc[i]) & 0x7fffffffu);
+          }
+        };
+        if (narrow)
+          activate(Columns<64>{});
+        else
+          activate(Columns<128>{});
+        // the row's maximum over its two (narrow: four) threads; two buffers, so that one barrier per
+        // tile is enough (a warp writes a buffer again only after every warp has read it and come to
+        // the next tile)
+        uint32_t* maxima = row_max + (tile & 1) * 2 * BM;
+        maxima[half * BM + row_in_tile] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(max_bar);
         ok = warp_wait(max_bar, tile & 1, abort_flag, p.status, kDevTimeoutEpilogue);
         if (!ok) break;
-        m = max(m, mine[(half ^ 1) * BM]);
+        m = max(m, maxima[(half ^ 1) * BM + row_in_tile]);
+        if (narrow) m = max(m, max(maxima[row_in_tile ^ 64], maxima[BM + (row_in_tile ^ 64)]));
         float s = __uint_as_float(m) / 448.0f;
         s = s == 0.f ? 1.f : s;
         // h never leaves in another form, so its codes may come from the reciprocal: the quotient
@@ -564,28 +602,42 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           codes[c] = make_uint4(v[0], v[1], v[2], v[3]);
         }
-        transpose_pieces(codes);
-        const int n = n0 + 16 * (lane & 3);
-        if (n < p.N) {  // N % 16 == 0: 16 columns are inside or outside
-          uint8_t* q = p.q_out + row4 * p.N + n;
+        if (narrow) {
+          if (row_ok) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r < rows4) *reinterpret_cast<uint4*>(q + (int64_t)r * p.N) = codes[r];
+            for (int c = 0; c < 2; ++c)
+              if (n0 + 16 * c < p.N) *reinterpret_cast<uint4*>(p.q_out + row * p.N + n0 + 16 * c) = codes[c];
+          }
+        } else {
+          transpose_pieces(codes);
+          const int n = n0 + 16 * (lane & 3);
+          if (n < p.N) {  // N % 16 == 0: 16 columns are inside or outside
+            uint8_t* q = p.q_out + row4 * p.N + n;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r < rows4) *reinterpret_cast<uint4*>(q + (int64_t)r * p.N) = codes[r];
+          }
         }
-        if (row_ok && half == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s;
+        if (row_ok && half == 0 && side == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s;
       } else {
-        const int n0 = w.n * BN + 128 * half;
+        const int n0 = w.n * BN + 128 * half + 64 * side;
         float* turn = turns + (warp - MATH_WARP0) * 32 * TURN_PITCH;
         const float rs = row_ok && p.row_scale ? p.row_scale[row] : 1.f;
-        if constexpr (SPLITS == 1) {
-          store_columns<OutT, 128>(p, acc, rs, row, rows4, n0, turn);
-        } else {
-          constexpr int W = 128 / SPLITS;
-          joined = true;
-          float own[W];
-          join_splits<SPLITS>(acc, own, smem_u32(smem), rank, split, half, row_in_tile);
-          store_columns<OutT, W>(p, own, rs, row, rows4, n0 + W * split, turn);
-        }
+        joined = true;
+        auto store = [&](auto width) {
+          constexpr int COLS = decltype(width)::value, W = COLS / SPLITS;
+          if constexpr (SPLITS == 1) {
+            store_columns<OutT, COLS>(p, acc, rs, row, rows4, n0, turn);
+          } else {
+            float own[W];
+            join_splits<SPLITS, COLS>(acc, own, smem_u32(smem), rank, split, half, row_in_tile);
+            store_columns<OutT, W>(p, own, rs, row, rows4, n0 + W * split, turn);
+          }
+        };
+        if (narrow)
+          store(Columns<64>{});
+        else
+          store(Columns<128>{});
       }
     }
     if (SPLITS > 1 && !joined) {  // an expired wait: the other pairs still meet this one
@@ -611,17 +663,25 @@ __global__ void __launch_bounds__(THREADS, 1)
         // B rows of half 0; half 1 is `next` rows on
         const int b0 = w.group * p.b_group_rows + n0 + rank * (SWIGLU ? p.N : 64);
         const int next = SWIGLU ? 64 : 128;
-        const int a0 = (w.m + rank) * BM;
-        const bool live = rank < w.tiles;  // an idle half multiplies what its stage holds; nobody stores it
-        const uint32_t bytes = (w.tiles * A_BYTES) + 4 * B_HALF_BYTES;  // of both CTAs
+        const bool narrow = w.tiles == 1;  // 64 of the copied 128 rows per CTA
+        const int a0 = narrow ? w.m * BM + 64 * rank : (w.m + rank) * BM;
+        const int b32 = w.group * p.b_group_rows + n0 + rank * 32;  // narrow SwiGLU: 32 gate and up rows per half
+        const uint32_t bytes = 2 * A_BYTES + 4 * B_HALF_BYTES;  // of both CTAs
         for (int kb = kb_begin; kb < kb_begin + kb_count; ++kb) {
           ok = lane_wait(empty_bar(s), phase ^ 1, empty_bar(s), phase ^ 1, abort_flag, p.status, kDevTimeoutProducer);
           if (!ok) break;
           const uint32_t dst = base + s * STAGE_BYTES, bar = lead_full + 8u * s;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), bytes);
-          if (live) tma_load_2d_pair(dst, &tm_a, bar, kb * BK, a0, pol_a);
-          tma_load_2d_pair(dst + A_BYTES, &tm_b, bar, kb * BK, b0, pol_b);
-          tma_load_2d_pair(dst + A_BYTES + B_HALF_BYTES, &tm_b, bar, kb * BK, b0 + next, pol_b);
+          tma_load_2d_pair(dst, &tm_a, bar, kb * BK, a0, pol_a);
+          if (SWIGLU && narrow) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // gate and up rows of half 0, then of half 1
+              tma_load_2d_pair(dst + A_BYTES + i * (B_HALF_BYTES / 2), &tm_b32, bar, kb * BK,
+                               b32 + 64 * (i >> 1) + (i & 1) * p.N, pol_b);
+          } else {
+            tma_load_2d_pair(dst + A_BYTES, &tm_b, bar, kb * BK, b0, pol_b);
+            tma_load_2d_pair(dst + A_BYTES + B_HALF_BYTES, &tm_b, bar, kb * BK, b0 + next, pol_b);
+          }
           filled |= 1u << s;
           if (++s == STAGES) s = 0, phase ^= 1;
         }
@@ -643,7 +703,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == 1 || warp == 3) {
     // ------------------------------------------------------------ MMA issue, one half (one thread)
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_e4m3(2 * BM, NACC);
       const uint32_t half = warp >> 1;
       const uint16_t both = (uint16_t)(3 << lead);
       const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
@@ -651,6 +710,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t s = 0, phase = 0, it = 0;
       bool ok = true;
       for (int u = cluster; ok && u < units; u += clusters) {
+        const uint32_t idesc = unit_of(p, u, 2, first, begins).tiles == 1 ? idesc_e4m3(BM, NACC) : idesc_e4m3(2 * BM, NACC);
         for (int kb = 0; kb < kb_count; ++kb, ++it) {
           const uint32_t buf = (it & 1) * 2 + half;
           ok = lane_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, full_bar(s), phase, abort_flag, p.status, kDevTimeoutMma);
@@ -679,8 +739,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true;
     for (int u = cluster; ok && u < units; u += clusters) {
       const Unit w = unit_of(p, u, 2, first, begins);
-      const int64_t row0 = (int64_t)(w.m + rank) * BM + lane;
-      const int valid = rank < w.tiles ? (int)min((int64_t)BM, p.rows - row0) : 0;  // row 32 i + lane: 32 i < valid
+      // slots 32 i + lane: the CTA's rows in order, or a narrow unit's 64 rows twice
+      const bool narrow = w.tiles == 1;
+      const int64_t row0 = (narrow ? (int64_t)w.m * BM + 64 * rank : (int64_t)(w.m + rank) * BM) + lane;
+      const int valid = (int)max((int64_t)0, min((int64_t)BM, p.rows - row0));  // the i-th row: from(i) < valid
+      auto from = [&](int i) { return 32 * (narrow ? i & 1 : i); };
       const float* sa = p.a_scale + (valid > 0 ? row0 : 0) * p.kb;
       int block = 2 * w.n + (lane & 1);
       if (SWIGLU) block = lane == 0 ? w.n : ((p.N + w.n * 128) >> 7) + (lane == 2);
@@ -693,16 +756,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (p.vec_scales) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            copy_async<16>(dst + 512 * i, 32 * i < valid ? sa + (int64_t)(32 * i) * p.kb + kb : p.a_scale,
-                           32 * i < valid);
+            copy_async<16>(dst + 512 * i, from(i) < valid ? sa + (int64_t)from(i) * p.kb + kb : p.a_scale,
+                           from(i) < valid);
           if (lane < 3) copy_async<16>(dst + 16 * BM, sb + kb, true);
         } else {
 #pragma unroll 1
           for (int j = 0; j < GROUP && kb + j < kb_begin + kb_count; ++j) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              copy_async<4>(dst + 512 * i + 4 * j, 32 * i < valid ? sa + (int64_t)(32 * i) * p.kb + kb + j : p.a_scale,
-                            32 * i < valid);
+              copy_async<4>(dst + 512 * i + 4 * j, from(i) < valid ? sa + (int64_t)from(i) * p.kb + kb + j : p.a_scale,
+                            from(i) < valid);
             if (lane < 3) copy_async<4>(dst + 16 * BM + 4 * j, sb + kb + j, true);
           }
         }
@@ -727,7 +790,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 template <typename OutT, bool SWIGLU, int SPLITS = 1>
-int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int clusters, bool pdl, cudaStream_t stream) {
+int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb32, const Params& p, int clusters, bool pdl,
+             cudaStream_t stream) {
   auto kernel = block_gemm_pair_kernel<OutT, SWIGLU, SPLITS>;
   SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   cudaLaunchConfig_t cfg = {};
@@ -743,7 +807,7 @@ int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
-  SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, p));
+  SB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tb32, p));
   count_launch();
   return STAGEML_OK;
 }
@@ -751,9 +815,9 @@ int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int 
 template <typename OutT>
 int run_plain(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int clusters, int splits, bool pdl,
               cudaStream_t stream) {
-  if (splits == 4) return run_pair<OutT, false, 4>(ta, tb, p, clusters, pdl, stream);
-  if (splits == 2) return run_pair<OutT, false, 2>(ta, tb, p, clusters, pdl, stream);
-  return run_pair<OutT, false>(ta, tb, p, clusters, pdl, stream);
+  if (splits == 4) return run_pair<OutT, false, 4>(ta, tb, tb, p, clusters, pdl, stream);
+  if (splits == 2) return run_pair<OutT, false, 2>(ta, tb, tb, p, clusters, pdl, stream);
+  return run_pair<OutT, false>(ta, tb, tb, p, clusters, pdl, stream);
 }
 
 // Clusters of SPLITS pairs that the device runs at one time (not all of its SMs: a cluster lies in
@@ -832,7 +896,12 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   SB_TRY(make_tmap_2d(&tb, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.groups * p.b_group_rows, (uint64_t)g.K,
                       (uint64_t)g.K, 64, BK, 128));
   const int clusters = (int)std::min<int64_t>(units, pairs);
-  if (g.swiglu) return run_pair<bf16, true>(ta, tb, p, clusters, g.pdl, stream);
+  if (g.swiglu) {
+    CUtensorMap tb32;  // a narrow unit's runs of 32 gate or up rows
+    SB_TRY(make_tmap_2d(&tb32, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.groups * p.b_group_rows, (uint64_t)g.K,
+                        (uint64_t)g.K, 32, BK, 128));
+    return run_pair<bf16, true>(ta, tb, tb32, p, clusters, g.pdl, stream);
+  }
   if (g.out_dtype == STAGEML_F32) return run_plain<float>(ta, tb, p, clusters, splits, g.pdl, stream);
   if (g.out_dtype == STAGEML_BF16) return run_plain<bf16>(ta, tb, p, clusters, splits, g.pdl, stream);
   return run_plain<f16>(ta, tb, p, clusters, splits, g.pdl, stream);

@@ -291,7 +291,7 @@ def test_moe_forward_blocks_routing_edges(ops, t):
     assert none.shape == (0, h)
 
 
-@pytest.mark.parametrize("t,e,k,shared", [(17, 64, 4, 1), (100, 128, 4, 0), (128, 64, 2, 2), (43, 64, 6, 0)])
+@pytest.mark.parametrize("t,e,k,shared", [(17, 64, 4, 1), (100, 128, 4, 0), (128, 64, 2, 2), (43, 64, 6, 0), (60, 128, 4, 1)])
 @pytest.mark.parametrize("skew", [False, True])
 def test_moe_forward_blocks_few_rows_per_expert(ops, t, e, k, shared, skew):
     """More than 16 tokens, few per expert on average; skewed, all slots name one expert (several row tiles)."""
