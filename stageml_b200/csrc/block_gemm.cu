@@ -847,14 +847,14 @@ int resident_clusters() {
 }
 
 // Pairs per tile: where the tiles leave SMs idle, several pairs share a tile's K blocks. A K block
-// takes a pair 0.4 us on an idle device and the exchange 2 us, so 12 blocks are worth it (64 x 4096
-// outputs over 8, 16, 32, 112 blocks: 9.8, 13.1, 19.8, 52 us alone, 9.8, 11.7, 15.2, 32 us in two;
-// 300 x 1000 over 32: 19.9 alone, 15.2 in two, 13.3 in four), while all clusters run at one time
-// (64 x 4096 in 16 clusters of eight CTAs: 25 us, in two turns).
+// takes a pair 0.25 (narrow units) to 0.4 us on an idle device and the exchange 1.5 to 2 us, so two pairs
+// pay from 12 blocks on (64 x 4096 outputs over 8, 12, 32, 112 blocks: 8.2, 9.5, 14.9, 36.0 us alone, 8.2,
+// 9.1, 12.2, 23.0 in two) and four from 24 (300 x 1000 over 12, 16, 32: 11.4, 12.2, 15.6 in two, 12.1,
+// 12.4, 14.3 in four), while all clusters run at one time (64 x 4096 in 16 clusters of eight CTAs took two
+// turns: 25 us, not 15).
 int splits_for(int64_t units, int kb) {
-  if (kb < 12) return 1;
-  if (units <= resident_clusters<4>()) return 4;
-  if (units <= resident_clusters<2>()) return 2;
+  if (kb >= 24 && units <= resident_clusters<4>()) return 4;
+  if (kb >= 12 && units <= resident_clusters<2>()) return 2;
   return 1;
 }
 

@@ -165,7 +165,7 @@ def test_block_matmul(ops, m, n, k, out):
 
 @pytest.mark.parametrize("out", [F32, BF16, F16])
 @pytest.mark.parametrize("m,n,k", [(17, 130, 1536), (64, 4096, 1552), (300, 500, 2048), (257, 1001, 1616), (500, 4095, 2064),
-                                   (33, 8, 14336), (2048, 1027, 272)])
+                                   (33, 8, 14336), (2048, 1027, 272), (300, 500, 3200), (257, 131, 4112)])
 def test_block_matmul_shared_k_and_odd_widths(ops, m, n, k, out):
     """Few tiles with a long K, whose blocks several CTA pairs share, and rows that do not start at 16 bytes."""
     x, xs, w, ws = operands(m, n, k, seed=m + n + k)
