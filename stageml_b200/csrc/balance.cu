@@ -14,8 +14,8 @@
 // per lane, so a warp works on 4 to 32 tokens at once and a softmax costs few shuffles.
 // Each lane sums its experts' p over its tokens in registers; a CTA adds them in a fixed
 // order in shared memory. Counts are integer atomics in shared memory. Batches of up to
-// kClusterValues logits run as one cluster whose first CTA adds the others' sums over
-// distributed shared memory and writes the loss: one launch. Longer ones run as many clusters,
+// kClusterValues logits and kClusterTokens tokens run as one cluster whose first CTA adds the
+// others' sums over distributed shared memory and writes the loss: one launch. Longer ones run as many clusters,
 // each leaving one partial, which a second kernel adds in cluster order (one partial per CTA
 // made that kernel 32 us, now 6). No floating-point atomics: the same bits
 // on every run. Backward: the softmax again from the logits, one pass. Bound: HBM for long
@@ -32,7 +32,10 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxE = 256;
 constexpr int kClusterCtas = 8;                // portable cluster size
-constexpr int64_t kClusterValues = 256 * 1024;  // logits of a one-launch batch
+// A one-launch batch: its logits, and its tokens, whose ids eight CTAs count one by one (20000 x 5, five
+// ids: 30 us in one cluster, 10 in several).
+constexpr int64_t kClusterValues = 256 * 1024, kClusterTokens = 4096;
+inline bool one_launch(int64_t T, int E) { return T * E <= kClusterValues && T <= kClusterTokens; }
 
 // Lanes per token and 4-expert groups per lane: expert (lane + LANES * j) * 4 + i.
 template <int LANES, int NV>
@@ -393,7 +396,7 @@ struct ForwardOut {
 template <typename T, typename L, bool VEC>
 int forward_layout(const T* logits, const BalanceIn& in, float coefficient, const ForwardOut& o, void* scratch,
                    cudaStream_t stream) {
-  const bool one = in.T * in.E <= kClusterValues;
+  const bool one = one_launch(in.T, in.E);
   int cluster = kClusterCtas, grid = 0;
   if (one) {  // a power of two of CTAs with a token group per warp, at least one
     for (cluster = 1; cluster < kClusterCtas && cluster < ctas_for(in.T, in.E, kClusterCtas);) cluster <<= 1;
@@ -454,7 +457,7 @@ int backward(const float* grad_loss, const void* logits, const int32_t* counts, 
 }  // namespace
 
 size_t balance_scratch_bytes(int64_t T, int E) {
-  return T * E <= kClusterValues ? 0 : (size_t)(long_ctas(T, E) / kClusterCtas) * (2 * E + 1) * 4;
+  return one_launch(T, E) ? 0 : (size_t)(long_ctas(T, E) / kClusterCtas) * (2 * E + 1) * 4;
 }
 
 int launch_balance_loss(const void* logits, int dtype, const void* ids, int ids_i64, const uint8_t* valid, int64_t T,
