@@ -384,8 +384,8 @@ int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* 
  * stageml_moe_forward without LoRA, with both products on e4m3 operands):
  *   out[t] = sum_j w[t,j] * W2_e . Q( silu(W1_e . Q(x_t)) * (W3_e . Q(x_t)) ),  e = ids[t, j],
  * plus the n_shared always-on experts (index E + i, weight 1). Q(v) is v as its e4m3 codes
- * and 1 x 128 scales hold it; the products sum in fp32, and a routed row leaves the down
- * projection in the activation dtype, weighted, before the fp32 sum over a token's slots.
+ * and 1 x 128 scales hold it; the products and the sum over a token's slots are fp32, rounded
+ * once to the activation dtype.
  * gate_up [E_tot, 2I, H] e4m3 (rows [0, I) = W1, [I, 2I) = W3), gate_up_scale
  * [E_tot, ceil(2I/128), ceil(H/128)]; down [E_tot, H, I], down_scale [E_tot, ceil(H/128),
  * ceil(I/128)], E_tot = E + n_shared. H and I are multiples of 16. An id outside [0, E) drops

@@ -19,7 +19,7 @@ struct MoeBlocksBuffers {
   float* h = nullptr;        // few rows: [rows_cap, I] silu(gate) * up in fp32
   uint8_t* hq = nullptr;     // [rows_cap, I] codes of silu(gate) * up
   float* hs = nullptr;       // [rows_cap, ceil(I/128)]
-  void* y = nullptr;         // [rows_cap, H] weighted rows of the down projection
+  float* y = nullptr;        // [rows_cap, H] weighted rows of the down projection, not rounded before the slots' sum
   int32_t* status = nullptr;
   size_t bytes = 0;
 };
@@ -48,7 +48,7 @@ void moe_blocks_carve(const stageml_moe_blocks_args* a, void* ws, MoeBlocksBuffe
   if (moe_blocks_skinny(a)) b->h = c.take<float>(rows * a->I);
   b->hq = c.take<uint8_t>(rows * a->I);
   b->hs = c.take<float>(rows * scale_blocks(a->I));
-  b->y = c.take_bytes(rows * a->H * 2);
+  b->y = c.take<float>(rows * a->H);
   b->status = c.take<int32_t>(1);
   b->bytes = c.off;
 }
@@ -141,10 +141,10 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   g.swiglu = false;
   g.row_scale = b.plan.row_weight;
   g.out = b.y;
-  g.out_dtype = a->act_dtype;
+  g.out_dtype = STAGEML_F32;
   SB_STAGE(STAGEML_STAGE_GEMM_DOWN, skinny ? launch_block_skinny(g, sk, st) : launch_block_gemm(g, st));
   SB_STAGE(STAGEML_STAGE_COMBINE, launch_combine(b.y, b.plan.pair_row, a->T, slots, a->H,
-                                                 a->act_dtype == STAGEML_BF16, a->out, st, nullptr, pdl));
+                                                 a->act_dtype == STAGEML_BF16, a->out, st, nullptr, pdl, true));
   return STAGEML_OK;
 }
 

@@ -2,7 +2,8 @@
 // routing weight already applied by the down-projection epilogue. This is the
 // out.index_add_(0, index, y * gates) of RequestExecutor.dynamic_one
 // (benchmarks/multitenant_bta_system_bench.py:413) done once per token with a
-// fixed slot order (fp32 sum, one rounding), so it is deterministic.
+// fixed slot order (fp32 sum, one rounding), so it is deterministic. Y is in the
+// output's 16-bit type or in fp32 (TY).
 #include "common.cuh"
 #include "host_util.h"
 #include "kernels.h"
@@ -10,8 +11,8 @@
 namespace sb {
 namespace {
 
-template <typename T>
-__global__ void combine_kernel(const T* __restrict__ y, const int32_t* __restrict__ pair_row, int T_, int kk, int H,
+template <typename TY, typename T>
+__global__ void combine_kernel(const TY* __restrict__ y, const int32_t* __restrict__ pair_row, int T_, int kk, int H,
                                T* __restrict__ out, const int32_t* __restrict__ T_dev, int t_base) {
   pdl_wait();  // y comes from the previous kernel
   const int t = blockIdx.y;
@@ -24,9 +25,14 @@ __global__ void combine_kernel(const T* __restrict__ y, const int32_t* __restric
   for (int j = 0; j < kk; ++j) {
     const int row = pair_row[(int64_t)t * kk + j];
     if (row < 0) continue;
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(y + (int64_t)row * H + c));
+    const uint4* src = reinterpret_cast<const uint4*>(y + (int64_t)row * H + c);
     float f[8];
-    unpack8<T>(u, f);
+    if constexpr (sizeof(TY) == 4) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else {
+      unpack8<T>(__ldg(src), f);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] += f[i];
   }
@@ -82,6 +88,24 @@ __global__ void direct_rows_kernel(const void* __restrict__ ids, int ids_i64, co
   row_scale[t] = bad ? 0.f : w;
 }
 
+// Tokens are the grid's second dimension; more than it takes go in several launches, the first of which may be
+// programmatic.
+template <typename TY, typename T>
+int run_combine(const void* y, const int32_t* pair_row, int T_, int kk, int H, void* out, cudaStream_t stream,
+                const int32_t* T_dev, bool pdl) {
+  constexpr int kMaxGridY = 65535;
+  const dim3 block(128);
+  for (int t0 = 0; t0 < T_; t0 += kMaxGridY) {
+    const int nt = std::min(kMaxGridY, T_ - t0);
+    const dim3 grid((unsigned)((H / 8 + block.x - 1) / block.x), (unsigned)nt);
+    SB_CUDA_CHECK(launch_kernel(combine_kernel<TY, T>, grid, block, 0, stream, pdl && t0 == 0, static_cast<const TY*>(y),
+                                pair_row + (int64_t)t0 * kk, nt, kk, H, static_cast<T*>(out) + (int64_t)t0 * H, T_dev, t0));
+    ::sb::count_launch();
+  }
+  SB_CUDA_CHECK(cudaGetLastError());
+  return STAGEML_OK;
+}
+
 }  // namespace
 
 int launch_direct_rows(const void* ids, int ids_dtype, const void* weights, int weights_dtype, const int32_t* tenant_ids,
@@ -97,37 +121,15 @@ int launch_direct_rows(const void* ids, int ids_dtype, const void* weights, int 
 }
 
 int launch_combine(const void* y, const int32_t* pair_row, int T_, int kk, int H, int dtype_bf16, void* out,
-                   cudaStream_t stream, const int32_t* T_dev, bool pdl) {
+                   cudaStream_t stream, const int32_t* T_dev, bool pdl, bool y_f32) {
   SB_CHECK_ARG(H % 8 == 0, "combine: H=%d must be a multiple of 8", H);
   if (T_ == 0 || H == 0) return STAGEML_OK;
-  dim3 block(128);
-  dim3 grid((unsigned)((H / 8 + block.x - 1) / block.x), (unsigned)T_);
   SB_CHECK_ARG(T_ <= 65535 * 64, "combine: too many tokens");
-  if (grid.y > 65535) {
-    // split tokens over several launches
-    for (int t0 = 0; t0 < T_; t0 += 65535) {
-      const int nt = std::min(65535, T_ - t0);
-      dim3 g2(grid.x, (unsigned)nt);
-      if (dtype_bf16)
-        (combine_kernel<bf16><<<g2, block, 0, stream>>>(static_cast<const bf16*>(y), pair_row + (int64_t)t0 * kk, nt,
-                                                        kk, H, static_cast<bf16*>(out) + (int64_t)t0 * H, T_dev, t0),
-         ::sb::count_launch());
-      else
-        (combine_kernel<f16><<<g2, block, 0, stream>>>(static_cast<const f16*>(y), pair_row + (int64_t)t0 * kk, nt,
-                                                       kk, H, static_cast<f16*>(out) + (int64_t)t0 * H, T_dev, t0),
-         ::sb::count_launch());
-    }
-  } else if (dtype_bf16) {
-    SB_CUDA_CHECK(launch_kernel(combine_kernel<bf16>, grid, block, 0, stream, pdl, static_cast<const bf16*>(y), pair_row,
-                                T_, kk, H, static_cast<bf16*>(out), T_dev, 0));
-    ::sb::count_launch();
-  } else {
-    SB_CUDA_CHECK(launch_kernel(combine_kernel<f16>, grid, block, 0, stream, pdl, static_cast<const f16*>(y), pair_row,
-                                T_, kk, H, static_cast<f16*>(out), T_dev, 0));
-    ::sb::count_launch();
-  }
-  SB_CUDA_CHECK(cudaGetLastError());
-  return STAGEML_OK;
+  if (dtype_bf16)
+    return y_f32 ? run_combine<float, bf16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl)
+                 : run_combine<bf16, bf16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl);
+  return y_f32 ? run_combine<float, f16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl)
+               : run_combine<f16, f16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl);
 }
 
 int launch_validate_tenants(const int32_t* in, int64_t n, int n_tenants, int32_t* out, int32_t* status,
