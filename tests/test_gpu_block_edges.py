@@ -43,3 +43,25 @@ def test_slots_beyond_the_16_bit_range(ops, t):
     y = ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w)
     # each slot's fp32 error is 1e-5 of 1024 times the sum: 1e-5 * 1024 * sqrt 2
     close(y, ref, TOL[F16] + 1.5e-2)
+
+
+@pytest.mark.parametrize("t", [16, 200])
+@pytest.mark.parametrize("scale", [1e-18, 1e-19, 1e-20, 1e-21, 1e-22, 1e-23])
+def test_rows_of_small_numbers(ops, t, scale):
+    """h at the bottom of fp32's range, with a channel of zeros: finite, and its definition's value. From 1e-21 on h
+    itself has only a few bits and the scale's rounding decides; there the output is only bounded."""
+    e, k, h, i = 4, 2, 192, 160
+    gu, gus, dn, dns = layer_weights(e, h, i, seed=26)
+    gu.view(torch.uint8)[:, 5] = 0  # a pruned gate channel: h[5] = 0
+    dns = torch.full_like(dns, 16.0)  # a power of two: the product of the two scales is exact
+    x = (randn(t, h, seed=27) * scale).to(BF16)
+    ids = randn(t, e, seed=28).topk(k, 1).indices.to(torch.int32)
+    w = torch.full((t, k), 0.5, device=DEV)
+    y = ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w)
+    assert y.isfinite().all()
+    ref = ref_layer(x, gu, gus, dn, dns, ids, w, 0)
+    if scale >= 1e-20:
+        close(y, ref, LAYER_TOL[BF16])
+    else:
+        wide = torch.nn.functional.silu(x.double()).abs().max()  # bound: |h| <= (|W| |x|)^2 / 2 over 192 terms of 4 / sqrt h
+        assert y.double().abs().max() <= 16 * 448 * i * max(float((8 * wide * math.sqrt(h)) ** 2), 2.0 ** -149 * 448)
