@@ -14,8 +14,35 @@ once, when the module is built. Tenants with LoRA adapters stay with ``ops.moe_f
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
+
+
+class _Route(torch.autograd.Function):
+    """ops.route_topk (ids, renormalised weights, logits) with the gradients of its weights and logits."""
+
+    @staticmethod
+    def forward(ctx, rows, router_w, k):
+        ctx.set_materialize_grads(False)
+        ids, weights, logits = ops.route_topk(rows, router_w, k)
+        ctx.save_for_backward(rows, router_w, ids, weights)
+        ctx.mark_non_differentiable(ids)
+        return ids, weights, logits
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _ids, d_weights, d_logits):
+        rows, router_w, ids, weights = ctx.saved_tensors
+        if d_weights is not None:  # a softmax over the chosen logits
+            d = weights * (d_weights - (d_weights * weights).sum(1, keepdim=True))
+            chosen = d.new_zeros(d.shape[0], router_w.shape[0]).scatter_(1, ids.long(), d)
+            d_logits = chosen if d_logits is None else d_logits + chosen
+        if d_logits is None:
+            return None, None, None
+        d_rows = (d_logits @ router_w).to(rows.dtype) if ctx.needs_input_grad[0] else None
+        d_router_w = d_logits.t() @ rows.float() if ctx.needs_input_grad[1] else None
+        return d_rows, d_router_w, None
 
 
 class FeedForwardBlock(torch.nn.Module):
@@ -67,10 +94,9 @@ class FeedForwardBlock(torch.nn.Module):
 
     def balance(self, normed, valid=None):
         """The router's balance loss on normed [..., H] -> (loss, counts per expert, tokens); differentiable in
-        router_w and normed."""
-        rows = normed.reshape(-1, normed.shape[-1])
-        logits = torch.nn.functional.linear(rows.float(), self.router_w)
-        ids, _ = ops.topk_from_logits(logits.detach(), self.k)
+        router_w and normed. The counts are of the experts that ``experts`` runs for the same rows."""
+        rows = normed.reshape(-1, normed.shape[-1]).contiguous()
+        ids, _, logits = _Route.apply(rows, self.router_w, self.k)
         return ops.balance_loss(logits, ids, self.balance_coefficient, valid=valid)
 
 
