@@ -45,6 +45,72 @@ class _Route(torch.autograd.Function):
         return d_rows, d_router_w, None
 
 
+def _row_values(x):
+    """x [rows, cols] as its codes hold it, fp32."""
+    q, scale = ops.quantize_e4m3_blocks(x)
+    return q.float() * scale.repeat_interleave(128, 1)[:, : x.shape[1]]
+
+
+def _tile_values(q, scale):
+    """A matrix of codes with a scale per 128 x 128 tile, fp32."""
+    rows, cols = q.shape
+    return q.float() * scale.repeat_interleave(128, 1)[:, :cols].repeat_interleave(128, 0)[:rows]
+
+
+class _Experts(torch.autograd.Function):
+    """ops.moe_forward_blocks with the gradients of its rows and routing weights; the experts are frozen.
+
+    The gradient passes the two roundings to e4m3 codes (rows, silu(gate) * up) as if they were not there, at the
+    values that the codes hold. It is the plain chain in fp32, one expert at a time: that expert's weights are
+    dequantized (12 H I bytes at a time) and multiplied by library products, and the host reads the rows per expert
+    once, so the backward pass cannot be captured in a graph. Forward products are the framework's kernels.
+    """
+
+    @staticmethod
+    def forward(ctx, rows, weights, ids, gate_up, gate_up_scale, down, down_scale, n_shared):
+        ctx.save_for_backward(rows, weights, ids, gate_up, gate_up_scale, down, down_scale)
+        ctx.n_shared = n_shared
+        return ops.moe_forward_blocks(rows, gate_up, gate_up_scale, down, down_scale, topk_ids=ids, topk_weights=weights,
+                                      n_shared=n_shared)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, weights, ids, gate_up, gate_up_scale, down, down_scale = ctx.saved_tensors
+        routed, k = gate_up.shape[0] - ctx.n_shared, weights.shape[1]
+        x, dy = _row_values(rows), dy.float()
+        dx, dw = torch.zeros_like(x), torch.zeros_like(weights)
+
+        def expert(j, x, dy, w):
+            """Gradients of the rows x and, one per row, of w in w * W2 (silu(W1 x) * (W3 x))."""
+            w13 = _tile_values(gate_up[j], gate_up_scale[j])
+            gate, up = (x @ w13.t()).chunk(2, 1)
+            sig = torch.sigmoid(gate)
+            act = gate * sig
+            dh = dy @ _tile_values(down[j], down_scale[j])
+            d_weight = (dh * _row_values(act * up)).sum(1)
+            dh = dh * w
+            d_gate = dh * up * (sig + act * (1 - sig))
+            return torch.cat((d_gate, dh * act), 1) @ w13, d_weight
+
+        flat = ids.reshape(-1).long()
+        flat = torch.where((flat >= 0) & (flat < routed), flat, routed)  # a slot without an expert
+        order = flat.argsort(stable=True)
+        at = 0
+        for j, n in enumerate(torch.bincount(flat, minlength=routed + 1).tolist()[:routed]):
+            if n == 0:
+                continue
+            pair = order[at:at + n]
+            at += n
+            token = pair // k
+            d_rows, d_weight = expert(j, x[token], dy[token], weights.view(-1)[pair][:, None])
+            dx.index_add_(0, token, d_rows)  # the router names an expert once per token: no two rows meet
+            dw.view(-1)[pair] = d_weight
+        for j in range(routed, gate_up.shape[0]):
+            dx += expert(j, x, dy, 1.0)[0]
+        return dx.to(rows.dtype), dw, None, None, None, None, None, None
+
+
 class FeedForwardBlock(torch.nn.Module):
     """Router, block-scaled experts, post norm, gate, residual sum and the next block's pre norm.
 
@@ -77,17 +143,16 @@ class FeedForwardBlock(torch.nn.Module):
         return x, ops.norm_residual(None, x, pre_weight=self.pre_weight, eps=self.eps)[1]
 
     def experts(self, normed):
-        """The routed experts' output for normed [..., H]."""
-        rows = normed.detach().reshape(-1, normed.shape[-1])
-        ids, weights, _ = ops.route_topk(rows, self.router_w.detach(), self.k)
-        y = ops.moe_forward_blocks(rows, self.gate_up, self.gate_up_scale, self.down, self.down_scale, topk_ids=ids,
-                                   topk_weights=weights, n_shared=self.n_shared)
+        """The routed experts' output for normed [..., H]; differentiable in normed and router_w."""
+        rows = normed.reshape(-1, normed.shape[-1]).contiguous()
+        ids, weights, _ = _Route.apply(rows, self.router_w, self.k)
+        y = _Experts.apply(rows, weights, ids, self.gate_up, self.gate_up_scale, self.down, self.down_scale, self.n_shared)
         return y.view(normed.shape)
 
     def forward(self, residual, normed, next_pre_weight=None):
         """-> (residual', normed') with next_pre_weight (the next block's pre norm), else (residual',).
 
-        Gradients reach the residual stream, the norms' weights and the gate; the experts are frozen.
+        Gradients reach both inputs, the norms' weights, the gate and the router; the experts' weights are frozen.
         """
         return ops.norm_residual(self.experts(normed), residual, post_weight=self.post_weight, gate=self.gate,
                                  residual_scale=self.residual_scale, pre_weight=next_pre_weight, eps=self.eps)

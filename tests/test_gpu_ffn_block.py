@@ -23,6 +23,96 @@ def make_block(seed=80, e=E, k=K, shared=1, h=H, i=I, **kw):
                             randn(e + shared, h, i, seed=seed + 2, scale=i ** -0.5, dtype=BF16), k, n_shared=shared, **args)
 
 
+def straight(x):
+    """x as its codes hold it, in float64; its gradient passes the rounding."""
+    q = dequant(*ref_codes(x.detach().float(), 1), 1)
+    return x + (q - x).detach()
+
+
+def ref_experts(block, normed, router_w, ids):
+    """The routed experts in float64 with the experts chosen as `ids`, differentiable in normed and router_w."""
+    e = block.router_w.shape[0]
+    weights = torch.gather(normed @ router_w.t(), 1, ids.long()).softmax(1)
+    x = straight(normed)
+    out = torch.zeros_like(normed)
+    for j in range(block.gate_up.shape[0]):
+        if j < e:
+            token, slot = (ids == j).nonzero(as_tuple=True)
+            w = weights[token, slot][:, None]
+        else:
+            token, w = torch.arange(normed.shape[0], device=DEV), 1.0
+        if token.numel() == 0:
+            continue
+        y = x[token] @ dequant(block.gate_up[j], block.gate_up_scale[j], 128).t()
+        i = y.shape[1] // 2
+        act = straight(torch.nn.functional.silu(y[:, :i]) * y[:, i:])
+        out = out.index_add(0, token, (act @ dequant(block.down[j], block.down_scale[j], 128).t()) * w)
+    return out
+
+
+def ref_rms(x, w, eps=1e-6):
+    return x * (x.square().mean(-1, keepdim=True) + eps).rsqrt() * w
+
+
+@pytest.mark.parametrize("t", [6, 200])
+def test_gradients_reach_the_input_and_the_router(ops, t):
+    """The experts' own gradient: of the rows that they read and of the router that weighs them."""
+    block = make_block()
+    x = randn(t, H, seed=90, dtype=BF16).requires_grad_(True)
+    g = randn(t, H, seed=91, dtype=BF16)
+    y = block.experts(x)
+    y.backward(g)
+    ids, _, _ = ops.route_topk(x.detach(), block.router_w.detach(), K)
+    xd, rd = x.detach().double().requires_grad_(True), block.router_w.detach().double().requires_grad_(True)
+    ref = ref_experts(block, xd, rd, ids)
+    close(y, ref, LAYER_TOL[BF16])
+    ref.backward(g.double())
+    close(x.grad, xd.grad, LAYER_TOL[BF16])
+    close(block.router_w.grad, rd.grad, LAYER_TOL[BF16])
+
+
+def test_gradients_of_two_blocks(ops):
+    """A stack: what an earlier block's inputs and weights get through the later block's experts."""
+    a, b = make_block(seed=100), make_block(seed=120)
+    x = randn(40, H, seed=92).requires_grad_(True)  # an fp32 stream, so that the roundings between the blocks are few
+    residual, normed = x, ops.norm_residual(None, x, pre_weight=a.pre_weight, normed_dtype=BF16)[1]
+    residual, normed2 = a(residual, normed, next_pre_weight=b.pre_weight)
+    out, = b(residual, normed2)
+    g = randn(40, H, seed=93)
+    out.backward(g)
+    names = ["pre_weight", "post_weight", "gate", "router_w"]
+    p = [{n: getattr(m, n).detach().double().requires_grad_(True) for n in names} for m in (a, b)]
+    xd = x.detach().double().requires_grad_(True)
+    r, n, pre = xd, None, p[0]["pre_weight"]
+    for m, q, got in ((a, p[0], normed), (b, p[1], normed2)):
+        n = ref_rms(r, q["pre_weight"])
+        n = n + (got.detach().double() - n).detach()  # the rows that the experts read, as the 16-bit type holds them
+        ids, _, _ = ops.route_topk(got.detach(), m.router_w.detach(), K)
+        y = ref_experts(m, n, q["router_w"], ids)
+        y = y + (m.experts(got.detach()).detach().double() - y).detach()
+        r = 0.9 * r + q["gate"] * ref_rms(y, q["post_weight"])
+    close(out, r, 1e-4)
+    r.backward(g.double())
+    close(x.grad, xd.grad, LAYER_TOL[BF16])
+    for m, q in ((a, p[0]), (b, p[1])):
+        for name in names:
+            close(getattr(m, name).grad, q[name].grad, LAYER_TOL[BF16])
+
+
+def test_gradient_is_the_same_every_run(ops):
+    block = make_block()
+    x = randn(150, H, seed=94, dtype=BF16)
+    g = randn(150, H, seed=95, dtype=BF16)
+    grads = []
+    for _ in range(3):
+        leaf = x.clone().requires_grad_(True)
+        block.zero_grad()
+        block.experts(leaf).backward(g)
+        grads.append((leaf.grad, block.router_w.grad.clone()))
+    for a, b in grads[1:]:
+        assert torch.equal(a, grads[0][0]) and torch.equal(b, grads[0][1])
+
+
 @pytest.mark.parametrize("t", [5, 300, 5000])
 def test_balance_counts_the_experts_that_ran(ops, t):
     """Ties between experts up to the order of a sum: the loss counts what the experts' router chose, not what another
