@@ -111,13 +111,17 @@ class _Experts(torch.autograd.Function):
         return dx.to(rows.dtype), dw, None, None, None, None, None, None
 
 
+CODE_BUFFERS = ("gate_up", "gate_up_scale", "down", "down_scale")
+
+
 class FeedForwardBlock(torch.nn.Module):
     """Router, block-scaled experts, post norm, gate, residual sum and the next block's pre norm.
 
     router_w [E, H] float32; gate_up [E + n_shared, 2I, H] (rows [:I] the SiLU branch) and down
     [E + n_shared, H, I] in float32, bfloat16 or float16; H and I multiples of 16. post_weight [H], gate
     [H] and pre_weight [H] are optional (no norm, gate 1, no norm). balance_coefficient scales the loss
-    of ``balance``.
+    of ``balance``. The quantized weights are buffers: saved, loaded and moved with the module, never cast. A router
+    cast to 16 bits is read as fp32.
     """
 
     def __init__(self, router_w, gate_up, down, k: int, *, n_shared: int = 0, pre_weight=None, post_weight=None,
@@ -133,10 +137,24 @@ class FeedForwardBlock(torch.nn.Module):
         self.router_w = torch.nn.Parameter(router_w.detach().float().contiguous())
         with torch.no_grad():
             codes = [ops.quantize_e4m3_blocks(w, tiles=True) for w in (gate_up, down)]
-        self.gate_up, self.gate_up_scale = codes[0]
-        self.down, self.down_scale = codes[1]
+        for names, pair in zip((CODE_BUFFERS[:2], CODE_BUFFERS[2:]), codes):
+            for name, t in zip(names, pair):
+                self.register_buffer(name, t)
         for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight), ("gate", gate)):
             self.register_parameter(name, None if w is None else torch.nn.Parameter(w.detach().clone()))
+
+    def _apply(self, fn, recurse=True):
+        """Moves as Module has them; casts leave the codes and their fp32 scales what they are."""
+        held = {name: self._buffers.pop(name) for name in CODE_BUFFERS}
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            self._buffers.update(held)
+        for name, t in held.items():
+            bits = t.view(torch.uint8)  # an integer tensor: casts of floating-point tensors pass it by
+            moved = fn(bits)
+            self._buffers[name] = (moved if moved.dtype == torch.uint8 else bits.to(moved.device)).view(t.dtype)
+        return self
 
     def start(self, x):
         """(residual, normed) of the stack's first block: x and its pre norm."""
@@ -145,7 +163,7 @@ class FeedForwardBlock(torch.nn.Module):
     def experts(self, normed):
         """The routed experts' output for normed [..., H]; differentiable in normed and router_w."""
         rows = normed.reshape(-1, normed.shape[-1]).contiguous()
-        ids, weights, _ = _Route.apply(rows, self.router_w, self.k)
+        ids, weights, _ = _Route.apply(rows, self.router_w.float(), self.k)
         y = _Experts.apply(rows, weights, ids, self.gate_up, self.gate_up_scale, self.down, self.down_scale, self.n_shared)
         return y.view(normed.shape)
 
@@ -161,7 +179,7 @@ class FeedForwardBlock(torch.nn.Module):
         """The router's balance loss on normed [..., H] -> (loss, counts per expert, tokens); differentiable in
         router_w and normed. The counts are of the experts that ``experts`` runs for the same rows."""
         rows = normed.reshape(-1, normed.shape[-1]).contiguous()
-        ids, _, logits = _Route.apply(rows, self.router_w, self.k)
+        ids, _, logits = _Route.apply(rows, self.router_w.float(), self.k)
         return ops.balance_loss(logits, ids, self.balance_coefficient, valid=valid)
 
 

@@ -113,6 +113,35 @@ def test_gradient_is_the_same_every_run(ops):
         assert torch.equal(a, grads[0][0]) and torch.equal(b, grads[0][1])
 
 
+def test_state_holds_the_experts(ops):
+    a, b = make_block(seed=80), make_block(seed=140)
+    names = {"gate_up", "gate_up_scale", "down", "down_scale"}
+    assert names <= set(a.state_dict())
+    x = randn(12, H, seed=96, dtype=BF16)
+    assert not torch.equal(a.experts(x), b.experts(x))
+    b.load_state_dict({k: v.cpu() for k, v in a.state_dict().items()})
+    assert torch.equal(a.experts(x), b.experts(x))
+    c = copy.deepcopy(a)
+    assert torch.equal(a.experts(x), c.experts(x))
+
+
+def test_moves_and_casts_keep_the_codes(ops):
+    block = make_block()
+    x = randn(12, H, seed=97, dtype=BF16)
+    want = block.experts(x)
+    block.cpu()
+    assert all(getattr(block, n).device.type == "cpu" for n in ("gate_up", "gate_up_scale", "down", "down_scale"))
+    block.to(DEV)
+    assert torch.equal(block.experts(x), want)
+    for cast in (lambda m: m.double(), lambda m: m.float(), lambda m: m.to(F16), lambda m: m.float()):
+        cast(block)
+        assert block.gate_up.dtype == block.down.dtype == torch.float8_e4m3fn
+        assert block.gate_up_scale.dtype == block.down_scale.dtype == F32
+    block.to(torch.device(DEV), F32)
+    assert block.experts(x).isfinite().all()
+    assert block.bfloat16().experts(x).isfinite().all()  # a router in 16 bits is read as fp32
+
+
 @pytest.mark.parametrize("t", [5, 300, 5000])
 def test_balance_counts_the_experts_that_ran(ops, t):
     """Ties between experts up to the order of a sum: the loss counts what the experts' router chose, not what another
