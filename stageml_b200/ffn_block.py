@@ -156,9 +156,16 @@ class FeedForwardBlock(torch.nn.Module):
             self._buffers[name] = (moved if moved.dtype == torch.uint8 else bits.to(moved.device)).view(t.dtype)
         return self
 
-    def start(self, x):
-        """(residual, normed) of the stack's first block: x and its pre norm."""
-        return x, ops.norm_residual(None, x, pre_weight=self.pre_weight, eps=self.eps)[1]
+    def start(self, x, normed_dtype=None):
+        """(residual, normed) of the stack's first block: x and its pre norm (x itself without pre_weight).
+
+        The experts read 16-bit rows: normed_dtype names their type, x's own by default, bfloat16 beside an fp32 x.
+        """
+        if normed_dtype is None:
+            normed_dtype = torch.bfloat16 if x.dtype == torch.float32 else x.dtype
+        if self.pre_weight is None:
+            return x, x.to(normed_dtype)
+        return x, ops.norm_residual(None, x, pre_weight=self.pre_weight, eps=self.eps, normed_dtype=normed_dtype)[1]
 
     def experts(self, normed):
         """The routed experts' output for normed [..., H]; differentiable in normed and router_w."""

@@ -142,6 +142,23 @@ def test_moves_and_casts_keep_the_codes(ops):
     assert block.bfloat16().experts(x).isfinite().all()  # a router in 16 bits is read as fp32
 
 
+def test_start_without_a_norm_and_with_an_fp32_stream(ops):
+    block = make_block(pre_weight=None)
+    x = randn(10, H, seed=98, dtype=BF16)
+    residual, normed = block.start(x)
+    assert residual is x and torch.equal(normed, x)
+    assert len(block(residual, normed)) == 1
+    x32 = randn(10, H, seed=99)
+    assert block.start(x32)[1].dtype == BF16
+    block = make_block()
+    for dtype, want in ((None, BF16), (F16, F16), (BF16, BF16)):
+        residual, normed = block.start(x32, normed_dtype=dtype)
+        assert residual is x32 and normed.dtype == want
+        close(normed, ref_rms(x32.double(), block.pre_weight.double()))
+        new, nxt = block(residual, normed, next_pre_weight=block.pre_weight)
+        assert new.dtype == F32 and nxt.dtype == want
+
+
 @pytest.mark.parametrize("t", [5, 300, 5000])
 def test_balance_counts_the_experts_that_ran(ops, t):
     """Ties between experts up to the order of a sum: the loss counts what the experts' router chose, not what another
