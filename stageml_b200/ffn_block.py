@@ -14,9 +14,9 @@ once, when the module is built. Tenants with LoRA adapters stay with ``ops.moe_f
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
+from .ops import differentiable_once
 
 
 class _Route(torch.autograd.Function):
@@ -31,7 +31,7 @@ class _Route(torch.autograd.Function):
         return ids, weights, logits
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, _ids, d_weights, d_logits):
         rows, router_w, ids, weights = ctx.saved_tensors
         if d_weights is not None:  # a softmax over the chosen logits
@@ -74,7 +74,7 @@ class _Experts(torch.autograd.Function):
                                       n_shared=n_shared)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         rows, weights, ids, gate_up, gate_up_scale, down, down_scale = ctx.saved_tensors
         routed, k = gate_up.shape[0] - ctx.n_shared, weights.shape[1]

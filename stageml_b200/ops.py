@@ -8,6 +8,7 @@ stream. Fake (meta) implementations are registered so the ops trace under
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -283,6 +284,37 @@ def _no_grad(name: str, *tensors) -> None:
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
+class _Last(torch.autograd.Function):
+    """Hands the first n tensors on; a gradient of them is an error."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        ctx.set_materialize_grads(False)
+        return tuple(None if t is None else t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("this operator is differentiable once: its gradient has no gradient of its own")
+
+
+def differentiable_once(backward):
+    """For an autograd function's backward: it runs without a graph, and under create_graph its results refuse a
+    gradient, also where the incoming gradients are constants."""
+
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        single = not isinstance(out, tuple)
+        out = (out,) if single else out
+        out = _Last.apply(len(out), *out, *ctx.saved_tensors, *grads)
+        return out[0] if single else out
+
+    return wrapped
+
+
 class _NormResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, block_out, residual, post_weight, gate, pre_weight, residual_scale, eps, normed_dtype):
@@ -293,6 +325,7 @@ class _NormResidual(torch.autograd.Function):
                                     normed_dtype))
 
     @staticmethod
+    @differentiable_once
     def backward(ctx, *grads):
         block_out, residual, post_weight, gate, pre_weight = ctx.saved_tensors
         grad_normed = grads[1] if len(grads) > 1 else None
@@ -314,7 +347,7 @@ def norm_residual(block_out, residual, *, post_weight=None, gate=None, residual_
     output rounded once. -> (new_residual, normed), (new_residual,) without pre_weight. quantize=True returns
     (new_residual, codes, scale) instead: normed as ``quantize_e4m3_blocks`` would hold it, the operand of the
     block-scaled products. normed_dtype (block_out's dtype by default, else residual's) names normed's type.
-    Differentiable, except with quantize. H <= 16384.
+    Differentiable once, except with quantize. H <= 16384.
     """
     ensure_cuda_device(residual)
     if torch.is_grad_enabled() and _any_grad(block_out, residual, post_weight, gate, pre_weight):
@@ -336,6 +369,7 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, counts, tokens
 
     @staticmethod
+    @differentiable_once
     def backward(ctx, grad_loss, _counts, _tokens):
         logits, counts, tokens, valid = ctx.saved_tensors
         return balance_loss_backward(grad_loss, logits, counts, tokens, *ctx.numbers, valid=valid), None, None, None
@@ -347,7 +381,7 @@ def balance_loss(logits, topk_ids, coefficient: float = 1.0, *, valid=None):
     loss = coefficient * E * sum_e f_e P_e: f_e the share of the chosen slots that went to expert e, P_e the mean
     softmax probability of e, both over the tokens with valid[t] (all without valid); tokens is their number.
     logits [T, E] as ``route_topk`` returns them (or bfloat16/float16), topk_ids [T, k] (negative: no expert).
-    Differentiable in logits; the counts carry no gradient.
+    Differentiable once, in logits; the counts carry no gradient.
     """
     ensure_cuda_device(logits)
     logits, topk_ids = logits.contiguous(), topk_ids.contiguous()

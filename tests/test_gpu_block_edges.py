@@ -65,3 +65,24 @@ def test_rows_of_small_numbers(ops, t, scale):
     else:
         wide = torch.nn.functional.silu(x.double()).abs().max()  # bound: |h| <= (|W| |x|)^2 / 2 over 192 terms of 4 / sqrt h
         assert y.double().abs().max() <= 16 * 448 * i * max(float((8 * wide * math.sqrt(h)) ** 2), 2.0 ** -149 * 448)
+
+
+# ------------------------------------------------------------------ gradients that are not there
+@pytest.mark.parametrize("constant", [False, True])
+def test_second_order_gradients_are_refused(ops, constant):
+    """Under create_graph the gradients refuse one of their own, with incoming gradients that need one and constant
+    ones, and do not drop out of a sum without a word."""
+    v = norm_inputs(6, 64, F32, F32, "channel", True, True, seed=31)
+    leaves = {k: x.clone().requires_grad_(True) for k, x in v.items()}
+    new, z = ops.norm_residual(leaves["y"], leaves["r"], post_weight=leaves["post"], gate=leaves["gate"],
+                               pre_weight=leaves["pre"])
+    first = torch.autograd.grad((new.sum() + z.sum()) if constant else (new * z).sum(), list(leaves.values()),
+                                create_graph=True)
+    for g in first:
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.square().sum() + leaves["r"].square().sum(), leaves["r"], retain_graph=True)
+    logits = randn(9, 8, seed=32).requires_grad_(True)
+    loss, _, _ = ops.balance_loss(logits, logits.detach().topk(2, 1).indices.to(torch.int32))
+    g, = torch.autograd.grad(loss if constant else loss * loss, logits, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g.square().sum() + logits.square().sum()).backward()

@@ -191,3 +191,11 @@ def test_balance_takes_fp32_rows(ops):
     x = randn(30, H, seed=102)
     loss, counts, tokens = block.balance(x)
     assert int(counts.sum()) == K * 30 and int(tokens) == 30 and loss.requires_grad
+
+
+def test_second_order_gradients_are_refused(ops):
+    block = make_block()
+    x = randn(8, H, seed=103, dtype=BF16).requires_grad_(True)
+    g, = torch.autograd.grad(block.experts(x).float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g.float().square().sum() + x.float().square().sum()).backward()
