@@ -327,6 +327,8 @@ class _NormResidual(torch.autograd.Function):
     @staticmethod
     @differentiable_once
     def backward(ctx, *grads):
+        if all(g is None for g in grads):  # its consumers have passed none on
+            return (None,) * 8
         block_out, residual, post_weight, gate, pre_weight = ctx.saved_tensors
         grad_normed = grads[1] if len(grads) > 1 else None
         d = norm_residual_backward(grads[0], grad_normed, block_out, residual, post_weight=post_weight, gate=gate,

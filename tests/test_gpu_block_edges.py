@@ -86,3 +86,22 @@ def test_second_order_gradients_are_refused(ops, constant):
     g, = torch.autograd.grad(loss if constant else loss * loss, logits, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         (g.square().sum() + logits.square().sum()).backward()
+
+
+def test_norm_residual_backward_without_any_gradient(ops):
+    """A consumer without a gradient of its own: the norm's node is reached with none, and passes none on."""
+
+    class Cut(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a):
+            return a.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+
+    r = randn(4, 64, seed=40).requires_grad_(True)
+    y = randn(4, 64, seed=41)
+    new, z = ops.norm_residual(y, r, pre_weight=torch.ones(64, device=DEV))
+    (Cut.apply(new).sum() + Cut.apply(z).sum()).backward()
+    assert r.grad is None
