@@ -12,6 +12,8 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -436,7 +438,25 @@ void check_float_dtype(const Tensor& t, const char* what) {
 }
 int64_t blocks128(int64_t n) { return (n + 127) / 128; }
 
+// These operators have no autograd kernel (below), so a gradient or a tangent that an input asks for would be dropped
+// without a word. The differentiable ones are called under their autograd functions, where grad mode is off.
+void refuse_gradient(const char* op, const Tensor& t) {
+  if (!t.defined()) return;
+  const bool asks = (c10::GradMode::is_enabled() && t.requires_grad()) ||
+                    (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
+  TORCH_CHECK(!asks, op, " has no gradient for its inputs here: call it under torch.no_grad() or on detached tensors, or "
+              "the differentiable function of stageml_b200.ops");
+}
+void refuse_gradient(const char* op, const c10::optional<Tensor>& t) {
+  if (t.has_value()) refuse_gradient(op, *t);
+}
+template <typename... Ts>
+void refuse_gradients(const char* op, const Ts&... tensors) {
+  (refuse_gradient(op, tensors), ...);
+}
+
 std::tuple<Tensor, Tensor> quantize_e4m3_blocks(const Tensor& x, bool tiles) {
+  refuse_gradients("quantize_e4m3_blocks", x);
   check_cuda(x, "x", x);
   check_float_dtype(x, "quantize_e4m3_blocks: x");
   TORCH_CHECK(x.dim() >= (tiles ? 2 : 1), "quantize_e4m3_blocks: x needs at least ", tiles ? 2 : 1, " dims");
@@ -457,6 +477,7 @@ std::tuple<Tensor, Tensor> quantize_e4m3_blocks(const Tensor& x, bool tiles) {
 
 Tensor block_matmul(const Tensor& x, const Tensor& x_scale, const Tensor& w, const Tensor& w_scale,
                     at::ScalarType out_dtype) {
+  refuse_gradients("block_matmul", x, x_scale, w, w_scale);
   check_cuda(x, "x", x);
   check_cuda(x_scale, "x_scale", x);
   check_cuda(w, "w", x);
@@ -486,6 +507,7 @@ Tensor block_matmul(const Tensor& x, const Tensor& x_scale, const Tensor& w, con
 Tensor moe_forward_blocks(const Tensor& x, const Tensor& gate_up, const Tensor& gate_up_scale, const Tensor& down,
                           const Tensor& down_scale, const c10::optional<Tensor>& topk_ids,
                           const c10::optional<Tensor>& topk_weights, int64_t n_shared) {
+  refuse_gradients("moe_forward_blocks", x, gate_up, gate_up_scale, down, down_scale, topk_weights);
   TORCH_CHECK(x.dim() == 2 && gate_up.dim() == 3 && down.dim() == 3, "moe_forward_blocks: x [T, H], gate_up [E, 2I, H], ",
               "down [E, H, I]");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
@@ -619,6 +641,7 @@ std::vector<Tensor> norm_residual(const c10::optional<Tensor>& block_out, const 
                                   const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
                                   const c10::optional<Tensor>& pre_weight, double residual_scale, double eps,
                                   bool quantize, c10::optional<at::ScalarType> normed_dtype) {
+  refuse_gradients("norm_residual", block_out, residual, post_weight, gate, pre_weight);
   const at::ScalarType bd = block_out.has_value()      ? block_out->scalar_type()
                             : normed_dtype.has_value() ? *normed_dtype
                                                        : residual.scalar_type();
@@ -655,6 +678,7 @@ std::vector<Tensor> norm_residual_backward(const c10::optional<Tensor>& grad_res
                                            const c10::optional<Tensor>& block_out, const Tensor& residual,
                                            const c10::optional<Tensor>& post_weight, const c10::optional<Tensor>& gate,
                                            const c10::optional<Tensor>& pre_weight, double residual_scale, double eps) {
+  refuse_gradients("norm_residual_backward", grad_residual, grad_normed, block_out, residual, post_weight, gate, pre_weight);
   TORCH_CHECK(grad_residual.has_value() || grad_normed.has_value(), "norm_residual_backward: no gradient given");
   const at::ScalarType bd = block_out.has_value()     ? block_out->scalar_type()
                             : grad_normed.has_value() ? grad_normed->scalar_type()
@@ -701,6 +725,7 @@ const uint8_t* valid_ptr(const c10::optional<Tensor>& valid, const Tensor& logit
 
 std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& topk_ids, double coefficient,
                                                 const c10::optional<Tensor>& valid) {
+  refuse_gradients("balance_loss", logits);
   check_cuda(logits, "logits", logits);
   check_cuda(topk_ids, "topk_ids", logits);
   check_float_dtype(logits, "balance_loss: logits");
@@ -725,6 +750,7 @@ std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, const Tens
 
 Tensor balance_loss_backward(const Tensor& grad_loss, const Tensor& logits, const Tensor& counts, const Tensor& tokens,
                              int64_t k, double coefficient, const c10::optional<Tensor>& valid) {
+  refuse_gradients("balance_loss_backward", grad_loss, logits);
   check_cuda(logits, "logits", logits);
   check_float_dtype(logits, "balance_loss_backward: logits");
   TORCH_CHECK(logits.dim() == 2, "balance_loss_backward: logits must be [T, E]");
@@ -821,8 +847,8 @@ TORCH_LIBRARY_IMPL(stageml, CUDA, m) {
 }
 
 // The operators above without an autograd formula of their own in the dispatcher: ops.py
-// wraps the differentiable ones in autograd functions and refuses gradients for the others,
-// so the dispatcher's generic autograd kernel (several us per call) is passed by.
+// wraps the differentiable ones in autograd functions, and each refuses gradients and tangents
+// itself, so the dispatcher's generic autograd kernel (several us per call) is passed by.
 TORCH_LIBRARY_IMPL(stageml, Autograd, m) {
   for (const char* op : {"quantize_e4m3_blocks", "block_matmul", "moe_forward_blocks", "norm_residual",
                          "norm_residual_backward", "balance_loss", "balance_loss_backward"})

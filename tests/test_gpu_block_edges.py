@@ -105,3 +105,65 @@ def test_norm_residual_backward_without_any_gradient(ops):
     new, z = ops.norm_residual(y, r, pre_weight=torch.ones(64, device=DEV))
     (Cut.apply(new).sum() + Cut.apply(z).sum()).backward()
     assert r.grad is None
+
+
+def _calls(ops):
+    """(name, call with the tensors of `t`, names of the tensors that could ask for a gradient)"""
+    raw = torch.ops.stageml
+    x, xs = ref_codes(randn(5, 128, seed=33), 1)
+    w, ws = ref_codes(randn(32, 128, seed=34), 128)
+    gu, gus, dn, dns = layer_weights(2, 128, 64, seed=35)
+    ids = torch.tensor([[0, 1]], dtype=torch.int32, device=DEV).repeat(5, 1)
+    logits, counts, tokens = randn(5, 8, seed=36), torch.ones(8, dtype=torch.int32, device=DEV), \
+        torch.full((), 5, dtype=torch.int32, device=DEV)
+    v = norm_inputs(5, 128, F32, F32, "channel", True, True, seed=37)
+    rows = randn(5, 128, seed=38)
+    t = {"x_scale": xs, "w_scale": ws, "gus": gus, "dns": dns, "h": randn(5, 128, seed=39, dtype=BF16),
+         "tw": torch.ones(5, 2, device=DEV), "logits": logits, "rows": rows, "g": torch.ones((), device=DEV), **v}
+    norm = lambda t: (t["y"], t["r"], t["post"], t["gate"], t["pre"])  # noqa: E731
+    kw = lambda t: {"post_weight": t["post"], "gate": t["gate"], "pre_weight": t["pre"]}  # noqa: E731
+    five = ["y", "r", "post", "gate", "pre"]
+    return t, [
+        ("quantize", lambda t: ops.quantize_e4m3_blocks(t["rows"]), ["rows"]),
+        ("matmul", lambda t: ops.block_matmul(x, t["x_scale"], w, t["w_scale"]), ["x_scale", "w_scale"]),
+        ("layer", lambda t: ops.moe_forward_blocks(t["h"], gu, t["gus"], dn, t["dns"], topk_ids=ids, topk_weights=t["tw"]),
+         ["h", "gus", "dns", "tw"]),
+        ("norm backward", lambda t: ops.norm_residual_backward(t["rows"], t["rows"], t["y"], t["r"], **kw(t)),
+         ["rows"] + five),
+        ("balance backward", lambda t: ops.balance_loss_backward(t["g"], t["logits"], counts, tokens, 2), ["g", "logits"]),
+        ("raw quantize", lambda t: raw.quantize_e4m3_blocks(t["rows"], False), ["rows"]),
+        ("raw norm", lambda t: raw.norm_residual(*norm(t), 1.0, 1e-6, False, None), five),
+        ("raw norm backward", lambda t: raw.norm_residual_backward(t["rows"], t["rows"], *norm(t), 1.0, 1e-6), five),
+        ("raw balance", lambda t: raw.balance_loss(t["logits"], ids, 1.0, None), ["logits"]),
+        ("raw balance backward", lambda t: raw.balance_loss_backward(t["g"], t["logits"], counts, tokens, 2, 1.0, None),
+         ["g", "logits"]),
+    ]
+
+
+def test_gradients_that_an_op_does_not_have_are_refused(ops):
+    """Every input that asks for a gradient where there is none, the raw ops' too; without grad mode they run."""
+    t, calls = _calls(ops)
+    for name, call, inputs in calls:
+        call(t)
+        for key in inputs:
+            asking = {**t, key: t[key].clone().requires_grad_(True)}
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(asking)
+            with torch.no_grad():
+                call(asking)
+
+
+def test_tangents_are_refused(ops):
+    import torch.autograd.forward_ad as fwd
+
+    t, calls = _calls(ops)
+    calls += [("norm", lambda t: ops.norm_residual(t["y"], t["r"], post_weight=t["post"], gate=t["gate"],
+                                                   pre_weight=t["pre"]), ["y", "r", "post", "gate", "pre"]),
+              ("balance", lambda t: ops.balance_loss(t["logits"], torch.zeros(5, 2, dtype=torch.int32, device=DEV)),
+               ["logits"])]
+    for name, call, inputs in calls:
+        for key in inputs:
+            with fwd.dual_level():
+                dual = {**t, key: fwd.make_dual(t[key], torch.ones_like(t[key]))}
+                with pytest.raises((RuntimeError, NotImplementedError), match="gradient|forward"):
+                    call(dual)
