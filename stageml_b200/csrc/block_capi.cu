@@ -24,16 +24,21 @@ struct MoeBlocksBuffers {
   size_t bytes = 0;
 };
 
-// At most kSkinnyRows tokens: no expert has more rows than that (a token names an expert once).
-// Four rows per expert or fewer: few experts have more than eight, which would stream their weights
-// again.
-bool moe_blocks_sparse(const stageml_moe_blocks_args* a) { return (int64_t)a->T * a->k <= 4 * (int64_t)a->E; }
+// Streaming products take 8 or 16 rows of a weight group per pass over its weights. 8: four routed rows per
+// expert or fewer, few experts have more than eight (64 experts, six of them and two shared, 16 tokens: 151 us
+// in passes of 8, 174 in passes of 16). Shared experts alone have one row per token: 16.
+bool moe_blocks_sparse(const stageml_moe_blocks_args* a) { return a->k > 0 && (int64_t)a->T * a->k <= 4 * (int64_t)a->E; }
 
-// Streaming products instead of tensor-core tiles. 64 experts of 2048 x 1408, six per token, two
-// shared: 17 tokens in 170 us, 32 in 197, 42 in 210. The tiles take the same time for any number of
-// rows up to 128 per expert (43 to 128 tokens in 194 to 199 us), the streams once more per 8 rows.
+// Streaming products instead of tensor-core tiles, whose time is the same for any number of rows up to
+// 128 per expert: up to kSkinnyRows tokens, and up to two routed rows per expert. 64 experts of 2048 x
+// 1408, two of them, 17, 32, 48, 64 tokens: 94, 130, 146, 156 us streamed, 124, 155, 171, 180 in tiles.
+// A shared expert has a row per token, and its passes come one after the other: with one, 107, 136, 162, 188
+// us streamed, 128, 154, 162, 184 in tiles; with four, 122, 167, 202, 238 and 131, 160, 177, 193. So 32 tokens
+// are the most beside shared experts, and 16 without routed ones (one of 4096 x 14336, 16 and 32 tokens: 75 and
+// 119 us streamed, 99 in tiles).
 bool moe_blocks_skinny(const stageml_moe_blocks_args* a) {
-  return a->T <= kSkinnyRows || (a->T <= 128 && (int64_t)a->T * a->k <= 2 * (int64_t)a->E);
+  if (a->T <= kSkinnyRows) return true;
+  return a->k > 0 && a->T <= (a->n_shared > 0 ? 32 : 128) && (int64_t)a->T * a->k <= 2 * (int64_t)a->E;
 }
 
 void moe_blocks_carve(const stageml_moe_blocks_args* a, void* ws, MoeBlocksBuffers* b) {

@@ -1,0 +1,29 @@
+"""Sizes of the block-scaled operators through the C ABI, without a GPU: workspaces, and which calls are refused."""
+
+import ctypes
+
+import pytest
+
+from stageml_b200 import capi
+from stageml_b200._native import load_capi
+
+P = 4096  # a non-null, 16-byte aligned address; never dereferenced
+
+
+@pytest.mark.parametrize("t,e,k,shared,streams", [
+    (1, 8, 2, 0, True), (16, 8, 2, 0, True), (16, 0, 0, 1, True),  # up to 16 tokens
+    (17, 8, 2, 0, False), (64, 64, 2, 0, True), (65, 64, 2, 0, False), (129, 256, 1, 0, False),  # two rows per expert
+    (17, 0, 0, 1, False), (64, 0, 0, 2, False), (128, 0, 0, 1, False),  # shared experts alone have a row per token
+    (32, 64, 2, 1, True), (33, 64, 2, 1, False), (64, 64, 2, 1, False), (128, 256, 2, 1, False),
+])
+def test_layer_streams_its_weights_for_few_rows_only(t, e, k, shared, streams):
+    """Streaming passes over an expert's weights once per 8 or 16 of its rows, tensor-core tiles once. The workspace
+    shows which one a call takes: only streaming keeps silu(gate) * up in fp32, 4 bytes per row and column."""
+    lib = load_capi()
+    i = 8192
+    a = capi.MoeBlocksArgs(T=t, H=16, I=i, E=e, k=k, n_shared=shared, act_dtype=capi.BF16, ids_dtype=capi.I32,
+                           weights_dtype=capi.F32)
+    need = lib.stageml_moe_blocks_workspace_bytes(ctypes.byref(a))
+    rows = lib.stageml_plan_rows_cap(t * (k + shared), e + shared)
+    assert need > rows * i
+    assert (need > 5 * rows * i) == streams

@@ -67,6 +67,16 @@ def test_rows_of_small_numbers(ops, t, scale):
         assert y.double().abs().max() <= 16 * 448 * i * max(float((8 * wide * math.sqrt(h)) ** 2), 2.0 ** -149 * 448)
 
 
+@pytest.mark.parametrize("t", [17, 32, 64, 128])
+@pytest.mark.parametrize("shared", [1, 3])
+def test_shared_experts_alone(ops, t, shared):
+    h, i = 256, 144
+    gu, gus, dn, dns = layer_weights(shared, h, i, seed=29)
+    x = randn(t, h, seed=30, dtype=BF16)
+    close(ops.moe_forward_blocks(x, gu, gus, dn, dns, n_shared=shared),
+          ref_layer(x, gu, gus, dn, dns, None, None, shared), LAYER_TOL[BF16])
+
+
 # ------------------------------------------------------------------ gradients that are not there
 @pytest.mark.parametrize("constant", [False, True])
 def test_second_order_gradients_are_refused(ops, constant):
