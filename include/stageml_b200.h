@@ -420,7 +420,8 @@ int stageml_moe_forward_blocks(const stageml_moe_blocks_args* args, void* worksp
  * [T, ceil(H/128)] (stageml_quantize_e4m3_blocks of the fp32 z) instead of `normed`.
  * The backward call takes the forward's inputs again (nothing else is saved) with the
  * gradients of r' and z (either may be NULL = zero) and writes the gradients of every
- * input that is present; the weights' and the gate's in their own dtype. H <= 16384. */
+ * input that is present; the weights' and the gate's in their own dtype. H <= 16384.
+ * The workspace query takes the call's own arguments: addresses off 16 bytes can need another size. */
 enum { STAGEML_GATE_NONE = 0, STAGEML_GATE_CHANNEL = 1, STAGEML_GATE_TOKEN = 2, STAGEML_GATE_FULL = 3 };
 typedef struct stageml_norm_args {
   int64_t T;

@@ -883,9 +883,6 @@ int resident_ctas(std::atomic<uint64_t>& last, K kernel, int threads, size_t sme
   return STAGEML_OK;
 }
 
-// The most owners of column sums (workspace): CTAs of at least 64 threads, 2048 threads per SM.
-int max_owners(const stageml_norm_args& a) { return (int)std::min<int64_t>(a.T, (int64_t)sm_count() * 32); }
-
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
 int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStream_t stream) {
   auto kernel = norm_residual_kernel<TR, TY, VEC, V, WARP, RING, STAGED>;
@@ -901,8 +898,9 @@ int run_forward(const stageml_norm_args& a, const Shape& s, float* z32, cudaStre
   return STAGEML_OK;
 }
 
+// With `owners` only its grid, the number of CTAs that each leave a row of column sums.
 template <typename TR, typename TY, int VEC, int V, bool WARP, bool RING, bool STAGED>
-int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cudaStream_t stream) {
+int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, int* owners, cudaStream_t stream) {
   auto kernel = norm_residual_backward_kernel<TR, TY, VEC, V, WARP, RING, STAGED>;
   const int n_sums = n_sums_of(a);
   size_t smem = 0;
@@ -913,6 +911,10 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
   // a warp takes four rows or more, for fewer rows of sums
   const int64_t ctas = WARP ? (a.T + 4 * kWarpRows - 1) / (4 * kWarpRows) : a.T;
   SB_TRY(resident_ctas(resident, kernel, s.threads, smem, ctas, &grid));
+  if (owners) {
+    *owners = grid;
+    return STAGEML_OK;
+  }
   SB_CUDA_CHECK(launch_kernel(kernel, dim3((unsigned)grid), dim3(s.threads), smem, stream, false, a, partial));
   count_launch();
   if (n_sums) {
@@ -925,9 +927,9 @@ int run_backward(const stageml_norm_args& a, const Shape& s, float* partial, cud
 }
 
 template <typename TR, typename TY>
-int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStream_t stream) {
+int dispatch(const stageml_norm_args& a, bool backward, float* scratch, int* owners, cudaStream_t stream) {
 #define SB_NORM(VEC, V, WARP, RING, STAGED, units) \
-  (backward ? run_backward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, stream) \
+  (backward ? run_backward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, owners, stream) \
             : run_forward<TR, TY, VEC, V, WARP, RING, STAGED>(a, shape_of(units, V, WARP), scratch, stream))
   // Few rows run straight from global memory with as many threads per row as possible; more
   // than two rows per SM are worth a CTA's staged factors, and so is one row of the scalar backward,
@@ -958,12 +960,12 @@ int dispatch(const stageml_norm_args& a, bool backward, float* scratch, cudaStre
 #undef SB_NORM
 }
 
-int launch_any(const stageml_norm_args& a, bool backward, float* scratch, cudaStream_t stream) {
-  if (a.resid_dtype == STAGEML_BF16) return dispatch<bf16, bf16>(a, backward, scratch, stream);
-  if (a.resid_dtype == STAGEML_F16) return dispatch<f16, f16>(a, backward, scratch, stream);
-  if (a.block_dtype == STAGEML_BF16) return dispatch<float, bf16>(a, backward, scratch, stream);
-  if (a.block_dtype == STAGEML_F16) return dispatch<float, f16>(a, backward, scratch, stream);
-  return dispatch<float, float>(a, backward, scratch, stream);
+int launch_any(const stageml_norm_args& a, bool backward, float* scratch, int* owners, cudaStream_t stream) {
+  if (a.resid_dtype == STAGEML_BF16) return dispatch<bf16, bf16>(a, backward, scratch, owners, stream);
+  if (a.resid_dtype == STAGEML_F16) return dispatch<f16, f16>(a, backward, scratch, owners, stream);
+  if (a.block_dtype == STAGEML_BF16) return dispatch<float, bf16>(a, backward, scratch, owners, stream);
+  if (a.block_dtype == STAGEML_F16) return dispatch<float, f16>(a, backward, scratch, owners, stream);
+  return dispatch<float, float>(a, backward, scratch, owners, stream);
 }
 
 }  // namespace
@@ -978,14 +980,21 @@ size_t norm_residual_scratch(const stageml_norm_args& a) {
 int launch_norm_residual(const stageml_norm_args& a, void* scratch, cudaStream_t stream) {
   if (a.T == 0) return STAGEML_OK;
   const bool two_step = a.codes && !vectors(a);
-  SB_TRY(launch_any(a, false, two_step ? static_cast<float*>(scratch) : nullptr, stream));
+  SB_TRY(launch_any(a, false, two_step ? static_cast<float*>(scratch) : nullptr, nullptr, stream));
   if (two_step)
     return launch_quantize_block_rows(scratch, STAGEML_F32, a.T, a.H, nullptr, 0, a.codes, a.code_scale, stream);
   return STAGEML_OK;
 }
 
 size_t norm_residual_backward_scratch(const stageml_norm_args& a) {
-  return (size_t)max_owners(a) * n_sums_of(a) * a.H * 4;
+  if (a.T == 0 || n_sums_of(a) == 0) return 0;
+  int owners = 0;
+  if (launch_any(a, true, nullptr, &owners, nullptr) != STAGEML_OK) {
+    // no device to ask: 32 CTAs of 64 threads fill an SM
+    clear_error();
+    owners = (int)std::min<int64_t>(a.T, (int64_t)sm_count() * 32);
+  }
+  return (size_t)owners * n_sums_of(a) * a.H * 4;
 }
 
 int launch_norm_residual_backward(const stageml_norm_args& a, void* scratch, cudaStream_t stream) {
@@ -997,7 +1006,7 @@ int launch_norm_residual_backward(const stageml_norm_args& a, void* scratch, cud
     if (a.pre_weight) SB_CUDA_CHECK(cudaMemsetAsync(a.d_pre, 0, a.H * es[a.pre_dtype], stream));
     return STAGEML_OK;
   }
-  return launch_any(a, true, static_cast<float*>(scratch), stream);
+  return launch_any(a, true, static_cast<float*>(scratch), nullptr, stream);
 }
 
 }  // namespace sb

@@ -177,3 +177,17 @@ def test_tangents_are_refused(ops):
                 dual = {**t, key: fwd.make_dual(t[key], torch.ones_like(t[key]))}
                 with pytest.raises((RuntimeError, NotImplementedError), match="gradient|forward"):
                     call(dual)
+
+
+# ------------------------------------------------------------------ sizes
+def test_norm_workspace_is_the_launched_grid(ops):
+    """The backward's partial sums: one row per CTA of the launch, of which no SM holds more than four here."""
+    v = norm_inputs(8192, 4096, BF16, BF16, "channel", True, True, wd=BF16, seed=45)
+    g = randn(8192, 4096, seed=46, dtype=BF16)
+    torch.cuda.synchronize()
+    kept = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    d = ops.norm_residual_backward(g, g, v["y"], v["r"], post_weight=v["post"], gate=v["gate"], pre_weight=v["pre"])
+    outputs = sum(t.numel() * t.element_size() for t in d if t is not None)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert torch.cuda.max_memory_allocated() - kept - outputs <= 4 * sms * 2 * 4096 * 4 + (1 << 20)
