@@ -106,15 +106,16 @@ __global__ void __launch_bounds__(256) quantize_block_rows_kernel(const T* __res
   const int64_t step = (int64_t)gridDim.x * 16;
   for (int64_t u0 = (int64_t)blockIdx.x * 16; u0 < units; u0 += step * kUnits) {
     Vals8<T> v[kUnits];
-    uint32_t row[kUnits], col[kUnits];
+    uint32_t row[kUnits], blk[kUnits];  // the column, 128 blk + 8 sub, can pass 32 bits
+    auto col = [&](int i) { return (int64_t)blk[i] * 128 + sub * 8; };
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const int64_t u = u0 + i * step + half;
       v[i].zero();
       if (u >= units) continue;
       row[i] = (uint32_t)u / nb;
-      col[i] = ((uint32_t)u - row[i] * nb) * 128 + sub * 8;
-      load_cols<T, VEC>(x + row[i] * cols, col[i], cols, v[i]);
+      blk[i] = (uint32_t)u - row[i] * nb;
+      load_cols<T, VEC>(x + row[i] * cols, col(i), cols, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
@@ -123,14 +124,14 @@ __global__ void __launch_bounds__(256) quantize_block_rows_kernel(const T* __res
       const BlockScale s(m);
       const uint2 code = v[i].encode(s);
       if (slots == 0) {
-        store_codes<VEC>(q + row[i] * cols, col[i], cols, code);
-        if (sub == 0) scale[(int64_t)row[i] * nb + (col[i] >> 7)] = s.s;
+        store_codes<VEC>(q + row[i] * cols, col(i), cols, code);
+        if (sub == 0) scale[(int64_t)row[i] * nb + blk[i]] = s.s;
       } else {
         for (int j = 0; j < slots; ++j) {
           const int64_t d = out_row[(int64_t)row[i] * slots + j];
           if (d < 0) continue;
-          store_codes<VEC>(q + d * cols, col[i], cols, code);
-          if (sub == 0) scale[d * nb + (col[i] >> 7)] = s.s;
+          store_codes<VEC>(q + d * cols, col(i), cols, code);
+          if (sub == 0) scale[d * nb + blk[i]] = s.s;
         }
       }
     }

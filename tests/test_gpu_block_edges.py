@@ -180,6 +180,19 @@ def test_tangents_are_refused(ops):
 
 
 # ------------------------------------------------------------------ sizes
+def test_quantize_columns_past_32_bits(ops):
+    cols = (1 << 32) + 1000 + 3  # not a multiple of 8 or 128: the kernel that keeps a row and a column index
+    x = torch.zeros(1, cols, device=DEV, dtype=BF16)
+    x[0, :512] = randn(512, seed=42, dtype=BF16)
+    x[0, -1003:] = randn(1003, seed=43, dtype=BF16)
+    q, s = ops.quantize_e4m3_blocks(x)
+    first = (cols - 1003) // 128 * 128
+    for lo, hi in ((0, 512), (first, cols)):
+        rq, rs = ref_codes(x[:, lo:hi], 1)
+        assert torch.equal(s[:, lo // 128: lo // 128 + blocks(hi - lo)], rs)
+        assert torch.equal(q[:, lo:hi].contiguous().view(torch.uint8), rq.view(torch.uint8))
+
+
 def test_norm_workspace_is_the_launched_grid(ops):
     """The backward's partial sums: one row per CTA of the launch, of which no SM holds more than four here."""
     v = norm_inputs(8192, 4096, BF16, BF16, "channel", True, True, wd=BF16, seed=45)
