@@ -10,6 +10,9 @@ namespace {
 
 inline bool is_float(int dtype) { return dtype == STAGEML_F32 || is16(dtype); }
 
+// The products round M and N up to whole tiles, and K up to a whole turn of a CTA's warps (4096 values), in 32 bits.
+constexpr int kMaxSize = 0x7fffffff - 8191;
+
 // ------------------------------------------------------------------ MoE layer
 struct MoeBlocksBuffers {
   stageml_moe_plan plan{};
@@ -66,6 +69,7 @@ int moe_blocks_validate(const stageml_moe_blocks_args* a, bool check_ptrs) {
   SB_CHECK_ARG(a->k <= a->E && a->k <= 8, "moe_blocks: k=%d must be <= min(E, 8)", a->k);
   SB_CHECK_ARG(a->k > 0 || a->E == 0, "moe_blocks: E=%d routed experts with k = 0", a->E);
   SB_CHECK_ARG(a->H % 16 == 0 && a->I % 16 == 0, "moe_blocks: H=%d and I=%d must be multiples of 16", a->H, a->I);
+  SB_CHECK_ARG(a->H <= kMaxSize && a->I <= kMaxSize, "moe_blocks: H=%d and I=%d: at most 2^31 - 8192", a->H, a->I);
   SB_CHECK_ARG((int64_t)(a->E + a->n_shared) * 2 * a->I <= 0x7fffffff && (int64_t)(a->E + a->n_shared) * a->H <= 0x7fffffff,
                "moe_blocks: too many weight rows");
   SB_CHECK_ARG(a->E + a->n_shared <= block_gemm_max_groups(), "moe_blocks: %d experts exceed %d", a->E + a->n_shared,
@@ -233,6 +237,8 @@ int stageml_block_matmul(const uint8_t* x, const float* x_scale, const uint8_t* 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   SB_CHECK_ARG(M >= 0 && N >= 0 && K >= 1, "block_matmul: bad sizes M=%d N=%d K=%d", M, N, K);
   SB_CHECK_ARG(K % 16 == 0, "block_matmul: K=%d must be a multiple of 16", K);
+  SB_CHECK_ARG(M <= kMaxSize && N <= kMaxSize && K <= kMaxSize, "block_matmul: M=%d, N=%d, K=%d: at most 2^31 - 8192", M,
+               N, K);
   SB_CHECK_ARG(is_float(out_dtype), "block_matmul: out_dtype must be F32, BF16 or F16");
   if (M == 0 || N == 0) return STAGEML_OK;
   SB_CHECK_ARG(x && x_scale && w && w_scale && out, "block_matmul: null pointer");

@@ -27,3 +27,15 @@ def test_layer_streams_its_weights_for_few_rows_only(t, e, k, shared, streams):
     rows = lib.stageml_plan_rows_cap(t * (k + shared), e + shared)
     assert need > rows * i
     assert (need > 5 * rows * i) == streams
+
+
+@pytest.mark.parametrize("m,n,k", [(0x7fffffff, 16, 16), (1, 0x7fffffff, 16), (64, 0x7fffff80, 16), (64, 64, 0x7ffffff0),
+                                   (1, 16, 0x7fffffff - 4095), (64, 16, 0x7fffffff - 4095)])
+def test_products_whose_rounded_sizes_pass_32_bits_are_refused(m, n, k):
+    lib = load_capi()
+    assert lib.stageml_block_matmul(P, P, P, P, m, n, k, capi.BF16, P, None, None) == capi.ERR_INVALID_ARG
+    assert "2^31" in lib.stageml_last_error().decode()
+    a = capi.MoeBlocksArgs(T=1, H=0x7fffffff - 4095, I=16, E=1, k=1, act_dtype=capi.BF16, ids_dtype=capi.I32,
+                           weights_dtype=capi.F32)
+    assert lib.stageml_moe_blocks_workspace_bytes(ctypes.byref(a)) == 0
+    assert "2^31" in lib.stageml_last_error().decode()
