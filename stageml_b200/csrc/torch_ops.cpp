@@ -518,6 +518,8 @@ Tensor moe_forward_blocks(const Tensor& x, const Tensor& gate_up, const Tensor& 
   TORCH_CHECK(gate_up.size(1) % 2 == 0 && gate_up.size(2) == H && down.size(0) == E_tot && down.size(1) == H &&
                   down.size(2) == I,
               "moe_forward_blocks: weight shapes do not match x");
+  TORCH_CHECK(T <= INT32_MAX && H <= INT32_MAX && I <= INT32_MAX && E_tot <= INT32_MAX,
+              "moe_forward_blocks: sizes past 2^31");
   TORCH_CHECK(n_shared >= 0 && n_shared <= E_tot, "moe_forward_blocks: n_shared out of range");
   TORCH_CHECK(gate_up_scale.scalar_type() == at::kFloat &&
                   gate_up_scale.sizes() == at::IntArrayRef({E_tot, blocks128(2 * I), blocks128(H)}),
@@ -759,6 +761,7 @@ Tensor balance_loss_backward(const Tensor& grad_loss, const Tensor& logits, cons
   TORCH_CHECK(counts.scalar_type() == at::kInt && counts.numel() == logits.size(1) &&
                   tokens.scalar_type() == at::kInt && tokens.numel() == 1,
               "balance_loss_backward: counts int32 [E] and tokens int32 [1] of the forward");
+  TORCH_CHECK(k >= 1 && k <= 8, "balance_loss_backward: k=", k, " must be in 1..8");
   const uint8_t* v = valid_ptr(valid, logits);
   c10::cuda::CUDAGuard guard(logits.device());
   auto grad = fresh(logits.sizes(), logits.scalar_type(), logits);

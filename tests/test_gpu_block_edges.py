@@ -193,6 +193,14 @@ def test_quantize_columns_past_32_bits(ops):
         assert torch.equal(q[:, lo:hi].contiguous().view(torch.uint8), rq.view(torch.uint8))
 
 
+def test_balance_backward_refuses_a_k_past_its_range(ops):
+    logits = randn(4, 8, seed=44)
+    _, counts, tokens = ops.balance_loss(logits, logits.topk(2, 1).indices.to(torch.int32))
+    for k in (0, 9, -1, (1 << 32) + 2):
+        with pytest.raises(RuntimeError, match="k="):
+            ops.balance_loss_backward(torch.ones((), device=DEV), logits, counts, tokens, k)
+
+
 def test_norm_workspace_is_the_launched_grid(ops):
     """The backward's partial sums: one row per CTA of the launch, of which no SM holds more than four here."""
     v = norm_inputs(8192, 4096, BF16, BF16, "channel", True, True, wd=BF16, seed=45)
