@@ -560,7 +560,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         // a thread's 64 columns of h from its 64 gate and 64 up sums, or 32 of a narrow unit
         const int n0 = w.n * 128 + 64 * half + 32 * side;
         uint32_t m = 0;
-        auto activate = [&](auto width) {  // h takes the gate values' place
+        // h takes the gate values' place. The quotient within 2 ulp of fp32, 2^-18 of the e4m3 step that follows: the
+        // correctly rounded division, which the streaming kernel has, spills here (Mixtral-shape layer, 2048 tokens:
+        // 1.28 ms, from 1.13). Below gate = -87.3 it gives 0 for less than 1.1e-36 of up.
+        auto activate = [&](auto width) {
           constexpr int COLS = decltype(width)::value / 2;
 #pragma unroll
           for (int i = 0; i < COLS; ++i) {
