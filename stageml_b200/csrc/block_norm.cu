@@ -362,20 +362,23 @@ struct RowRing {
   uint8_t* base;
   uint32_t stage_bytes;
   uint64_t* full;          // [STAGES]
-  volatile int* abort_flag;
+  volatile int* abort_flag;  // [2]: a wait has run out; rows whose copies have been issued
   int32_t* status;
 
   __device__ void init(uint8_t* smem, uint32_t bytes, uint64_t* bars, int* flag, int32_t* st) {
     base = smem, stage_bytes = bytes, full = bars, abort_flag = flag, status = st;
     if (threadIdx.x == 0) {
       for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&full[i]), 1);
-      *flag = 0;
+      flag[0] = flag[1] = 0;
       fence_barrier_init();
     }
     __syncthreads();
   }
-  // The copies of the n-th row of this CTA (thread 0); null sources are left out.
+  // The copies of the n-th row of this CTA (thread 0); null sources are left out. None after a wait has run out:
+  // the stage may still be the target of earlier ones.
   __device__ void fill(uint32_t n, const void* const (&src)[4], const uint32_t (&bytes)[4]) {
+    if (abort_flag[0]) return;
+    abort_flag[1] = (int)n + 1;
     fence_proxy_async_smem();  // the stage's reads (ordered by the caller's barrier) come first
     const uint32_t bar = smem_u32(&full[n % STAGES]);
     uint32_t dst = smem_u32(base) + n % STAGES * stage_bytes, total = 0;
@@ -395,6 +398,15 @@ struct RowRing {
               kDevTimeoutProducer);
     return smem_u32(base) + n % STAGES * stage_bytes;
   }
+  // After the last row (thread 0): if a wait has run out, copies may still be on their way into this CTA's shared
+  // memory; it does not leave before they have landed, or as much time has passed again.
+  __device__ void drain() {
+    if (!abort_flag[0]) return;
+    volatile int never = 0;
+    const uint32_t issued = (uint32_t)abort_flag[1];
+    for (uint32_t n = issued > STAGES ? issued - STAGES : 0; n < issued; ++n)
+      mbar_wait(smem_u32(&full[n % STAGES]), (n / STAGES) & 1, &never, status, kDefaultWaitNs, kDevTimeoutDrain);
+  }
 };
 
 // Without a ring every input of a row is loaded before its first sum, while the values fit in
@@ -409,7 +421,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
   __shared__ uint64_t bars[STAGES];
-  __shared__ int flag;
+  __shared__ int flag[2];
   int phase = 0;
   const int nt = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
   const int H = a.H;
@@ -427,7 +439,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
     ring.fill(n, src, bytes);
   };
   if constexpr (RING) {
-    ring.init(row_smem, r_bytes + y_bytes, bars, &flag, a.status);
+    ring.init(row_smem, r_bytes + y_bytes, bars, flag, a.status);
     if (threadIdx.x == 0)
       for (int i = 0; i < STAGES; ++i) fill(i);
   }
@@ -544,6 +556,8 @@ __global__ void __launch_bounds__(kMaxThreads) norm_residual_kernel(const stagem
       }
     }
   }
+  if constexpr (RING)
+    if (threadIdx.x == 0) ring.drain();
 }
 
 // Column sums that the backward keeps: S (for the post weight and a per-channel gate), dw_pre.
@@ -562,7 +576,7 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
   __shared__ uint64_t bars[STAGES];
-  __shared__ int flag;
+  __shared__ int flag[2];
   int phase = 0;
   const int nt = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
   const int H = a.H;
@@ -584,7 +598,7 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
     ring.fill(n, src, bytes);
   };
   if constexpr (RING) {
-    ring.init(row_smem, 2 * (r_bytes + y_bytes), bars, &flag, a.status);
+    ring.init(row_smem, 2 * (r_bytes + y_bytes), bars, flag, a.status);
     if (threadIdx.x == 0)
       for (int i = 0; i < STAGES; ++i) fill(i);
   }
@@ -771,6 +785,8 @@ __global__ void __launch_bounds__(kMaxThreads, (RING && V == 1) || (!RING && V *
       store_vals<VEC>(static_cast<TY*>(a.d_block_out) + base + c, t);
     }
   }
+  if constexpr (RING)
+    if (threadIdx.x == 0) ring.drain();
   if (n_sums_of(a) == 0) return;
   float* out = partial + (int64_t)blockIdx.x * n_sums_of(a) * H;
   if constexpr (WARP) {
