@@ -212,3 +212,77 @@ def test_norm_workspace_is_the_launched_grid(ops):
     outputs = sum(t.numel() * t.element_size() for t in d if t is not None)
     sms = torch.cuda.get_device_properties(0).multi_processor_count
     assert torch.cuda.max_memory_allocated() - kept - outputs <= 4 * sms * 2 * 4096 * 4 + (1 << 20)
+
+
+# ------------------------------------------------------------------ tracing, streams
+def test_fake_implementations_match(ops):
+    """Under a fake tensor mode each op gives what it really gives: shapes, types, strides."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    raw = torch.ops.stageml
+    x, xs = ref_codes(randn(5, 200, seed=50), 1)
+    w, ws = ref_codes(randn(130, 200, seed=51), 128)
+    x, w = x[:, :192].contiguous(), w[:, :192].contiguous()
+    gu, gus, dn, dns = layer_weights(3, 144, 80, seed=52)
+    ids = torch.tensor([[0, 1]], dtype=torch.int32, device=DEV).repeat(5, 1)
+    rows, wide = randn(5, 144, seed=53, dtype=BF16), randn(3, 5, 300, seed=54, dtype=BF16)
+    v = norm_inputs(5, 300, F32, BF16, "token", True, True, seed=55)
+    norm = (v["y"], v["r"], v["post"], v["gate"], v["pre"])
+    bare = (None, v["r"], None, None, v["pre"])
+    dr, dz = randn(5, 300, seed=56), randn(5, 300, seed=57, dtype=BF16)
+    logits = randn(5, 9, seed=58, dtype=F16)
+    counts, tokens = torch.ones(9, dtype=torch.int32, device=DEV), torch.full((), 5, dtype=torch.int32, device=DEV)
+    calls = [
+        (raw.quantize_e4m3_blocks, (wide, False)), (raw.quantize_e4m3_blocks, (wide, True)),
+        (raw.quantize_e4m3_blocks, (wide[0, 0], False)),
+        (raw.block_matmul, (x, xs, w, ws, F16)), (raw.block_matmul, (x, xs, w, ws, F32)),
+        (raw.moe_forward_blocks, (rows, gu, gus, dn, dns, ids, torch.ones(5, 2, device=DEV), 1)),
+        (raw.moe_forward_blocks, (rows, gu, gus, dn, dns, None, None, 3)),
+        (raw.norm_residual, (*norm, 0.5, 1e-6, False, None)), (raw.norm_residual, (*norm, 0.5, 1e-6, True, BF16)),
+        (raw.norm_residual, (*bare, 1.0, 1e-6, False, F16)), (raw.norm_residual, (*bare, 1.0, 1e-6, False, None)),
+        (raw.norm_residual, (v["y"], v["r"], None, None, None, 1.0, 1e-6, False, None)),
+        (raw.norm_residual, (v["y"].t().contiguous().t(), v["r"].t().contiguous().t(), None, None, v["pre"], 1.0, 1e-6,
+                             False, None)),
+        (raw.norm_residual_backward, (dr, dz, *norm, 0.5, 1e-6)),
+        (raw.norm_residual_backward, (dr, None, *bare, 0.5, 1e-6)),
+        (raw.balance_loss, (logits, ids, 0.1, None)),
+        (raw.balance_loss_backward, (torch.ones((), device=DEV), logits, counts, tokens, 2, 0.1, None)),
+    ]
+    for op, args in calls:
+        real = op(*args)
+        with FakeTensorMode() as mode:
+            fake = op(*[mode.from_tensor(a) if isinstance(a, torch.Tensor) else a for a in args])
+        real, fake = ([o] if isinstance(o, torch.Tensor) else list(o) for o in (real, fake))
+        assert len(real) == len(fake)
+        for a, b in zip(real, fake):
+            assert (a.shape, a.dtype, a.device, a.stride()) == (b.shape, b.dtype, b.device, b.stride()), op
+
+
+def test_products_on_two_streams_at_once(ops):
+    """The tile kernels of two streams share the device and nothing else: the bits of each alone."""
+    small, large = [], []
+    for m, n, k in ((64, 4096, 4096), (300, 1000, 2048)):  # several CTA pairs to a tile
+        xs = ref_codes(randn(m, k, seed=m), 1)
+        small.append((*xs, *ref_codes(randn(n, k, seed=n, scale=k ** -0.5), 128)))
+    m, n, k = 1500, 2824, 1424
+    large.append((*ref_codes(randn(m, k, seed=m), 1), *ref_codes(randn(n, k, seed=n, scale=k ** -0.5), 128)))
+    gu, gus, dn, dns = layer_weights(6, 256, 208, seed=60)
+    x = randn(700, 256, seed=61, dtype=BF16)
+    top = randn(700, 6, seed=62).topk(3, 1)
+    ids, w = top.indices.to(torch.int32), top.values.softmax(1)
+    work = [lambda: [ops.block_matmul(*o, out_dtype=F32) for o in small],
+            lambda: [ops.block_matmul(*o) for o in large] +
+                    [ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w)]]
+    want = [f() for f in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[], []]
+    for _ in range(20):
+        for s, f, g in zip(streams, work, got):
+            with torch.cuda.stream(s):
+                g.append(f())
+    torch.cuda.synchronize()
+    for g, ref in zip(got, want):
+        for outs in g:
+            for a, b in zip(outs, ref):
+                assert torch.equal(a, b)
