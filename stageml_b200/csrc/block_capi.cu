@@ -152,8 +152,8 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   g.out = b.y;
   g.out_dtype = STAGEML_F32;
   SB_STAGE(STAGEML_STAGE_GEMM_DOWN, skinny ? launch_block_skinny(g, sk, st) : launch_block_gemm(g, st));
-  SB_STAGE(STAGEML_STAGE_COMBINE, launch_combine(b.y, b.plan.pair_row, a->T, slots, a->H,
-                                                 a->act_dtype == STAGEML_BF16, a->out, st, nullptr, pdl, true));
+  SB_STAGE(STAGEML_STAGE_COMBINE, launch_combine_f32(b.y, b.plan.pair_row, a->T, slots, a->H,
+                                                     a->act_dtype == STAGEML_BF16, a->out, st, pdl));
   return STAGEML_OK;
 }
 

@@ -24,32 +24,24 @@ struct BlockScale {
     r = __frcp_rn(s);
     fast = s > 8.0779357e-28f && s < 1.2379400e27f;
   }
-  enum Quotient { kDivide, kExact, kNear };
-  template <Quotient Q>
+  template <bool FAST>
   __device__ __forceinline__ float quotient(float v) const {
-    if (Q == kDivide) return v / s;
+    if (!FAST) return v / s;
     const float q0 = v * r;
-    return Q == kNear ? q0 : fmaf(fmaf(-q0, s, v), r, q0);
+    return fmaf(fmaf(-q0, s, v), r, q0);
   }
-  // four values to four codes (a NaN's sign is lost)
-  template <Quotient Q>
+  // four magnitudes to four codes without their signs
+  template <bool FAST>
   __device__ __forceinline__ uint32_t encode4(const float* f) const {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(quotient<Q>(f[0]), quotient<Q>(f[1])), __NV_SATFINITE,
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(quotient<FAST>(f[0]), quotient<FAST>(f[1])), __NV_SATFINITE,
                                                  __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(quotient<Q>(f[2]), quotient<Q>(f[3])), __NV_SATFINITE,
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(quotient<FAST>(f[2]), quotient<FAST>(f[3])), __NV_SATFINITE,
                                                  __NV_E4M3);
     return lo | hi << 16;
   }
-  // eight values
+  // eight magnitudes
   __device__ __forceinline__ uint2 encode8(const float (&f)[8]) const {
-    return fast ? make_uint2(encode4<kExact>(f), encode4<kExact>(f + 4))
-                : make_uint2(encode4<kDivide>(f), encode4<kDivide>(f + 4));
-  }
-  // Eight values that are sums of fp32 products, with rounding errors of their own: the product with the reciprocal
-  // is within 2 ulp of fp32 of the quotient, 2^-19 of an e4m3 step, and saves two operations per value.
-  __device__ __forceinline__ uint2 encode8_near(const float (&f)[8]) const {
-    return fast ? make_uint2(encode4<kNear>(f), encode4<kNear>(f + 4))
-                : make_uint2(encode4<kDivide>(f), encode4<kDivide>(f + 4));
+    return fast ? make_uint2(encode4<true>(f), encode4<true>(f + 4)) : make_uint2(encode4<false>(f), encode4<false>(f + 4));
   }
   __device__ __forceinline__ uint2 encode_signed8(const float (&f)[8]) const {
     float m[8];

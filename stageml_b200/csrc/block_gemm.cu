@@ -41,7 +41,6 @@
 // Every wait is bounded. No load is multicast.
 #include <atomic>
 
-#include "block_codes.cuh"
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -586,15 +585,31 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!ok) break;
         m = max(m, maxima[(half ^ 1) * BM + row_in_tile]);
         if (narrow) m = max(m, max(maxima[row_in_tile ^ 64], maxima[BM + (row_in_tile ^ 64)]));
-        // the quantizer's range test matters here too: rows of small numbers make an h whose scale has no finite
-        // reciprocal
-        const BlockScale s(m);
+        // h never leaves in another form, so its codes may come from the reciprocal: the quotient is within
+        // 2 ulp of fp32, 2^-19 of an e4m3 step. A scale without a finite or normal reciprocal (rows of small
+        // numbers) is moved by a power of two, with its row, first.
+        float s = __uint_as_float(m) / 448.0f;
+        s = s == 0.f ? 1.f : s;
+        const float shift = s < 0x1p-100f ? 0x1p100f : s > 0x1p100f ? 0x1p-100f : 1.f;
+        if (shift != 1.f) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) acc[i] *= shift;
+        }
+        const float inv = 1.f / (s * shift);
         uint4 codes[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint2 lo = s.encode8_near(*reinterpret_cast<const float(*)[8]>(acc + 16 * c));
-          const uint2 hi = s.encode8_near(*reinterpret_cast<const float(*)[8]>(acc + 16 * c + 8));
-          codes[c] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* f = acc + 16 * c + 4 * i;
+            const uint32_t lo =
+                __nv_cvt_float2_to_fp8x2(make_float2(f[0] * inv, f[1] * inv), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi =
+                __nv_cvt_float2_to_fp8x2(make_float2(f[2] * inv, f[3] * inv), __NV_SATFINITE, __NV_E4M3);
+            v[i] = lo | hi << 16;
+          }
+          codes[c] = make_uint4(v[0], v[1], v[2], v[3]);
         }
         if (narrow) {
           if (row_ok) {
@@ -612,7 +627,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (r < rows4) *reinterpret_cast<uint4*>(q + (int64_t)r * p.N) = codes[r];
           }
         }
-        if (row_ok && half == 0 && side == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s.s;
+        if (row_ok && half == 0 && side == 0) p.q_scale[row * ((p.N + 127) / 128) + w.n] = s;
       } else {
         const int n0 = w.n * BN + 128 * half + 64 * side;
         float* turn = turns + (warp - MATH_WARP0) * 32 * TURN_PITCH;

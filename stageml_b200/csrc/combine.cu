@@ -2,8 +2,7 @@
 // routing weight already applied by the down-projection epilogue. This is the
 // out.index_add_(0, index, y * gates) of RequestExecutor.dynamic_one
 // (benchmarks/multitenant_bta_system_bench.py:413) done once per token with a
-// fixed slot order (fp32 sum, one rounding), so it is deterministic. Y is in the
-// output's 16-bit type or in fp32 (TY).
+// fixed slot order (fp32 sum, one rounding), so it is deterministic.
 #include "common.cuh"
 #include "host_util.h"
 #include "kernels.h"
@@ -11,8 +10,8 @@
 namespace sb {
 namespace {
 
-template <typename TY, typename T>
-__global__ void combine_kernel(const TY* __restrict__ y, const int32_t* __restrict__ pair_row, int T_, int kk, int H,
+template <typename T>
+__global__ void combine_kernel(const T* __restrict__ y, const int32_t* __restrict__ pair_row, int T_, int kk, int H,
                                T* __restrict__ out, const int32_t* __restrict__ T_dev, int t_base) {
   pdl_wait();  // y comes from the previous kernel
   const int t = blockIdx.y;
@@ -25,18 +24,41 @@ __global__ void combine_kernel(const TY* __restrict__ y, const int32_t* __restri
   for (int j = 0; j < kk; ++j) {
     const int row = pair_row[(int64_t)t * kk + j];
     if (row < 0) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(y + (int64_t)row * H + c);
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(y + (int64_t)row * H + c));
     float f[8];
-    if constexpr (sizeof(TY) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else {
-      unpack8<T>(__ldg(src), f);
-    }
+    unpack8<T>(u, f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] += f[i];
   }
   *reinterpret_cast<uint4*>(out + (int64_t)t * H + c) = pack8<T>(acc);
+}
+
+// The same from fp32 rows, 4 columns per thread: a warp's load is 512 bytes in a row, and up to eight slots' loads
+// are on their way at once (4096 tokens of 2048 columns, eight slots each: 104 us with one 8-column slot at a time).
+template <typename T>
+__global__ void combine_f32_kernel(const float* __restrict__ y, const int32_t* __restrict__ pair_row, int T_, int kk, int H,
+                                   T* __restrict__ out) {
+  constexpr int kSlots = 8;
+  pdl_wait();  // y comes from the previous kernel
+  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
+  if (c >= H) return;
+  for (int t = blockIdx.y; t < T_; t += gridDim.y) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < kk; j0 += kSlots) {
+      float4 v[kSlots];
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        const int row = j0 + j < kk ? __ldg(pair_row + (int64_t)t * kk + j0 + j) : -1;
+        v[j] = row >= 0 ? __ldg(reinterpret_cast<const float4*>(y + (int64_t)row * H + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) acc[0] += v[j].x, acc[1] += v[j].y, acc[2] += v[j].z, acc[3] += v[j].w;
+    }
+    T h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = from_f32<T>(acc[i]);
+    *reinterpret_cast<uint2*>(out + (int64_t)t * H + c) = *reinterpret_cast<const uint2*>(h);
+  }
 }
 
 __global__ void validate_tenants_kernel(const int32_t* __restrict__ in, int64_t n, int n_tenants,
@@ -88,24 +110,6 @@ __global__ void direct_rows_kernel(const void* __restrict__ ids, int ids_i64, co
   row_scale[t] = bad ? 0.f : w;
 }
 
-// Tokens are the grid's second dimension; more than it takes go in several launches, the first of which may be
-// programmatic.
-template <typename TY, typename T>
-int run_combine(const void* y, const int32_t* pair_row, int T_, int kk, int H, void* out, cudaStream_t stream,
-                const int32_t* T_dev, bool pdl) {
-  constexpr int kMaxGridY = 65535;
-  const dim3 block(128);
-  for (int t0 = 0; t0 < T_; t0 += kMaxGridY) {
-    const int nt = std::min(kMaxGridY, T_ - t0);
-    const dim3 grid((unsigned)((H / 8 + block.x - 1) / block.x), (unsigned)nt);
-    SB_CUDA_CHECK(launch_kernel(combine_kernel<TY, T>, grid, block, 0, stream, pdl && t0 == 0, static_cast<const TY*>(y),
-                                pair_row + (int64_t)t0 * kk, nt, kk, H, static_cast<T*>(out) + (int64_t)t0 * H, T_dev, t0));
-    ::sb::count_launch();
-  }
-  SB_CUDA_CHECK(cudaGetLastError());
-  return STAGEML_OK;
-}
-
 }  // namespace
 
 int launch_direct_rows(const void* ids, int ids_dtype, const void* weights, int weights_dtype, const int32_t* tenant_ids,
@@ -121,15 +125,52 @@ int launch_direct_rows(const void* ids, int ids_dtype, const void* weights, int 
 }
 
 int launch_combine(const void* y, const int32_t* pair_row, int T_, int kk, int H, int dtype_bf16, void* out,
-                   cudaStream_t stream, const int32_t* T_dev, bool pdl, bool y_f32) {
+                   cudaStream_t stream, const int32_t* T_dev, bool pdl) {
   SB_CHECK_ARG(H % 8 == 0, "combine: H=%d must be a multiple of 8", H);
   if (T_ == 0 || H == 0) return STAGEML_OK;
+  dim3 block(128);
+  dim3 grid((unsigned)((H / 8 + block.x - 1) / block.x), (unsigned)T_);
   SB_CHECK_ARG(T_ <= 65535 * 64, "combine: too many tokens");
+  if (grid.y > 65535) {
+    // split tokens over several launches
+    for (int t0 = 0; t0 < T_; t0 += 65535) {
+      const int nt = std::min(65535, T_ - t0);
+      dim3 g2(grid.x, (unsigned)nt);
+      if (dtype_bf16)
+        (combine_kernel<bf16><<<g2, block, 0, stream>>>(static_cast<const bf16*>(y), pair_row + (int64_t)t0 * kk, nt,
+                                                        kk, H, static_cast<bf16*>(out) + (int64_t)t0 * H, T_dev, t0),
+         ::sb::count_launch());
+      else
+        (combine_kernel<f16><<<g2, block, 0, stream>>>(static_cast<const f16*>(y), pair_row + (int64_t)t0 * kk, nt,
+                                                       kk, H, static_cast<f16*>(out) + (int64_t)t0 * H, T_dev, t0),
+         ::sb::count_launch());
+    }
+  } else if (dtype_bf16) {
+    SB_CUDA_CHECK(launch_kernel(combine_kernel<bf16>, grid, block, 0, stream, pdl, static_cast<const bf16*>(y), pair_row,
+                                T_, kk, H, static_cast<bf16*>(out), T_dev, 0));
+    ::sb::count_launch();
+  } else {
+    SB_CUDA_CHECK(launch_kernel(combine_kernel<f16>, grid, block, 0, stream, pdl, static_cast<const f16*>(y), pair_row,
+                                T_, kk, H, static_cast<f16*>(out), T_dev, 0));
+    ::sb::count_launch();
+  }
+  SB_CUDA_CHECK(cudaGetLastError());
+  return STAGEML_OK;
+}
+
+int launch_combine_f32(const float* y, const int32_t* pair_row, int T_, int kk, int H, int dtype_bf16, void* out,
+                       cudaStream_t stream, bool pdl) {
+  SB_CHECK_ARG(H % 4 == 0, "combine: H=%d must be a multiple of 4", H);
+  if (T_ == 0 || H == 0) return STAGEML_OK;
+  const dim3 block(128), grid((unsigned)((H / 4 + block.x - 1) / block.x), (unsigned)std::min(T_, 65535));
   if (dtype_bf16)
-    return y_f32 ? run_combine<float, bf16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl)
-                 : run_combine<bf16, bf16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl);
-  return y_f32 ? run_combine<float, f16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl)
-               : run_combine<f16, f16>(y, pair_row, T_, kk, H, out, stream, T_dev, pdl);
+    SB_CUDA_CHECK(launch_kernel(combine_f32_kernel<bf16>, grid, block, 0, stream, pdl, y, pair_row, T_, kk, H,
+                                static_cast<bf16*>(out)));
+  else
+    SB_CUDA_CHECK(launch_kernel(combine_f32_kernel<f16>, grid, block, 0, stream, pdl, y, pair_row, T_, kk, H,
+                                static_cast<f16*>(out)));
+  ::sb::count_launch();
+  return STAGEML_OK;
 }
 
 int launch_validate_tenants(const int32_t* in, int64_t n, int n_tenants, int32_t* out, int32_t* status,

@@ -85,10 +85,13 @@ int launch_tc_shrink(const ShrinkLaunch& s, const void* rows, cudaStream_t strea
 int launch_pair_shrink(const ShrinkLaunch& s, const int32_t* pair_row, int64_t P, cudaStream_t stream,
                        bool pdl = false);
 
-// combine.cu: out[t] = sum_j Y[pair_row[t*kk + j]]; Y in out's 16-bit type, or in fp32 (y_f32)
+// combine.cu: out[t] = sum_j Y[pair_row[t*kk + j]]
 int launch_combine(const void* y, const int32_t* pair_row, int T, int kk, int H, int dtype_bf16, void* out,
                    cudaStream_t stream, const int32_t* T_dev = nullptr,  // rows >= *T_dev left untouched
-                   bool pdl = false, bool y_f32 = false);
+                   bool pdl = false);
+// The same from fp32 rows to 16-bit outputs.
+int launch_combine_f32(const float* y, const int32_t* pair_row, int T, int kk, int H, int dtype_bf16, void* out,
+                       cudaStream_t stream, bool pdl);
 // One-expert top-1 layer in token order: row_tenant[t] = validated tenant, row_scale[t] =
 // routing weight (1 without weights), both -1 / 0 with status for an expert id other
 // than 0 or a tenant out of range.
