@@ -122,6 +122,7 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
   g.N = a->I;
   g.swiglu = true;
   g.group_offsets = b.plan.group_offsets;
+  g.group_counts = b.plan.group_counts;
   g.q_out = b.hq;
   g.q_scale = b.hs;
   g.status = status;
@@ -131,7 +132,6 @@ int moe_blocks_impl(const stageml_moe_blocks_args* a, void* ws, size_t ws_bytes,
     sk.max_rows = moe_blocks_sparse(a) ? std::min(a->T, 8) : a->T;
     sk.row_map = b.plan.row_token;
     sk.tile_group = b.plan.tile_group;
-    sk.group_counts = b.plan.group_counts;
     sk.num_tiles = b.plan.num_tiles;
     sk.tiles_cap = (int)(b.plan.rows_cap / 128);
     g.out = b.h;

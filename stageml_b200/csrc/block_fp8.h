@@ -38,12 +38,13 @@ struct BlockGemmLaunch {
   int K = 0;
   int N = 0;                       // output columns
   bool swiglu = false;
-  // grouped rows (a MoE plan's padded rows): [groups + 1] row offsets, multiples of 128, at most
-  // block_gemm_max_groups() groups; null: plain rows, all of group 0
+  // grouped rows (a MoE plan's padded rows): [groups + 1] row offsets, multiples of 128, and [groups] rows without
+  // the padding; at most block_gemm_max_groups() groups. Null: plain rows, all of group 0
   const int32_t* group_offsets = nullptr;
+  const int32_t* group_counts = nullptr;
   const float* row_scale = nullptr;
   void* out = nullptr;             // [rows, N] out_dtype (plain)
-  int out_dtype = STAGEML_BF16;    // F32, BF16 or F16
+  int out_dtype = STAGEML_BF16;    // F32, BF16 or F16; grouped rows of block_gemm.cu: F32
   uint8_t* q_out = nullptr;        // [rows, N] e4m3 (swiglu)
   float* q_scale = nullptr;        // [rows, ceil(N/128)] (swiglu)
   int32_t* status = nullptr;
@@ -57,7 +58,6 @@ struct BlockSkinny {
   int max_rows = 0;  // plain rows: their number, at most kSkinnyRows; grouped: up to 8 or more per group expected
   const int32_t* row_map = nullptr;
   const int32_t* tile_group = nullptr;
-  const int32_t* group_counts = nullptr;
   const int32_t* num_tiles = nullptr;
   int tiles_cap = 0;
 };

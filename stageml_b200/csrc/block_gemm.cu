@@ -87,6 +87,7 @@ struct Params {
   const float* b_scale;
   int vec_scales;               // four scales of a row are one aligned 16-byte load
   const int32_t* group_offsets; // grouped rows: [groups + 1] padded row offsets; null: plain rows
+  const int32_t* group_counts;  // grouped rows: [groups] rows without the padding
   int groups;
   int64_t rows;
   const float* row_scale;
@@ -185,19 +186,22 @@ __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
 struct Unit {
   int m, n, group;  // m = first row tile
   int tiles;        // row tiles of the unit
+  int rows;         // grouped rows: without the padding of the group's last tile
 };
 
-// first[g] = row units of the groups before g, begin[g] = their row tiles (grouped rows), in shared
-// memory: read from global memory for each unit, they were 0.7 us of every role's unit. One warp.
+// first[g] = row units of the groups before g, begin[g] = 128 times their row tiles, plus the rows of padding
+// that end group g (less than 128; grouped rows), in shared memory: read from global memory for each unit,
+// they were 0.7 us of every role's unit. One warp.
 __device__ __forceinline__ void group_units(const Params& p, int step, int32_t* first, int32_t* begin) {
   const int lane = threadIdx.x & 31;
-  for (int g = lane; g <= p.groups; g += 32) begin[g] = p.group_offsets[g] / BM;
+  for (int g = lane; g <= p.groups; g += 32)
+    begin[g] = g < p.groups ? p.group_offsets[g + 1] - p.group_counts[g] : p.group_offsets[g];
   __syncwarp();
   int base = 0;
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
     const int g = g0 + lane;
     int c = 0;
-    if (g < p.groups) c = (begin[g + 1] - begin[g] + step - 1) / step;
+    if (g < p.groups) c = (begin[g + 1] / BM - begin[g] / BM + step - 1) / step;
     int s = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -213,9 +217,12 @@ __device__ __forceinline__ void group_units(const Params& p, int step, int32_t* 
 // Unit u -> row tiles and column tile. All column tiles of a weight group's row units (or of
 // a band of plain row units) come before the next group, row units fastest, so that the
 // CTAs at work at one time share weight tiles and the group's rows stay in L2.
+template <bool GROUPED>
 __device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const int32_t* first, const int32_t* begins) {
   Unit w;
-  if (p.group_offsets) {
+  // the pointer is always there for grouped rows; without the test the SwiGLU kernel is allocated otherwise and
+  // spills (64 experts of 2048 x 1408, 43 tokens: 206 us)
+  if (GROUPED && p.group_offsets) {
     const int r = u / p.n_tiles;
     int lo = 0, hi = p.groups - 1;  // the last group with first[g] <= r (empty groups are passed over)
     while (lo < hi) {
@@ -225,13 +232,14 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const 
       else
         hi = mid - 1;
     }
-    const int begin = begins[lo], tiles = begins[lo + 1] - begin;
+    const int begin = begins[lo] / BM, tiles = begins[lo + 1] / BM - begin;
     const int cnt = first[lo + 1] - first[lo], local = u - first[lo] * p.n_tiles;
     w.group = lo;
     w.n = local / cnt;
     const int m = (local - w.n * cnt) * step;
     w.m = begin + m;
     w.tiles = min(step, tiles - m);
+    w.rows = w.tiles * BM - (m + w.tiles == tiles ? begins[lo] % BM : 0);
   } else {
     const int tiles = (int)((p.rows + BM - 1) / BM), all = (tiles + step - 1) / step;
     const int band = u / (p.n_tiles * kBandUnits) * kBandUnits;
@@ -241,6 +249,7 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int step, const 
     const int m = (band + local - w.n * cnt) * step;
     w.m = m;
     w.tiles = min(step, tiles - m);
+    w.rows = 0;
   }
   return w;
 }
@@ -382,9 +391,9 @@ struct Columns {
   static constexpr int value = N;
 };
 
-// OutT: output element (plain); SWIGLU writes codes and ignores it. SPLITS pairs of a cluster share a
-// tile's K blocks; a cluster then has one tile.
-template <typename OutT, bool SWIGLU, int SPLITS>
+// OutT: output element (plain); SWIGLU writes codes and ignores it. GROUPED rows or plain ones. SPLITS pairs
+// of a cluster share a tile's K blocks; a cluster then has one tile.
+template <typename OutT, bool SWIGLU, bool GROUPED, int SPLITS>
 __global__ void __launch_bounds__(THREADS, 1)
     block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                            const __grid_constant__ CUtensorMap tm_b32, const Params p) {
@@ -437,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish_pair();
   }
-  if (warp == 2 && p.group_offsets) group_units(p, 2, first, begins);
+  if (GROUPED && warp == 2) group_units(p, 2, first, begins);
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
@@ -445,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem_base = *tmem_slot;
   volatile int never_abort = 0;
 
-  const int row_units = p.group_offsets ? first[p.groups] : (int)((p.rows + 2 * BM - 1) / (2 * BM));
+  const int row_units = GROUPED ? first[p.groups] : (int)((p.rows + 2 * BM - 1) / (2 * BM));
   const int units = row_units * p.n_tiles;
 
   if (warp >= MATH_WARP0) {
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t it = 0, grp = 0, tile = 0;
     bool ok = true, joined = false;
     for (int u = cluster; ok && u < units; u += clusters, ++tile) {
-      const Unit w = unit_of(p, u, 2, first, begins);
+      const Unit w = unit_of<GROUPED>(p, u, 2, first, begins);
       // One row tile: 64 rows per CTA, lanes 64..127 the same rows' later columns (`side`).
       const bool narrow = w.tiles == 1;
       const int side = narrow ? quarter >> 1 : 0;
@@ -552,9 +561,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) break;
       const int64_t row = narrow ? (int64_t)w.m * BM + 64 * rank + (row_in_tile & 63)
                                  : (int64_t)(w.m + rank) * BM + row_in_tile;
-      const bool row_ok = row < p.rows;
+      // The padding of fp32 rows is not stored (64 experts of 2048 x 1408, 128 tokens: 7 of 8 rows of the tiles);
+      // that of the codes is, a byte per value: their kernel has no register left for the row count.
+      const int64_t end = SWIGLU || !GROUPED ? p.rows : (int64_t)w.m * BM + w.rows;
+      const bool row_ok = row < end;
       const int64_t row4 = row - (lane & 3);  // the first of the four rows that four lanes store together
-      const int rows4 = (int)max((int64_t)0, min((int64_t)4, p.rows - row4));
+      const int rows4 = (int)max((int64_t)0, min((int64_t)4, end - row4));
       if (SWIGLU) {
         // a thread's 64 columns of h from its 64 gate and 64 up sums, or 32 of a narrow unit
         const int n0 = w.n * 128 + 64 * half + 32 * side;
@@ -667,7 +679,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t s = 0, phase = 0, filled = 0;  // filled: bit i = stage i has been filled
       bool ok = true;
       for (int u = cluster; ok && u < units; u += clusters) {
-        const Unit w = unit_of(p, u, 2, first, begins);
+        const Unit w = unit_of<GROUPED>(p, u, 2, first, begins);
         const int n0 = w.n * (SWIGLU ? 128 : BN);
         // B rows of half 0; half 1 is `next` rows on
         const int b0 = w.group * p.b_group_rows + n0 + rank * (SWIGLU ? p.N : 64);
@@ -719,7 +731,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t s = 0, phase = 0, it = 0;
       bool ok = true;
       for (int u = cluster; ok && u < units; u += clusters) {
-        const uint32_t idesc = unit_of(p, u, 2, first, begins).tiles == 1 ? idesc_e4m3(BM, NACC) : idesc_e4m3(2 * BM, NACC);
+        const uint32_t idesc = unit_of<GROUPED>(p, u, 2, first, begins).tiles == 1 ? idesc_e4m3(BM, NACC) : idesc_e4m3(2 * BM, NACC);
         for (int kb = 0; kb < kb_count; ++kb, ++it) {
           const uint32_t buf = (it & 1) * 2 + half;
           ok = lane_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, full_bar(s), phase, abort_flag, p.status, kDevTimeoutMma);
@@ -747,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t grp = 0;
     bool ok = true;
     for (int u = cluster; ok && u < units; u += clusters) {
-      const Unit w = unit_of(p, u, 2, first, begins);
+      const Unit w = unit_of<GROUPED>(p, u, 2, first, begins);
       // slots 32 i + lane: the CTA's rows in order, or a narrow unit's 64 rows twice
       const bool narrow = w.tiles == 1;
       const int64_t row0 = (narrow ? (int64_t)w.m * BM + 64 * rank : (int64_t)(w.m + rank) * BM) + lane;
@@ -798,10 +810,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <typename OutT, bool SWIGLU, int SPLITS = 1>
+template <typename OutT, bool SWIGLU, bool GROUPED, int SPLITS = 1>
 int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb32, const Params& p, int clusters, bool pdl,
              cudaStream_t stream) {
-  auto kernel = block_gemm_pair_kernel<OutT, SWIGLU, SPLITS>;
+  auto kernel = block_gemm_pair_kernel<OutT, SWIGLU, GROUPED, SPLITS>;
   SB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * SPLITS * clusters);
@@ -824,9 +836,9 @@ int run_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb
 template <typename OutT>
 int run_plain(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int clusters, int splits, bool pdl,
               cudaStream_t stream) {
-  if (splits == 4) return run_pair<OutT, false, 4>(ta, tb, tb, p, clusters, pdl, stream);
-  if (splits == 2) return run_pair<OutT, false, 2>(ta, tb, tb, p, clusters, pdl, stream);
-  return run_pair<OutT, false>(ta, tb, tb, p, clusters, pdl, stream);
+  if (splits == 4) return run_pair<OutT, false, false, 4>(ta, tb, tb, p, clusters, pdl, stream);
+  if (splits == 2) return run_pair<OutT, false, false, 2>(ta, tb, tb, p, clusters, pdl, stream);
+  return run_pair<OutT, false, false>(ta, tb, tb, p, clusters, pdl, stream);
 }
 
 // Clusters of SPLITS pairs that the device runs at one time (not all of its SMs: a cluster lies in
@@ -837,7 +849,7 @@ int resident_clusters() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if ((n = known[dev].load(std::memory_order_relaxed)) != 0) return n;
-  auto kernel = block_gemm_pair_kernel<bf16, false, SPLITS>;
+  auto kernel = block_gemm_pair_kernel<bf16, false, false, SPLITS>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * SPLITS);
   cfg.blockDim = dim3(THREADS);
@@ -873,6 +885,8 @@ int block_gemm_max_groups() { return MAX_GROUPS; }
 
 int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   if (g.a_rows == 0 || g.N == 0) return STAGEML_OK;
+  SB_CHECK_ARG(!g.swiglu || g.group_offsets, "block_gemm: SwiGLU rows are grouped");
+  SB_CHECK_ARG(g.swiglu || !g.group_offsets || g.out_dtype == STAGEML_F32, "block_gemm: grouped rows leave in fp32");
   Params p{};
   p.K = g.K;
   p.N = g.N;
@@ -883,6 +897,7 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
   p.a_scale = g.a_scale;
   p.b_scale = g.b_scale;
   p.group_offsets = g.group_offsets;
+  p.group_counts = g.group_counts;
   p.groups = g.groups;
   p.rows = g.a_rows;
   p.row_scale = g.row_scale;
@@ -909,8 +924,9 @@ int launch_block_gemm(const BlockGemmLaunch& g, cudaStream_t stream) {
     CUtensorMap tb32;  // a narrow unit's runs of 32 gate or up rows
     SB_TRY(make_tmap_2d(&tb32, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)g.groups * p.b_group_rows, (uint64_t)g.K,
                         (uint64_t)g.K, 32, BK, 128));
-    return run_pair<bf16, true>(ta, tb, tb32, p, clusters, g.pdl, stream);
+    return run_pair<bf16, true, true>(ta, tb, tb32, p, clusters, g.pdl, stream);
   }
+  if (g.group_offsets) return run_pair<float, false, true>(ta, tb, tb, p, clusters, g.pdl, stream);
   if (g.out_dtype == STAGEML_F32) return run_plain<float>(ta, tb, p, clusters, splits, g.pdl, stream);
   if (g.out_dtype == STAGEML_BF16) return run_plain<bf16>(ta, tb, p, clusters, splits, g.pdl, stream);
   return run_plain<f16>(ta, tb, p, clusters, splits, g.pdl, stream);

@@ -220,7 +220,7 @@ int launch_block_skinny(const BlockGemmLaunch& g, const BlockSkinny& s, cudaStre
   p.units_n = (g.N + kUnitRows - 1) / kUnitRows;
   p.rows = s.max_rows;
   p.tile_group = s.tile_group;
-  p.group_counts = s.group_counts;
+  p.group_counts = g.group_counts;
   p.group_offsets = g.group_offsets;
   p.num_tiles = s.num_tiles;
   p.tiles_cap = s.tiles_cap;
