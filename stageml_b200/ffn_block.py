@@ -170,8 +170,14 @@ class FeedForwardBlock(torch.nn.Module):
     def experts(self, normed):
         """The routed experts' output for normed [..., H]; differentiable in normed and router_w."""
         rows = normed.reshape(-1, normed.shape[-1]).contiguous()
-        ids, weights, _ = _Route.apply(rows, self.router_w.float(), self.k)
-        y = _Experts.apply(rows, weights, ids, self.gate_up, self.gate_up_scale, self.down, self.down_scale, self.n_shared)
+        router_w = self.router_w.float()
+        codes = (self.gate_up, self.gate_up_scale, self.down, self.down_scale)
+        if torch.is_grad_enabled() and (rows.requires_grad or router_w.requires_grad):
+            ids, weights, _ = _Route.apply(rows, router_w, self.k)
+            y = _Experts.apply(rows, weights, ids, *codes, self.n_shared)
+        else:  # decoding: without the autograd functions' host code
+            ids, weights, _ = ops.route_topk(rows, router_w, self.k)
+            y = ops.moe_forward_blocks(rows, *codes, topk_ids=ids, topk_weights=weights, n_shared=self.n_shared)
         return y.view(normed.shape)
 
     def forward(self, residual, normed, next_pre_weight=None):

@@ -113,6 +113,17 @@ def test_gradient_is_the_same_every_run(ops):
         assert torch.equal(a, grads[0][0]) and torch.equal(b, grads[0][1])
 
 
+def test_the_same_with_and_without_grad_mode(ops):
+    block = make_block()
+    x = randn(9, H, seed=104, dtype=BF16)
+    want = block.experts(x)
+    assert want.requires_grad
+    with torch.no_grad():
+        assert torch.equal(block.experts(x), want.detach())
+    block.requires_grad_(False)
+    assert not block.experts(x).requires_grad and block.experts(x.clone().requires_grad_(True)).requires_grad
+
+
 def test_state_holds_the_experts(ops):
     a, b = make_block(seed=80), make_block(seed=140)
     names = {"gate_up", "gate_up_scale", "down", "down_scale"}
