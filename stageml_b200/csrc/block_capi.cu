@@ -28,20 +28,23 @@ struct MoeBlocksBuffers {
 };
 
 // Streaming products take 8 or 16 rows of a weight group per pass over its weights. 8: four routed rows per
-// expert or fewer, few experts have more than eight (64 experts, six of them and two shared, 16 tokens: 151 us
-// in passes of 8, 174 in passes of 16). Shared experts alone have one row per token: 16.
+// expert or fewer, few experts have more than eight (64 experts, six of them and two shared, 16 tokens: 148 us
+// in passes of 8, 169 in passes of 16). Shared experts alone have one row per token: 16.
 bool moe_blocks_sparse(const stageml_moe_blocks_args* a) { return a->k > 0 && (int64_t)a->T * a->k <= 4 * (int64_t)a->E; }
 
 // Streaming products instead of tensor-core tiles, whose time is the same for any number of rows up to
-// 128 per expert: up to kSkinnyRows tokens, and up to two routed rows per expert. 64 experts of 2048 x
-// 1408, two of them, 17, 32, 48, 64 tokens: 94, 130, 146, 156 us streamed, 124, 155, 171, 180 in tiles.
-// A shared expert has a row per token, and its passes come one after the other: with one, 107, 136, 162, 188
-// us streamed, 128, 154, 162, 184 in tiles; with four, 122, 167, 202, 238 and 131, 160, 177, 193. So 32 tokens
-// are the most beside shared experts, and 16 without routed ones (one of 4096 x 14336, 16 and 32 tokens: 75 and
-// 119 us streamed, 99 in tiles).
+// 128 per expert: up to kSkinnyRows tokens, and up to 128 routed rows, two per expert. Streamed and in tiles, us:
+//   64 experts of 2048 x 1408, two of them, 17, 32, 48, 64 tokens      88, 137, 147, 162    110, 144, 158, 173
+//   128 of 2048 x 768, four of them, 17, 32, 64                        107, 161, 212        123, 161, 208
+//   256 of 2048 x 768, eight of them, 16, 17, 32                       197, 205, 287        200, 202, 267
+// A shared expert has a row per token, and its passes come one after the other:
+//   64 experts as above and one shared, 17, 24, 32, 64                 100, 110, 146, 191   116, 120, 144, 175
+//   and four shared                                                    113, 139, 152, 236   119, 136, 143, 179
+//   one shared of 4096 x 14336 alone, 8, 16, 17, 32                    60, 76, 108, 119     96, 97, 97, 96
+// so 24 tokens are the most beside shared experts, and 16 without routed ones.
 bool moe_blocks_skinny(const stageml_moe_blocks_args* a) {
   if (a->T <= kSkinnyRows) return true;
-  return a->k > 0 && a->T <= (a->n_shared > 0 ? 32 : 128) && (int64_t)a->T * a->k <= 2 * (int64_t)a->E;
+  return a->k > 0 && (a->n_shared == 0 || a->T <= 24) && (int64_t)a->T * a->k <= std::min<int64_t>(128, 2 * (int64_t)a->E);
 }
 
 void moe_blocks_carve(const stageml_moe_blocks_args* a, void* ws, MoeBlocksBuffers* b) {

@@ -12,9 +12,10 @@ P = 4096  # a non-null, 16-byte aligned address; never dereferenced
 
 @pytest.mark.parametrize("t,e,k,shared,streams", [
     (1, 8, 2, 0, True), (16, 8, 2, 0, True), (16, 0, 0, 1, True),  # up to 16 tokens
-    (17, 8, 2, 0, False), (64, 64, 2, 0, True), (65, 64, 2, 0, False), (129, 256, 1, 0, False),  # two rows per expert
+    (17, 8, 2, 0, False), (64, 64, 2, 0, True), (65, 64, 2, 0, False),  # two rows per expert
+    (128, 256, 1, 0, True), (129, 256, 1, 0, False), (32, 128, 4, 0, True), (33, 128, 4, 0, False),  # 128 routed rows
     (17, 0, 0, 1, False), (64, 0, 0, 2, False), (128, 0, 0, 1, False),  # shared experts alone have a row per token
-    (32, 64, 2, 1, True), (33, 64, 2, 1, False), (64, 64, 2, 1, False), (128, 256, 2, 1, False),
+    (24, 64, 2, 1, True), (25, 64, 2, 1, False), (64, 64, 2, 1, False), (128, 256, 2, 1, False),
 ])
 def test_layer_streams_its_weights_for_few_rows_only(t, e, k, shared, streams):
     """Streaming passes over an expert's weights once per 8 or 16 of its rows, tensor-core tiles once. The workspace
