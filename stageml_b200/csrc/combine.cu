@@ -3,6 +3,8 @@
 // out.index_add_(0, index, y * gates) of RequestExecutor.dynamic_one
 // (benchmarks/multitenant_bta_system_bench.py:413) done once per token with a
 // fixed slot order (fp32 sum, one rounding), so it is deterministic.
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_util.h"
 #include "kernels.h"
@@ -33,31 +35,42 @@ __global__ void combine_kernel(const T* __restrict__ y, const int32_t* __restric
   *reinterpret_cast<uint4*>(out + (int64_t)t * H + c) = pack8<T>(acc);
 }
 
-// The same from fp32 rows, 4 columns per thread: a warp's load is 512 bytes in a row, and up to eight slots' loads
-// are on their way at once (4096 tokens of 2048 columns, eight slots each: 104 us with one 8-column slot at a time).
-template <typename T>
-__global__ void combine_f32_kernel(const float* __restrict__ y, const int32_t* __restrict__ pair_row, int T_, int kk, int H,
-                                   T* __restrict__ out) {
-  constexpr int kSlots = 8;
+// The same from fp32 rows: 4 columns per lane, so that a warp's load is 512 bytes in a row, and eight loads on their
+// way at once: SLOTS slots of a token (more go in turns) and 8 / SLOTS column groups per thread. One 8-column slot at a
+// time took 104 us for 4096 tokens of 2048 columns with eight slots, and eight slots for two 22, not 17, for 2048 x 4096.
+template <typename T, int SLOTS>
+__global__ void __launch_bounds__(128) combine_f32_kernel(const float* __restrict__ y, const int32_t* __restrict__ pair_row,
+                                                          int T_, int kk, int H, T* __restrict__ out) {
+  constexpr int GROUPS = 8 / SLOTS;
   pdl_wait();  // y comes from the previous kernel
-  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
-  if (c >= H) return;
+  const int c = (blockIdx.x * GROUPS * blockDim.x + threadIdx.x) * 4, step = 4 * blockDim.x;
   for (int t = blockIdx.y; t < T_; t += gridDim.y) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j0 = 0; j0 < kk; j0 += kSlots) {
-      float4 v[kSlots];
+    float4 acc[GROUPS];
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) {
+    for (int g = 0; g < GROUPS; ++g) acc[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 < kk; j0 += SLOTS) {
+      float4 v[SLOTS][GROUPS];
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j) {
         const int row = j0 + j < kk ? __ldg(pair_row + (int64_t)t * kk + j0 + j) : -1;
-        v[j] = row >= 0 ? __ldg(reinterpret_cast<const float4*>(y + (int64_t)row * H + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* src = y + (int64_t)row * H + c;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+          v[j][g] = row >= 0 && c + g * step < H ? __ldg(reinterpret_cast<const float4*>(src + g * step))
+                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) acc[0] += v[j].x, acc[1] += v[j].y, acc[2] += v[j].z, acc[3] += v[j].w;
-    }
-    T h[4];
+      for (int j = 0; j < SLOTS; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = from_f32<T>(acc[i]);
-    *reinterpret_cast<uint2*>(out + (int64_t)t * H + c) = *reinterpret_cast<const uint2*>(h);
+        for (int g = 0; g < GROUPS; ++g)
+          acc[g].x += v[j][g].x, acc[g].y += v[j][g].y, acc[g].z += v[j][g].z, acc[g].w += v[j][g].w;
+    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      if (c + g * step >= H) break;
+      const T h[4] = {from_f32<T>(acc[g].x), from_f32<T>(acc[g].y), from_f32<T>(acc[g].z), from_f32<T>(acc[g].w)};
+      *reinterpret_cast<uint2*>(out + (int64_t)t * H + c + g * step) = *reinterpret_cast<const uint2*>(h);
+    }
   }
 }
 
@@ -162,15 +175,20 @@ int launch_combine_f32(const float* y, const int32_t* pair_row, int T_, int kk, 
                        cudaStream_t stream, bool pdl) {
   SB_CHECK_ARG(H % 4 == 0, "combine: H=%d must be a multiple of 4", H);
   if (T_ == 0 || H == 0) return STAGEML_OK;
-  const dim3 block(128), grid((unsigned)((H / 4 + block.x - 1) / block.x), (unsigned)std::min(T_, 65535));
-  if (dtype_bf16)
-    SB_CUDA_CHECK(launch_kernel(combine_f32_kernel<bf16>, grid, block, 0, stream, pdl, y, pair_row, T_, kk, H,
-                                static_cast<bf16*>(out)));
-  else
-    SB_CUDA_CHECK(launch_kernel(combine_f32_kernel<f16>, grid, block, 0, stream, pdl, y, pair_row, T_, kk, H,
-                                static_cast<f16*>(out)));
-  ::sb::count_launch();
-  return STAGEML_OK;
+  auto run = [&](auto* o, auto slots) {
+    using T = std::remove_pointer_t<decltype(o)>;
+    constexpr int SLOTS = decltype(slots)::value, COLS = 128 * 4 * (8 / SLOTS);
+    const dim3 grid((unsigned)((H + COLS - 1) / COLS), (unsigned)std::min(T_, 65535));
+    SB_CUDA_CHECK(launch_kernel(combine_f32_kernel<T, SLOTS>, grid, dim3(128), 0, stream, pdl, y, pair_row, T_, kk, H, o));
+    ::sb::count_launch();
+    return (int)STAGEML_OK;
+  };
+  auto slots_for = [&](auto* o) {
+    if (kk <= 2) return run(o, std::integral_constant<int, 2>{});
+    if (kk <= 4) return run(o, std::integral_constant<int, 4>{});
+    return run(o, std::integral_constant<int, 8>{});
+  };
+  return dtype_bf16 ? slots_for(static_cast<bf16*>(out)) : slots_for(static_cast<f16*>(out));
 }
 
 int launch_validate_tenants(const int32_t* in, int64_t n, int n_tenants, int32_t* out, int32_t* status,
