@@ -23,16 +23,16 @@
 // A unit of one row tile (a short batch, the odd last tile of an expert) is narrow: 64 rows per CTA,
 // MMAs of M = 128, whose accumulators hold columns [0, 64) of a half in lanes 0..63 and [64, 128) in
 // lanes 64..127: 64 sums per thread, half the work of a pair with an idle CTA. 64 experts of 2048 x
-// 1408 with at most 128 rows each in 197 us, from 250; 64 x 4096 x 4096 in 12 us, from 15.
+// 1408 with at most 128 rows each in 195 us (two CTAs per tile: 250); 64 x 4096 x 4096 in 11.5 us.
 //
 // SwiGLU: half h of a tile is 64 gate rows and the matching 64 up rows of B, so a thread
 // holds the gate and up values of the same columns; the epilogue forms
 // h = silu(gate) * up in fp32 and writes it as e4m3 codes with one scale per (row, 128
 // columns), the next product's operand, so h never exists in 16 bits.
 //
-// Measured: 2048 x 11008 x 4096 in 91 us (2.0 PFLOP/s) alone and 110 us (1.7) in a run of them, where
-// the board's 1 kW holds the clock at 1.65 GHz; the accumulator round trip and then power bound it,
-// the tensor pipe is active half of the time.
+// Measured: 2048 x 11008 x 4096 in 103 to 109 us (1.7 to 1.8 PFLOP/s) in a run of calls, where the board's
+// 1 kW holds the clock at 1.65 GHz, 92 us (2.0) in short ones; the accumulator round trip and then power bound
+// it, the tensor pipe is active half of the time.
 //
 // Plain products of few tiles: clusters of two or four pairs, each with its share of a tile's K blocks;
 // the sums meet over distributed shared memory, in a fixed order, and each pair stores its share of
@@ -869,9 +869,9 @@ int resident_clusters() {
 
 // Pairs per tile: where the tiles leave SMs idle, several pairs share a tile's K blocks. A K block
 // takes a pair 0.25 (narrow units) to 0.4 us on an idle device and the exchange 1.5 to 2 us, so two pairs
-// pay from 12 blocks on (64 x 4096 outputs over 8, 12, 32, 112 blocks: 8.2, 9.5, 14.9, 36.0 us alone, 8.2,
-// 9.1, 12.2, 23.0 in two) and four from 24 (300 x 1000 over 12, 16, 32: 11.4, 12.2, 15.6 in two, 12.1,
-// 12.4, 14.3 in four), while all clusters run at one time (64 x 4096 in 16 clusters of eight CTAs took two
+// pay from 12 blocks on (64 x 4096 outputs over 8, 12, 32, 112 blocks: 7.5, 8.9, 14.7, 38.6 us alone, 7.6,
+// 8.5, 11.5, 23.9 in two) and four from 24 (300 x 1000 over 16, 24, 32: 11.2, 12.8, 14.5 in two, 11.6,
+// 12.6, 13.3 in four), while all clusters run at one time (64 x 4096 in 16 clusters of eight CTAs took two
 // turns: 25 us, not 15).
 int splits_for(int64_t units, int kb) {
   if (kb >= 24 && units <= resident_clusters<4>()) return 4;

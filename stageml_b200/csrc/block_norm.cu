@@ -35,10 +35,10 @@
 // that owns the column. Each CTA takes every gridDim-th row and writes its sums once; a second
 // kernel adds them in CTA order: no atomics, the same bits on every run.
 //
-// Bound: HBM for the forward (8192 x 4096 bf16 in 45 us, 268 MB: 6.0 TB/s); the backward (112 us,
-// 336 MB, 3.0 TB/s) by the issue slots, 70 % of which its arithmetic takes: two norms recomputed and
+// Bound: HBM for the forward (8192 x 4096 bf16 in 45 us, 268 MB: 6.0 TB/s); the backward (109 us,
+// 336 MB, 3.1 TB/s) by the issue slots, 70 % of which its arithmetic takes: two norms recomputed and
 // two differentiated per element. Widths that are not multiples of 8 take scalar loads (777 x 2047,
-// fp32 stream: forward 8, backward 17 us) and beyond 4096 columns more registers than there are.
+// fp32 stream: forward 8, backward 19 us) and beyond 4096 columns more registers than there are.
 #include <atomic>
 
 #include "block_codes.cuh"

@@ -11,10 +11,10 @@
 // for both operands, so nothing is shuffled. Rows are the N side (8 or 16 of them). The
 // matrix unit is far from its limit here; tcgen05 would only add its set-up time: the same
 // 1 x 4096 x 4096 product took 18 us on the pair kernel, bound by one accumulator round trip
-// per K block, and takes 5 here. Measured over 64 experts of 2048 x 1408 with six per token: 8, 16
-// and 32 tokens in 114, 163 and 197 us, weights at 3.5 to 4 TB/s. Loading the next unit's weights
-// before the sums of this one meet was no faster (111, 159 and 191 us) and slowed long
-// rows down (8 experts of 4096 x 14336, 8 tokens: 319 us, not 293).
+// per K block, and takes 5 here. Measured over 64 experts of 2048 x 1408 with six per token and two
+// shared: 8, 16 and 21 tokens in 113, 149 and 170 us, weights at 3.5 to 4 TB/s. Loading the next unit's
+// weights before the sums of this one meet was no faster (111 us, not 114, for 8 tokens at the time) and
+// slowed long rows down (8 experts of 4096 x 14336, 8 tokens: 319 us, not 293).
 #include "block_fp8.h"
 #include "common.cuh"
 #include "host_util.h"

@@ -52,7 +52,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t c, int64_t col
 // Rows of whole blocks, in place: block u of the flattened tensor starts at 128 u and no row
 // index is needed. 8 lanes per block, 16 values each: the scale and the shuffles, which every
 // lane pays for per block, weigh half of what they do with 16 lanes (8192 x 4096 bf16 values:
-// 26.6 us with 16 lanes, 20.4 with 8, 5.0 TB/s; instructions bound the former, not HBM). All
+// 26.6 us with 16 lanes, 21 with 8, 4.8 TB/s; instructions bound the former, not HBM). All
 // blocks of a round are loaded before the first is encoded.
 constexpr int kFlat = 2;
 template <typename T>
