@@ -286,3 +286,53 @@ def test_products_on_two_streams_at_once(ops):
         for outs in g:
             for a, b in zip(outs, ref):
                 assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+def test_norm_rows_past_32_bits(ops):
+    """2.3e9 values: the last rows are those of the same rows alone, outputs and gradients."""
+    t, h, n = 140000, 16384, 300
+    g = torch.Generator(device=DEV).manual_seed(70)
+    r, y, dr, dz = (torch.empty(t, h, device=DEV, dtype=BF16).normal_(generator=g) for _ in range(4))
+    pre, post = 1 + randn(h, seed=71, scale=0.1), 1 + randn(h, seed=72, scale=0.1)
+    args = dict(post_weight=post, pre_weight=pre)
+    tail = {"y": y[-n:], "r": r[-n:], "post": post, "gate": None, "pre": pre}
+    new, z = ops.norm_residual(y, r, **args)
+    _, q, s = ops.norm_residual(y, r, quantize=True, **args)
+    rn, rz, ref = ref_norm(tail, 1.0, 1e-6, (dr[-n:], dz[-n:]))
+    close(new[-n:], rn), close(z[-n:], rz)
+    assert float((dequant(q[-n:], s[-n:], 1) - rz).norm() / rz.norm()) < 0.04  # half a step of e4m3 at most: 2^-4
+    del new, z, q, s
+    d = ops.norm_residual_backward(dr, dz, y, r, **args)
+    close(d[0][-n:], ref["r"]), close(d[1][-n:], ref["y"])
+
+
+def test_layer_rows_past_32_bits(ops):
+    """560000 slots of 4096 columns: the fp32 rows that are summed lie past 2^31 values; tokens of both ends."""
+    t, e, k, h, i = 70000, 16, 8, 4096, 128
+    gu, gus, dn, dns = layer_weights(e, h, i, seed=73)
+    x = randn(t, h, seed=74, dtype=BF16)
+    ids = torch.rand(t, e, generator=torch.Generator(device=DEV).manual_seed(75), device=DEV).topk(k, 1).indices.to(torch.int32)
+    w = torch.rand(t, k, generator=torch.Generator(device=DEV).manual_seed(76), device=DEV)
+    y = ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w)
+    for part in (slice(0, 100), slice(t - 100, t)):
+        close(y[part], ref_layer(x[part], gu, gus, dn, dns, ids[part], w[part], 0), LAYER_TOL[BF16])
+
+
+def test_balance_logits_past_32_bits(ops):
+    t, e = 8500000, 256  # 2.2e9 logits
+    g = torch.Generator(device=DEV).manual_seed(77)
+    logits = torch.empty(t, e, device=DEV, dtype=BF16).normal_(generator=g)
+    ids = torch.randint(0, e, (t, 1), generator=g, device=DEV, dtype=torch.int32)
+    loss, counts, tokens = ops.balance_loss(logits, ids)
+    assert int(tokens) == t and torch.equal(counts.long(), torch.bincount(ids.view(-1), minlength=e))
+    p = torch.zeros(e, dtype=torch.float64, device=DEV)
+    for lo in range(0, t, 500000):
+        p += torch.softmax(logits[lo:lo + 500000].double(), 1).sum(0)
+    f = counts.double() / t
+    # fp32 partial sums of about 150 tokens' probabilities per lane, then 3500 of those: sqrt(3500) * 2^-24
+    close(loss, e * (f * p / t).sum())
+    grad = ops.balance_loss_backward(torch.full((), 1e6, device=DEV), logits, counts, tokens, 1)
+    x = torch.softmax(logits[-200:].double(), 1)
+    ref = 1e6 * e / t * x * (f - (x * f).sum(1, keepdim=True))
+    close(grad[-200:], ref)
