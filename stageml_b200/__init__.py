@@ -6,7 +6,8 @@ The public surface mirrors the reference package ``stageml`` for this path:
 ``adapter_cache``, ``moe_lora_layers``, ``custom_op_registry`` and
 ``vllm_stage_router``. Their CUDA inputs run on hand-written sm_100a kernels
 behind the C ABI in ``include/stageml_b200.h`` (``ops`` is the thin Python
-layer over it). Importing the package does not touch CUDA; the native
+layer over it); ``ffn_block`` is the feed-forward sublayer on block-scaled FP8
+weights, which the reference does not have. Importing the package does not touch CUDA; the native
 libraries load on first use of ``stageml_b200.ops``.
 """
 
