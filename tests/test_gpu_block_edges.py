@@ -77,6 +77,18 @@ def test_shared_experts_alone(ops, t, shared):
           ref_layer(x, gu, gus, dn, dns, None, None, shared), LAYER_TOL[BF16])
 
 
+@pytest.mark.parametrize("t,e", [(8, 64), (40, 64), (200, 8), (3000, 64)])
+def test_layer_same_bits_every_run(ops, t, e):
+    h, i, k = 512, 272, 6
+    gu, gus, dn, dns = layer_weights(e + 1, h, i, seed=80)
+    x = randn(t, h, seed=81, dtype=BF16)
+    top = randn(t, e, seed=82).topk(k, 1)
+    ids, w = top.indices.to(torch.int32), top.values.softmax(1)
+    first = ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w, n_shared=1)
+    for _ in range(5):
+        assert torch.equal(ops.moe_forward_blocks(x, gu, gus, dn, dns, topk_ids=ids, topk_weights=w, n_shared=1), first)
+
+
 # ------------------------------------------------------------------ gradients that are not there
 @pytest.mark.parametrize("constant", [False, True])
 def test_second_order_gradients_are_refused(ops, constant):
